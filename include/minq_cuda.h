@@ -441,6 +441,113 @@ minq_status minq_generate_sampled(minq_model* m, minq_sampler* s, const uint32_t
                                   minq_token_cb on_token, void* user, uint32_t* tokens_out,
                                   minq_gen_stats* stats);
 
+/* ---------------------------------------------------------------------- */
+/* Serving step over a paged 4-bit K/V cache (no reference counterpart: the  */
+/* reference's KVCache, model.rs:100-131, is one contiguous f32 history).    */
+/*                                                                           */
+/* A pool of pages holds the keys (another the values) of one layer:         */
+/*   [n_pages][n_kv][page_size][head_dim / 32] Q4_0 blocks                    */
+/* (quantize.rs:120-143, 20 bytes per 32 values: 6.4 times smaller than f32); */
+/* page_size is a power of two in 16..1024. Slot s is position s % page_size  */
+/* of page s / page_size. Request r's position i lies in page                 */
+/* table[r * table_stride + i / page_size]. One step of a batch: extend the   */
+/* tables, write each layer's new keys and values, attend, and draw a token   */
+/* per row. All calls are asynchronous on `stream`, keep no state, and may be  */
+/* captured into a CUDA graph. All pointers are device memory.                */
+
+/* What a pages call found (info[0]): 0, or the bits below. A call that finds
+ * anything changes neither tables nor lengths nor the free list. */
+enum {
+  MINQ_PAGES_SHORT = 1,           /* too few free pages: info[1] more are needed */
+  MINQ_PAGES_ROW_FULL = 2,        /* a request does not fit its table row */
+  MINQ_PAGES_TOO_MANY_TOKENS = 4, /* more new tokens than max_tokens */
+  MINQ_PAGES_BAD_LENGTH = 8,      /* a negative length */
+  MINQ_PAGES_BAD_PAGE = 16        /* a page id or free count outside the pool */
+};
+
+/* Grow request r (n_req <= 8192) from lens[r] to lens[r] + new_tokens[r]
+ * positions. The step's new pages, numbered j in the order (request,
+ * position), are free_pages[*n_free - 1 - j] and go into `table`;
+ * q_start [n_req + 1] gets the running sum of new_tokens, and for token t of
+ * request r slots[t] (t < max_tokens) its slot and positions[t] (or NULL) its
+ * position lens[r] + t - q_start[r]. Tokens behind the last one get slot -1
+ * and position 0. lens_out [n_req] and n_free_out [1] may be lens and n_free
+ * (in place); free_pages is not changed. info [2]. When something was found
+ * the step is empty: q_start all 0, slots all -1, lens_out = lens. */
+minq_status minq_pages_extend(const int32_t* lens, const int32_t* new_tokens, size_t n_req,
+                              size_t page_size, int32_t* table, size_t table_stride,
+                              const int32_t* free_pages, size_t n_pages, const int32_t* n_free,
+                              size_t max_tokens, int32_t* lens_out, int32_t* n_free_out,
+                              int32_t* q_start, int64_t* slots, int32_t* positions, int32_t* info,
+                              void* stream);
+
+/* Cut request r to min(lens[r], keep[r]) positions (0: it ended) and put its
+ * pages back on top of the free list (capacity n_pages), in the order that
+ * undoes an extend. Table entries beyond the new length stay as they are. */
+minq_status minq_pages_trim(const int32_t* lens, const int32_t* keep, size_t n_req,
+                            size_t page_size, const int32_t* table, size_t table_stride,
+                            int32_t* free_pages, size_t n_pages, const int32_t* n_free,
+                            int32_t* lens_out, int32_t* n_free_out, int32_t* info, void* stream);
+
+/* Quantise the rows of n_tokens tokens into the pools: token t's keys are
+ * [n_kv][head_dim] at k + t * k_stride (floats), its values at
+ * v + t * v_stride; codes are bit-identical to minq_quantize(MINQ_Q4_0).
+ * A slot outside the pool (the padding's -1) is skipped. Slots inside it must
+ * be distinct: the content of one that is named twice is unspecified.
+ * head_dim: a multiple of 32 up to 256; pools 16-byte aligned. */
+minq_status minq_kv4_write(const float* k, const float* v, size_t k_stride, size_t v_stride,
+                           const int64_t* slots, size_t n_tokens, size_t n_kv, size_t head_dim,
+                           void* k_pages, void* v_pages, size_t n_pages, size_t page_size,
+                           void* stream);
+
+/* The values that the rows at `slots` stand for, in minq_kv4_write's layout
+ * (zeros for a slot outside the pool). */
+minq_status minq_kv4_read(const void* k_pages, const void* v_pages, size_t n_pages,
+                          size_t page_size, const int64_t* slots, size_t n_tokens, size_t n_kv,
+                          size_t head_dim, float* k, float* v, size_t k_stride, size_t v_stride,
+                          void* stream);
+
+/* Causal attention (model.rs:223-248) of the step's tokens over the pools.
+ * lens [n_req] are the lengths with the step's tokens, whose keys and values
+ * are already written: token t of request r (q_start[r] <= t <
+ * q_start[r + 1]) sits at position i = lens[r] - (q_start[r + 1] - t) and
+ * attends over positions 0..=i. q: token t, head h at
+ * q + t * q_stride + h * head_dim (RoPE'd); out likewise, f32. Scores are
+ * scaled by `scale` (1 / sqrt(head_dim) in the reference). A row that sees
+ * nothing is zero; positions in a page whose id is outside the pool, or past
+ * the table row, are not seen; rows behind q_start[n_req] are left as they
+ * were. Any n_req <= 8192, n_tokens <= 2^24, n_heads a multiple of n_kv,
+ * head_dim a multiple of 32 up to 256. `workspace` (16-byte aligned) holds
+ * minq_kv4_attend_workspace_bytes(...) bytes, needs no initial value, and
+ * must not be shared by calls that may overlap. */
+size_t minq_kv4_attend_workspace_bytes(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv,
+                                       size_t head_dim);
+minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_start,
+                            size_t n_tokens, const int32_t* lens, size_t n_req,
+                            const int32_t* table, size_t table_stride, const void* k_pages,
+                            const void* v_pages, size_t n_pages, size_t page_size, size_t n_heads,
+                            size_t n_kv, size_t head_dim, float scale, float* out,
+                            size_t out_stride, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* One token per row of logits from the row's uniform (Sampler::sample,
+ * sampler.rs:47-109, batched, with min-p and without a random state). Row r
+ * is n floats at logits + r * row_stride; temperature (NULL: 1; <= 0:
+ * greedy), top_k (NULL or <= 0: off), top_p (NULL or >= 1: off), min_p (NULL
+ * or <= 0: off) and uniforms ([0, 1)) hold one value per row. With
+ * w = exp((x - max) / T) and the order (x descending, index ascending) the
+ * kept tokens are the shortest of: the first top_k; those up to the running
+ * sum top_p * sum(w); those with w >= min_p (never fewer than one). The token
+ * is the first kept one whose running sum reaches u * (kept sum), in that
+ * order when a filter is on and by index otherwise; logits of -infinity or
+ * NaN are never drawn, and a row of nothing else gives token 0. Greedy rows
+ * (also top_k = 1) take minq_argmax's token. Sums are f64. n <= 4194304,
+ * n_rows <= 2^20. */
+minq_status minq_sample_rows(const float* logits, size_t row_stride, size_t n_rows, size_t n,
+                             const float* temperature, const int32_t* top_k, const float* top_p,
+                             const float* min_p, const float* uniforms, uint32_t* tokens,
+                             void* stream);
+
 /* The model's CUDA stream (cudaStream_t as void*). */
 void* minq_model_stream(minq_model* m);
 

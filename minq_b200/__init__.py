@@ -12,5 +12,9 @@ from .api import (  # noqa: F401
     argmax, dequantize_q4_0, dequantize_q8_0, eval_ppl, matvec_f32, quantize_q4_0, quantize_q8_0,
     tp_unique_id,
 )
+from .serving import (  # noqa: F401
+    PAGES_BAD_LENGTH, PAGES_BAD_PAGE, PAGES_ROW_FULL, PAGES_SHORT, PAGES_TOO_MANY_TOKENS, PageStep,
+    PageTrim, kv4_attend, kv4_pool, kv4_read, kv4_write, pages_extend, pages_trim, sample_rows,
+)
 
 __version__ = "0.1.0"

@@ -126,6 +126,14 @@ SIGNATURES = {
     "minq_sampler_sample": (I, [P, P, S, P]),
     "minq_sampler_rng_u32": (I, [P, S, P]),
     "minq_generate_sampled": (I, [P, P, P, S, S, P, S, TOKEN_CB, P, P, C.POINTER(GenStats)]),
+    "minq_pages_extend": (I, [P, P, S, S, P, S, P, S, P, S, P, P, P, P, P, P, P]),
+    "minq_pages_trim": (I, [P, P, S, S, P, S, P, S, P, P, P, P, P]),
+    "minq_kv4_write": (I, [P, P, S, S, P, S, S, S, P, P, S, S, P]),
+    "minq_kv4_read": (I, [P, P, S, S, P, S, S, S, P, P, S, S, P]),
+    "minq_kv4_attend_workspace_bytes": (S, [S, S, S, S, S]),
+    "minq_kv4_attend": (I, [P, S, P, S, P, S, P, S, P, P, S, S, S, S, S, C.c_float, P, S, P, S,
+                            P]),
+    "minq_sample_rows": (I, [P, S, S, S, P, P, P, P, P, P, P]),
     "minq_debug_inject_timeout": (I, [P, I]),
 }
 

@@ -113,7 +113,7 @@ minq_status take_device_status() {
               "a bounded device-side wait timed out (status " + std::to_string(v) + ")");
 }
 
-static minq_status require_device() {
+minq_status require_device() {
   int n = 0;
   cudaError_t e = cudaGetDeviceCount(&n);
   if (e != cudaSuccess || n == 0)

@@ -22,6 +22,9 @@ void set_error(const std::string& msg);
 minq_status fail(minq_status code, const std::string& msg);
 minq_status cuda_fail(cudaError_t e, const char* what);
 
+// MINQ_OK when a CUDA device is present.
+minq_status require_device();
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 

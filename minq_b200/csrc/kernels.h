@@ -164,6 +164,9 @@ minq_status launch_epilogue(const float* acc, const float* bias, const float* re
                             size_t n, cudaStream_t s);
 minq_status launch_swiglu(const float* g, const float* u, float* h, size_t n, cudaStream_t s);
 minq_status launch_advance_pos(int* pos, int by, cudaStream_t s);
+// pages.cu: page sizes of the paged 4-bit cache (a power of two in 16..1024,
+// so that 16 positions lie in one page and a 16-byte aligned run)
+bool kv4_page_size_ok(size_t page_size);
 // sampler.cu: the device a sampler was created on
 int sampler_device(const minq_sampler* s);
 // per-row negative log-likelihood (ppl.rs:30-35) of logits [rows][V] at
