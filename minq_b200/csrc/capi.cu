@@ -178,7 +178,8 @@ minq_status minq_device_status(void) {
   MINQ_CUDA_TRY(cudaDeviceSynchronize());
   const minq_status a = take_device_status();
   const minq_status b = take_static_attn_status();
-  return a != MINQ_OK ? a : b;
+  const minq_status c = take_kv4_status();
+  return a != MINQ_OK ? a : b != MINQ_OK ? b : c;
 }
 
 minq_status minq_kernel_timer_start(const char* family) {

@@ -7,12 +7,52 @@
 // the Q4_0 blocks stand for. Positions beyond the table row, in a page whose
 // id is outside the pool, or before the start (pos < 0) do not exist; a row
 // that sees nothing is zero.
+//
+// The tensor-core kernel (head_dim 64, 128). With k_t = d_tb (c_tb - 8) for
+// block b of 32 dimensions, scale s and codes c in 0..15,
+//   score  z_t  = sum_b d_tb sum_i s q_i (c_ti - 8)
+//   output o_i  = sum_t (p_t e_tb) (c_ti - 8)      (e: the scales of V)
+// so the codes enter the MMAs exactly and the scales stay f32: they multiply
+// the 32-dimension partial scores, and the weights before P V. q and p_t e_tb
+// are split into two f16 parts (22 bits), each part one MMA with f32
+// accumulation, which keeps the products to about f32's own rounding:
+//   * q is scaled per row by a power of two that puts its largest value in
+//     [2^10, 2^11), so the low part's smallest step is 2^-35 of that value;
+//   * p e is scaled by 2^10 / 2^floor(log2 max e), which follows the largest
+//     value scale seen, like the running maximum of the softmax; a step of its
+//     low part is 2^-34 of the largest p e.
+// Codes become exact signed f16 integers, two per instruction pair. (Left
+// unsigned, as the subnormals that their bits are, they cost half as much,
+// but the offset 8 sum q then costs the scores a digit.)
+//
+// Tiles are transposed, scores = K (16 positions) x q^T (8 columns) and
+// o^T = V^T (16 dimensions) x p^T: a column is a (token, query head) pair of one
+// kv head, so the 4 to 8 heads of a group fill the MMA's narrow side. A V tile
+// has its positions along k; two positions' codes are paired by one byte
+// permutation of their words.
+//
+// Each warp owns every NW-th tile of 16 positions and keeps its own running
+// maximum, sum and accumulator; its K and V rows (16 rows of one page: two
+// contiguous runs) come by bulk copies into a private ring, so no warp waits
+// for another until the item's end. The maximum is only moved when a weight
+// would exceed 2^4 (one vote a tile), which leaves the accumulator alone
+// almost always.
+//
+// Work split. An item is (request, kv head, column tile); its weight is its
+// number of positions plus a constant for its start and end. The items of the
+// step lie on one line, and CTA c takes the c-th of equal pieces of it,
+// computed on the device from the lengths (no host synchronisation, graphs
+// replay over changing lengths). An item that lies in one CTA is written out
+// directly; the pieces of the others go to the workspace and a second small
+// launch joins them in a fixed order, so results repeat bit for bit.
+#include <cuda_fp16.h>
 #include <math.h>
 
 #include <string>
 
 #include "common.cuh"
 #include "kernels.h"
+#include "pipeline.cuh"
 
 namespace minq {
 
@@ -34,6 +74,13 @@ struct Kv4AttnParams {
   float scale;
   float* out;
   size_t out_stride;
+  // tensor-core kernel
+  int gsz, hgroups, tpt;  // columns: heads per group tile, tiles per kv head, tokens per tile
+  int n_cta;
+  float* part_o;   // [n_cta][2][cols][hd] unnormalised partial outputs
+  float* part_ml;  // [n_cta][2][cols][2] their maxima and sums
+  int4* rec;       // [n_cta] the split item that starts in this CTA: (request, head tile, column
+                   // tile, parts)
 };
 
 // Request of token t, or -1 where t lies behind the last sequence (or the
@@ -121,7 +168,682 @@ __global__ void __launch_bounds__(128) kv4_attend_rows_kernel(Kv4AttnParams p) {
     if (b < nb) out[b * 32 + lane] = l != 0.0f ? o[b] / l : 0.0f;
 }
 
+
+// ---- tensor cores ------------------------------------------------------------
+
+// Set when a bounded wait gave up (read and cleared by take_kv4_status): a
+// file-scope word, so that no call allocates.
+__device__ int g_kv4_status;
+
+constexpr int kKvWarps = 8;
+constexpr int kKvStages = 4;
+constexpr int kKvTile = 16;     // positions per tile
+constexpr int kKvItem = 64;     // an item's start and end, in positions
+constexpr int kKvMinPiece = 256;  // positions per CTA below which an item is not split further
+
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// (x, y) as two f16 pairs, high and low parts.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = h2_bits(h);
+  lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+// The codes in nibbles 0..3 of both halves of x as exact signed integers:
+// 0x6400 | c is 1024 + c in f16, and 0x6400 | 16 c is 1024 + 16 c.
+__device__ __forceinline__ void codes4(uint32_t x, uint32_t* y) {
+  const __half2 m8 = __float2half2_rn(-1032.0f), m72 = __float2half2_rn(-72.0f),
+                r16 = __float2half2_rn(0.0625f);
+  const uint32_t z = x >> 8;
+  y[0] = h2_bits(__hadd2(bits_h2((x & 0x000f000fu) | 0x64006400u), m8));
+  y[1] = h2_bits(__hfma2(bits_h2((x & 0x00f000f0u) | 0x64006400u), r16, m72));
+  y[2] = h2_bits(__hadd2(bits_h2((z & 0x000f000fu) | 0x64006400u), m8));
+  y[3] = h2_bits(__hfma2(bits_h2((z & 0x00f000f0u) | 0x64006400u), r16, m72));
+}
+
+// o[0..1] += c[0..1], one packed addition.
+__device__ __forceinline__ void add2(float* o, const float* c) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(o[0]), "+f"(o[1])
+      : "f"(c[0]), "f"(c[1]));
+}
+
+// The line of items. Request r: n tokens in J column tiles per head tile.
+struct KvReq {
+  int r, t0, n, len;  // request, first token, tokens, positions
+  long long base;     // weight of column tile j: base + (j + 1) * tpt
+  long long J;
+};
+__device__ __forceinline__ KvReq kv_req(const Kv4AttnParams& p, int r) {
+  KvReq q;
+  q.r = r;
+  const int a = p.q_start[r], b = p.q_start[r + 1];
+  const bool ok = a >= 0 && b <= p.n_tokens && a < b;  // a valid run of tokens
+  q.t0 = ok ? a : 0;
+  q.n = ok ? b - a : 0;
+  q.len = p.lens[r];
+  const int prior = q.len - q.n;
+  q.base = (prior > 0 ? prior : 0) + kKvItem;
+  q.J = (q.n + p.tpt - 1) / p.tpt;
+  return q;
+}
+// Weight of column tiles 0 .. j - 1.
+__device__ __forceinline__ long long kv_cum(const KvReq& q, int tpt, long long j) {
+  return j * q.base + (long long)tpt * (j * (j + 1) / 2);
+}
+
+template <int HD, int NT>
+struct KvGeom {
+  static constexpr int NB = HD / 32;             // blocks per row
+  static constexpr int ROW = NB * kQ4Bytes;      // bytes per row
+  static constexpr int SIDE = kKvTile * ROW;     // K (or V) bytes per tile
+  static constexpr int RING = kKvStages * 2 * SIDE;
+  static constexpr int COLS = 8 * NT;
+  static constexpr int OP = HD + 8;              // row pitch of the merge area (floats)
+  static constexpr int MERGE = COLS * OP * 4;
+  static constexpr int PER_WARP = RING > MERGE ? RING : MERGE;
+  static constexpr int SMEM = kKvWarps * PER_WARP + kKvWarps * COLS * 8 + kKvWarps * kKvStages * 8 +
+                              256;
+};
+
+// One warp's state for an item.
+template <int HD, int NT>
+struct KvState {
+  static constexpr int NB = HD / 32;
+  uint32_t q[NT][NB][2][4];  // [..][k step]: b0 b1 of the high, b0 b1 of the low part
+  float cn[NT][2];           // scores to log2 units
+  int lim[NT][2];            // positions the column sees
+  float m[NT][2], l[NT][2];
+  float o[NT][NB][2][4];
+  float vref, vinv;          // 2^floor(log2 max value scale), 2^10 / vref
+  bool first;                // no tile seen yet (uniform over the warp)
+};
+
+// One tile of 16 positions whose K and V rows are at k and v.
+template <int HD, int NT, bool MASK>
+__device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, const uint8_t* v,
+                                        int pos0, int lim_max, int n_nt) {
+  constexpr int NB = HD / 32;
+  constexpr int ROW = NB * kQ4Bytes;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  // scores
+  float s[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+  const uint8_t* k0 = k + g * ROW;
+  const uint8_t* k1 = k0 + 8 * ROW;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(k0 + b * kQ4Bytes + 4 + 4 * t);
+    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(k1 + b * kQ4Bytes + 4 + 4 * t);
+    const float d0 = *reinterpret_cast<const float*>(k0 + b * kQ4Bytes);
+    const float d1 = *reinterpret_cast<const float*>(k1 + b * kQ4Bytes);
+    uint32_t a0[4], a1[4];  // dimensions (0, 4), (1, 5), (2, 6), (3, 7) of the lane's eight
+    codes4(w0, a0);
+    codes4(w1, a1);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (NT > 1 && n >= n_nt) break;
+      // the small parts first: an MMA truncates its sum, and a truncation next
+      // to the small sums is worth nothing
+      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      mma_f16(c, a0[0], a1[0], a0[1], a1[1], st.q[n][b][0][2], st.q[n][b][0][3]);
+      mma_f16(c, a0[2], a1[2], a0[3], a1[3], st.q[n][b][1][2], st.q[n][b][1][3]);
+      mma_f16(c, a0[0], a1[0], a0[1], a1[1], st.q[n][b][0][0], st.q[n][b][0][1]);
+      mma_f16(c, a0[2], a1[2], a0[3], a1[3], st.q[n][b][1][0], st.q[n][b][1][1]);
+      s[n][0] = fmaf(c[0], d0, s[n][0]);
+      s[n][1] = fmaf(c[1], d0, s[n][1]);
+      s[n][2] = fmaf(c[2], d1, s[n][2]);
+      s[n][3] = fmaf(c[3], d1, s[n][3]);
+    }
+  }
+  // value scales of positions g and g + 8
+  const uint8_t* v0 = v + g * ROW;
+  const uint8_t* v1 = v0 + 8 * ROW;
+  float e0[NB], e1[NB];
+  float emax = 0.0f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    e0[b] = *reinterpret_cast<const float*>(v0 + b * kQ4Bytes);
+    e1[b] = *reinterpret_cast<const float*>(v1 + b * kQ4Bytes);
+    if (MASK) {  // what no column sees may be anything
+      if (pos0 + g >= lim_max) e0[b] = 0.0f;
+      if (pos0 + g + 8 >= lim_max) e1[b] = 0.0f;
+    }
+    // infinite and NaN scales stay out of the reference
+    emax = fmaxf(emax, fabsf(e0[b]) < INFINITY ? fabsf(e0[b]) : 0.0f);
+    emax = fmaxf(emax, fabsf(e1[b]) < INFINITY ? fabsf(e1[b]) : 0.0f);
+  }
+  if (__any_sync(0xffffffffu, emax >= 2.0f * st.vref)) {
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) emax = fmaxf(emax, __shfl_xor_sync(0xffffffffu, emax, o));
+    const float ref = fmaxf(__uint_as_float(__float_as_uint(emax) & 0x7f800000u), st.vref);
+    const float f = st.vref / ref;  // powers of two
+    st.vref = ref;
+    st.vinv = 1024.0f / ref;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.o[n][b][j][i] *= f;
+  }
+  // softmax: x = z - m in log2 units
+  bool move = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (NT > 1 && n >= n_nt) break;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[n][i] = fmaf(s[n][i], st.cn[n][i & 1], -st.m[n][i & 1]);
+      if (MASK && pos0 + g + (i >> 1) * 8 >= st.lim[n][i & 1]) s[n][i] = -INFINITY;
+      move |= s[n][i] > 4.0f;
+    }
+  }
+  if (st.first || __any_sync(0xffffffffu, move)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (NT > 1 && n >= n_nt) break;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = fmaxf(s[n][c], s[n][c + 2]);
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+        // the first tile sets the maximum (a column that sees none of it sees
+        // none of the later ones), then it only grows
+        if (st.first)
+          x = x == -INFINITY ? 0.0f : x;
+        else
+          x = fmaxf(x, 0.0f);
+        const float a = st.first ? 1.0f : ex2(-x);
+        st.m[n][c] += x;
+        st.l[n][c] *= a;
+        s[n][c] -= x;
+        s[n][c + 2] -= x;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            st.o[n][b][j][c] *= a;
+            st.o[n][b][j][c + 2] *= a;
+          }
+      }
+    }
+    st.first = false;
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (NT > 1 && n >= n_nt) break;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[n][i] = ex2(s[n][i]);
+    st.l[n][0] += s[n][0] + s[n][2];
+    st.l[n][1] += s[n][1] + s[n][3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[n][i] *= st.vinv;
+  }
+  // o^T += V^T p^T: lane g holds 4 dimensions of a block (its half word),
+  // positions 2t, 2t + 1, 2t + 8, 2t + 9
+  const uint8_t* vw = v + 2 * t * ROW + 4 + 2 * g;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const uint32_t h0 = *reinterpret_cast<const uint16_t*>(vw + b * kQ4Bytes);
+    const uint32_t h1 = *reinterpret_cast<const uint16_t*>(vw + b * kQ4Bytes + ROW);
+    const uint32_t h2 = *reinterpret_cast<const uint16_t*>(vw + b * kQ4Bytes + 8 * ROW);
+    const uint32_t h3 = *reinterpret_cast<const uint16_t*>(vw + b * kQ4Bytes + 9 * ROW);
+    const uint32_t xl = __byte_perm(h0, h1, 0x5410), xh = __byte_perm(h2, h3, 0x5410);
+    uint32_t y[2][4];  // [pair of positions][dimension]
+    codes4(xl, y[0]);
+    codes4(xh, y[1]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (NT > 1 && n >= n_nt) break;
+      float p0 = s[n][0] * e0[b], p1 = s[n][1] * e0[b], p2 = s[n][2] * e1[b], p3 = s[n][3] * e1[b];
+      if (MASK) {  // a weight of zero stays zero whatever the scale is
+        p0 = s[n][0] == 0.0f ? 0.0f : p0;
+        p1 = s[n][1] == 0.0f ? 0.0f : p1;
+        p2 = s[n][2] == 0.0f ? 0.0f : p2;
+        p3 = s[n][3] == 0.0f ? 0.0f : p3;
+      }
+      uint32_t hi0, lo0, hi1, lo1;
+      split2(p0, p1, hi0, lo0);
+      split2(p2, p3, hi1, lo1);
+      hi0 = transpose8x8(hi0);
+      hi1 = transpose8x8(hi1);
+      lo0 = transpose8x8(lo0);
+      lo1 = transpose8x8(lo1);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // the tile's sum by itself, then added with rounding: MMAs into the
+        // running sum would truncate it once each, always towards zero
+        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma_f16(c, y[0][2 * j], y[0][2 * j + 1], y[1][2 * j], y[1][2 * j + 1], lo0, lo1);
+        mma_f16(c, y[0][2 * j], y[0][2 * j + 1], y[1][2 * j], y[1][2 * j + 1], hi0, hi1);
+        add2(st.o[n][b][j], c);
+        add2(st.o[n][b][j] + 2, c + 2);
+      }
+    }
+  }
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 2 : 1)
+    kv4_attend_kernel(const __grid_constant__ Kv4AttnParams p) {
+  using GM = KvGeom<HD, NT>;
+  constexpr int NB = GM::NB, COLS = GM::COLS;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* ring_all = smem;
+  float2* s_ml = reinterpret_cast<float2*>(smem + kKvWarps * GM::PER_WARP);  // [warp][cols]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_ml + kKvWarps * COLS);
+  __shared__ long long s_red[kKvWarps];
+  __shared__ long long s_find[2];  // request and offset at this CTA's start
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int cta = blockIdx.x;
+  uint8_t* ring = ring_all + warp * GM::PER_WARP;
+  uint64_t* bar = bars + warp * kKvStages;
+  if (lane < kKvStages) mbar_init(&bar[lane], 1);
+  mbar_fence_init();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // where this CTA's piece of the line starts
+  const int H = p.nkv * p.hgroups;
+  long long total = 0;
+  for (int r = tid; r < p.n_req; r += kKvWarps * 32) {
+    const KvReq q = kv_req(p, r);
+    total += H * kv_cum(q, p.tpt, q.J);
+  }
+  const long long mine = total;  // with n_req <= 256: request tid's weight
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) s_red[warp] = total;
+  if (tid == 0) s_find[0] = -1;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kKvWarps; ++w) total += s_red[w];
+  long long per = (total + p.n_cta - 1) / p.n_cta;
+  const long long least = kKvMinPiece + kKvItem;
+  if (per < least) per = least;
+  const long long u0 = per * cta, u1 = u0 + per < total ? u0 + per : total;
+  if (u0 >= u1) {
+    if (tid == 0) p.rec[cta] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  long long before = 0;  // weight of the requests of earlier rounds
+  for (int r0 = 0; r0 < p.n_req; r0 += kKvWarps * 32) {
+    const int r = r0 + tid;
+    long long w = mine;
+    if (p.n_req > kKvWarps * 32) {
+      w = 0;
+      if (r < p.n_req) {
+        const KvReq q = kv_req(p, r);
+        w = H * kv_cum(q, p.tpt, q.J);
+      }
+    }
+    long long incl = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_red[warp] = incl;
+    __syncthreads();
+    long long start = before + incl - w;
+    for (int x = 0; x < kKvWarps; ++x) {
+      if (x < warp) start += s_red[x];
+      before += s_red[x];
+    }
+    if (r < p.n_req && start <= u0 && u0 < start + w) {
+      s_find[0] = r;
+      s_find[1] = start;
+    }
+    if (before > u0) break;  // uniform
+  }
+  __syncthreads();
+  if (s_find[0] < 0) return;  // cannot happen: the line's pieces cover it
+  KvReq rq = kv_req(p, (int)s_find[0]);
+  long long s0;  // start of the current item on the line
+  int h;         // its head tile
+  long long j;   // its column tile
+  {
+    const long long W = kv_cum(rq, p.tpt, rq.J), off = u0 - s_find[1];
+    h = (int)(off / W);
+    const long long x = off - h * W;
+    long long lo = 0, hi = rq.J;
+    while (hi - lo > 1) {
+      const long long mid = (lo + hi) >> 1;
+      if (kv_cum(rq, p.tpt, mid) <= x)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    j = lo;
+    s0 = s_find[1] + h * W + kv_cum(rq, p.tpt, j);
+  }
+
+  uint32_t fill = 0, used = 0;  // tiles issued / consumed by this warp so far
+  int4 rec = make_int4(0, 0, 0, 0);
+  bool alive = true;
+  KvState<HD, NT> st;
+  long long u = u0;
+  while (u < u1) {
+    const long long w = rq.base + (j + 1) * p.tpt;
+    const long long x0 = u - s0, x1 = (u1 - s0 < w ? u1 - s0 : w);
+    const int kvh = h / p.hgroups, h0 = kvh * (p.nh / p.nkv) + (h % p.hgroups) * p.gsz;
+    const int nhead = min(p.gsz, p.nh / p.nkv - (h % p.hgroups) * p.gsz);
+    const int tok0 = (int)(j * p.tpt), ntok = min(p.tpt, rq.n - tok0);
+    const int prior = rq.len - rq.n;
+    // positions of the table row (tile ends stay inside 31 bits)
+    const long long cap = min((long long)p.table_stride << p.page_shift, 0x7fffff00ll);
+    // positions that the tile's last token sees
+    long long lim_all = (long long)prior + tok0 + ntok;
+    lim_all = lim_all < cap ? lim_all : cap;
+    const int lim_max = lim_all > 0 ? (int)lim_all : 0;
+    const int n_nt = (ntok * p.gsz + 7) / 8;
+
+    // --- columns: q as f16 parts, limits
+    int lim_min = lim_max;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int col = n * 8 + g, ct = col / p.gsz, ch = col - ct * p.gsz;
+      const bool on = ct < ntok && ch < nhead;
+      const float* qp = p.q + (size_t)(rq.t0 + tok0 + (on ? ct : 0)) * p.q_stride +
+                        (size_t)(h0 + (on ? ch : 0)) * HD + 8 * t;
+      float v[NB][8];
+      float amax = 0.0f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[b][e] = on ? qp[b * 32 + e] : 0.0f;
+          amax = fmaxf(amax, fabsf(v[b][e]));
+        }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // f: a power of two with amax * f in [2^10, 2^11)
+      const int ex = min(max((int)(__float_as_uint(amax) >> 23), 24), 254);
+      const float f = __uint_as_float((uint32_t)(264 - ex) << 23);
+      const float cn = p.scale * 1.4426950408889634f * (1.0f / f);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float* e = v[b] + 2 * x;
+          split2(e[0] * f, e[4] * f, st.q[n][b][x][0], st.q[n][b][x][2]);
+          split2(e[1] * f, e[5] * f, st.q[n][b][x][1], st.q[n][b][x][3]);
+        }
+      }
+      st.cn[n][0] = __shfl_sync(0xffffffffu, cn, 8 * t);
+      st.cn[n][1] = __shfl_sync(0xffffffffu, cn, 8 * t + 4);
+      long long lim = on ? (long long)prior + tok0 + ct + 1 : 0;
+      lim = lim < 0 ? 0 : lim < cap ? lim : cap;
+      st.lim[n][0] = __shfl_sync(0xffffffffu, (int)lim, 8 * t);
+      st.lim[n][1] = __shfl_sync(0xffffffffu, (int)lim, 8 * t + 4);
+      if (on) lim_min = min(lim_min, (int)lim);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        st.m[n][c] = 0.0f;
+        st.l[n][c] = 0.0f;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st.o[n][b][y][i] = 0.0f;
+    }
+    lim_min = (int)__reduce_min_sync(0xffffffffu, (unsigned)lim_min);
+    st.vref = 7.8886091e-31f;  // 2^-100
+    st.vinv = 1024.0f / st.vref;
+    st.first = true;
+
+    // --- tiles [ta, tb) of the item, every kKvWarps-th from this warp's
+    const long long n_tiles = (lim_max + kKvTile - 1) / kKvTile;
+    long long ta = x0 > kKvItem ? (x0 - kKvItem + kKvTile - 1) / kKvTile : 0;
+    long long tb = x1 == w ? n_tiles : x1 > kKvItem ? (x1 - kKvItem + kKvTile - 1) / kKvTile : 0;
+    ta = ta < n_tiles ? ta : n_tiles;
+    tb = tb < n_tiles ? tb : n_tiles;
+    const int my = tb > ta + warp ? (int)((tb - ta - warp + kKvWarps - 1) / kKvWarps) : 0;
+    const size_t row0 = ((size_t)kvh << p.page_shift) * GM::ROW;
+    const size_t page_bytes = ((size_t)p.nkv << p.page_shift) * GM::ROW;
+    const int* tab = p.table + (size_t)rq.r * p.table_stride;
+    // page ids of this warp's next 32 tiles, one per lane
+    int ids = -1, ids_next = -1;
+    auto load_ids = [&](int i0) {
+      const int i = i0 + lane;
+      if (i >= my) return -1;
+      const long long pos = (ta + warp + (long long)i * kKvWarps) * kKvTile;
+      return tab[pos >> p.page_shift];
+    };
+    auto issue = [&](int i, int id) {  // lane 0
+      const uint32_t sidx = fill % kKvStages;
+      if (id >= 0 && id < p.n_pages) {
+        const long long pos = (ta + warp + (long long)i * kKvWarps) * kKvTile;
+        const size_t off = (size_t)id * page_bytes + row0 +
+                           (size_t)(pos & ((1ll << p.page_shift) - 1)) * GM::ROW;
+        uint8_t* dst = ring + sidx * 2 * GM::SIDE;
+        mbar_arrive_expect_tx(&bar[sidx], 2 * GM::SIDE);
+        bulk_g2s(dst, p.k_pages + off, GM::SIDE, &bar[sidx]);
+        bulk_g2s(dst + GM::SIDE, p.v_pages + off, GM::SIDE, &bar[sidx]);
+      } else {
+        mbar_arrive(&bar[sidx]);
+      }
+    };
+    ids = load_ids(0);
+    ids_next = load_ids(32);
+    // tile i's id: lane i % 32 of the current or the next group of 32
+    const int first = min(my, kKvStages);
+    for (int i = 0; i < first; ++i) {
+      const int id = __shfl_sync(0xffffffffu, ids, i);
+      if (lane == 0 && alive) issue(i, id);
+      ++fill;
+    }
+    for (int i = 0; i < my; ++i) {
+      const uint32_t sidx = used % kKvStages;
+      if (alive) alive = mbar_wait_timed(&bar[sidx], (used / kKvStages) & 1, &g_kv4_status);
+      alive = __all_sync(0xffffffffu, alive);
+      ++used;
+      const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+      if (alive && id >= 0 && id < p.n_pages) {
+        const int pos0 = (int)((ta + warp + (long long)i * kKvWarps) * kKvTile);
+        const uint8_t* kt = ring + sidx * 2 * GM::SIDE;
+        if (pos0 + kKvTile > lim_min)
+          kv_tile<HD, NT, true>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt);
+        else
+          kv_tile<HD, NT, false>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt);
+      }
+      __syncwarp();
+      if (i + kKvStages < my) {
+        const int nx = i + kKvStages;
+        const int a = __shfl_sync(0xffffffffu, ids, nx & 31);
+        const int b = __shfl_sync(0xffffffffu, ids_next, nx & 31);
+        if (lane == 0 && alive) issue(nx, (nx >> 5) == (i >> 5) ? a : b);
+        ++fill;
+      }
+      if ((i & 31) == 31) {
+        ids = ids_next;
+        ids_next = load_ids(i + 33);
+      }
+    }
+
+    // --- join the warps
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1)
+          st.l[n][c] += __shfl_xor_sync(0xffffffffu, st.l[n][c], o);
+        if (st.l[n][c] == 0.0f) st.m[n][c] = -3.0e38f;  // saw nothing
+        if (g == 0) s_ml[warp * COLS + n * 8 + 2 * t + c] = make_float2(st.m[n][c], st.l[n][c]);
+      }
+    __syncthreads();
+    float* area = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float f[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float M = -3.0e38f;
+#pragma unroll
+        for (int x = 0; x < kKvWarps; ++x)
+          M = fmaxf(M, s_ml[x * COLS + n * 8 + 2 * t + c].x);
+        f[c] = ex2(st.m[n][c] - M) * (st.vref * 0.0009765625f);
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float* a = area + (n * 8 + 2 * t) * GM::OP + b * 32 + 4 * g + 2 * y;
+          const float* o = st.o[n][b][y];
+          *reinterpret_cast<float2*>(a) = make_float2(o[0] * f[0], o[2] * f[0]);
+          *reinterpret_cast<float2*>(a + GM::OP) = make_float2(o[1] * f[1], o[3] * f[1]);
+        }
+    }
+    __syncthreads();
+    const bool whole = x0 == 0 && x1 == w;
+    const int slot = x0 > 0 ? 0 : 1;
+    for (int i = tid; i < COLS * HD; i += kKvWarps * 32) {
+      const int col = i / HD, d = i - col * HD;
+      const int ct = col / p.gsz, ch = col - ct * p.gsz;
+      if (ct >= ntok || ch >= nhead) continue;
+      float M = -3.0e38f, L = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kKvWarps; ++x) M = fmaxf(M, s_ml[x * COLS + col].x);
+#pragma unroll
+      for (int x = 0; x < kKvWarps; ++x) {
+        const float2 ml = s_ml[x * COLS + col];
+        L += ml.y * ex2(ml.x - M);
+        sum += reinterpret_cast<const float*>(ring_all + x * GM::PER_WARP)[col * GM::OP + d];
+      }
+      if (whole) {
+        p.out[(size_t)(rq.t0 + tok0 + ct) * p.out_stride + (size_t)(h0 + ch) * HD + d] =
+            L != 0.0f ? sum / L : 0.0f;
+      } else {
+        const size_t at = ((size_t)cta * 2 + slot) * COLS + col;
+        p.part_o[at * HD + d] = sum;
+        if (d == 0) {
+          p.part_ml[at * 2] = M;
+          p.part_ml[at * 2 + 1] = L;
+        }
+      }
+    }
+    if (!whole && slot == 1)
+      rec = make_int4(rq.r, h, (int)j, (int)((s0 + w - 1) / per) - cta + 1);
+    // the merge area is the ring of the next item's bulk copies
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+
+    u = s0 += w;
+    if (++j == rq.J) {
+      j = 0;
+      if (++h == H) {
+        h = 0;
+        do {
+          if (rq.r + 1 >= p.n_req) break;
+          rq = kv_req(p, rq.r + 1);
+        } while (rq.J == 0);
+      }
+    }
+  }
+  if (tid == 0) p.rec[cta] = rec;
+}
+
+// Joins the pieces of the item that starts in CTA blockIdx.x and goes on in
+// the next ones, in their order. One block per column.
+template <int HD>
+__global__ void __launch_bounds__(HD) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
+  pdl_wait();
+  const int c = blockIdx.x, col = blockIdx.y, cols = gridDim.y, d = threadIdx.x;
+  const int4 rec = p.rec[c];
+  const int parts = min(rec.w, p.n_cta - c);
+  if (parts >= 2) {
+    const KvReq q = kv_req(p, rec.x);
+    const int kvh = rec.y / p.hgroups, hg = rec.y % p.hgroups;
+    const int ct = col / p.gsz, ch = col - ct * p.gsz;
+    const int tok = rec.z * p.tpt + ct, head = hg * p.gsz + ch;
+    if (tok < q.n && ct < p.tpt && head < p.nh / p.nkv) {
+      auto at = [&](int i) { return ((size_t)(c + i) * 2 + (i == 0 ? 1 : 0)) * cols + col; };
+      float M = -3.0e38f;
+      for (int i = 0; i < parts; ++i) M = fmaxf(M, p.part_ml[at(i) * 2]);
+      float L = 0.0f, sum = 0.0f;
+#pragma unroll 4
+      for (int i = 0; i < parts; ++i) {
+        const float f = ex2(p.part_ml[at(i) * 2] - M);
+        L += p.part_ml[at(i) * 2 + 1] * f;
+        sum += p.part_o[at(i) * HD + d] * f;
+      }
+      p.out[(size_t)(q.t0 + tok) * p.out_stride +
+            (size_t)(kvh * (p.nh / p.nkv) + head) * HD + d] = L != 0.0f ? sum / L : 0.0f;
+    }
+  }
+  pdl_launch_dependents();
+}
+
+// How the tensor-core kernel is launched for a call, or n_cta = 0 where the
+// rows kernel serves it.
+struct KvPlan {
+  int nt, n_cta;
+  size_t ws;
+};
+KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_t hd) {
+  KvPlan k{};
+  if ((hd != 64 && hd != 128) || n_kv == 0 || n_req == 0) return k;
+  const size_t G = n_heads / n_kv;
+  k.nt = G > 8 || n_tokens > n_req ? 2 : 1;
+  k.n_cta = sm_count() * (k.nt == 1 ? 2 : 1);
+  k.ws = (size_t)k.n_cta * (2 * 8 * k.nt * (hd + 2) * 4 + sizeof(int4));
+  return k;
+}
+
+template <int HD, int NT>
+minq_status launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
+  using GM = KvGeom<HD, NT>;
+  MINQ_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kv4_attend_kernel<HD, NT>), GM::SMEM));
+  MINQ_CUDA_TRY(launch_k(kv4_attend_kernel<HD, NT>, dim3(p.n_cta), dim3(kKvWarps * 32), GM::SMEM, s,
+                         p));
+  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3(p.n_cta, GM::COLS), dim3(HD), 0, s, p));
+  return MINQ_OK;
+}
+
 }  // namespace
+
+minq_status take_kv4_status() {
+  int v = 0;
+  MINQ_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_kv4_status, sizeof(int)));
+  if (v == 0) return MINQ_OK;
+  const int zero = 0;
+  MINQ_CUDA_TRY(cudaMemcpyToSymbol(g_kv4_status, &zero, sizeof(int)));
+  return fail(MINQ_ERR_TIMEOUT, "a bounded wait of kv4_attend timed out");
+}
 
 }  // namespace minq
 
@@ -131,7 +853,7 @@ extern "C" {
 
 size_t minq_kv4_attend_workspace_bytes(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv,
                                        size_t head_dim) {
-  return 0;
+  return kv_plan(n_req, n_tokens, n_heads, n_kv, head_dim).ws;
 }
 
 minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_start,
@@ -160,9 +882,11 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
     return fail(MINQ_ERR_ARG, "null pointer");
   if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15)
     return fail(MINQ_ERR_ARG, "kv4_attend: pools must be 16-byte aligned");
-  if (workspace_bytes <
-      minq_kv4_attend_workspace_bytes(n_req, n_tokens, n_heads, n_kv, head_dim))
+  const KvPlan plan = kv_plan(n_req, n_tokens, n_heads, n_kv, head_dim);
+  if (plan.ws && (!workspace || workspace_bytes < plan.ws))
     return fail(MINQ_ERR_ARG, "workspace smaller than minq_kv4_attend_workspace_bytes");
+  if (plan.ws && (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(MINQ_ERR_ARG, "kv4_attend: workspace must be 16-byte aligned");
   MINQ_TRY(require_device());
   Kv4AttnParams p{};
   p.q = q;
@@ -183,6 +907,20 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
   p.scale = scale;
   p.out = out;
   p.out_stride = out_stride;
+  if (plan.ws) {
+    const int G = (int)(n_heads / n_kv), cols = 8 * plan.nt;
+    p.gsz = G < cols ? G : cols;
+    p.hgroups = (G + p.gsz - 1) / p.gsz;
+    p.tpt = cols / p.gsz;
+    p.n_cta = plan.n_cta;
+    p.rec = static_cast<int4*>(workspace);
+    p.part_o = reinterpret_cast<float*>(p.rec + plan.n_cta);
+    p.part_ml = p.part_o + (size_t)plan.n_cta * 2 * cols * head_dim;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (head_dim == 64)
+      return plan.nt == 1 ? launch_kv4_attend<64, 1>(p, s) : launch_kv4_attend<64, 2>(p, s);
+    return plan.nt == 1 ? launch_kv4_attend<128, 1>(p, s) : launch_kv4_attend<128, 2>(p, s);
+  }
   const size_t rows = n_tokens * n_heads;
   MINQ_CUDA_TRY(launch_k(kv4_attend_rows_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0,
                          (cudaStream_t)stream, p));
