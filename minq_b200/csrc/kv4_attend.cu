@@ -31,9 +31,9 @@
 // has its positions along k; two positions' codes are paired by one byte
 // permutation of their words.
 //
-// Each warp owns every NW-th tile of 16 positions and keeps its own running
-// maximum, sum and accumulator; its K and V rows (16 rows of one page: two
-// contiguous runs) come by bulk copies into a private ring, so no warp waits
+// Each warp owns every NW-th tile of 32 positions and keeps its own running
+// maximum, sum and accumulator; its K and V rows (16 or 32 rows of one
+// page: a contiguous run each) come by bulk copies into a private ring, so no warp waits
 // for another until the item's end. The maximum is only moved when a weight
 // would exceed 2^4 (one vote a tile), which leaves the accumulator alone
 // almost always.
@@ -175,11 +175,10 @@ __global__ void __launch_bounds__(128) kv4_attend_rows_kernel(Kv4AttnParams p) {
 // file-scope word, so that no call allocates.
 __device__ int g_kv4_status;
 
-constexpr int kKvWarps = 8;
-constexpr int kKvStages = 4;
-constexpr int kKvTile = 16;     // positions per tile
-constexpr int kKvItem = 64;     // an item's start and end, in positions
-constexpr int kKvMinPiece = 256;  // positions per CTA below which an item is not split further
+constexpr int kKvWarps = 4;
+constexpr int kKvTile = 32;     // positions per tile
+constexpr int kKvItem = 256;    // an item's start and end, in positions
+constexpr int kKvMinPiece = 128;  // positions per CTA below which an item is not split further
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -188,6 +187,14 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_zero(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
+                                             uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
@@ -204,10 +211,13 @@ __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cas
 
 // (x, y) as two f16 pairs, high and low parts.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = h2_bits(h);
-  lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+  hi = h2_bits(__floats2half2_rn(x, y));
+  float a, b;  // hi - x, exact; the mixed-precision form needs no conversion
+  asm("{\n\t.reg .f16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\t"
+      "sub.rn.f32.f16 %1, h, %4;\n\t}"
+      : "=f"(a), "=f"(b)
+      : "r"(hi), "f"(x), "f"(y));
+  lo = h2_bits(__floats2half2_rn(-a, -b));
 }
 
 // The codes in nibbles 0..3 of both halves of x as exact signed integers:
@@ -258,13 +268,15 @@ template <int HD, int NT>
 struct KvGeom {
   static constexpr int NB = HD / 32;             // blocks per row
   static constexpr int ROW = NB * kQ4Bytes;      // bytes per row
-  static constexpr int SIDE = kKvTile * ROW;     // K (or V) bytes per tile
-  static constexpr int RING = kKvStages * 2 * SIDE;
+  static constexpr int HALF = 16 * ROW;          // K (or V) bytes of 16 positions
+  static constexpr int SIDE = 2 * HALF;          // and of a tile
+  static constexpr int STAGES = HD == 128 ? 2 : 4;
+  static constexpr int RING = STAGES * 2 * SIDE;
   static constexpr int COLS = 8 * NT;
   static constexpr int OP = HD + 8;              // row pitch of the merge area (floats)
   static constexpr int MERGE = COLS * OP * 4;
   static constexpr int PER_WARP = RING > MERGE ? RING : MERGE;
-  static constexpr int SMEM = kKvWarps * PER_WARP + kKvWarps * COLS * 8 + kKvWarps * kKvStages * 8 +
+  static constexpr int SMEM = kKvWarps * PER_WARP + kKvWarps * COLS * 8 + kKvWarps * STAGES * 8 +
                               256;
 };
 
@@ -281,64 +293,72 @@ struct KvState {
   bool first;                // no tile seen yet (uniform over the warp)
 };
 
-// One tile of 16 positions whose K and V rows are at k and v.
+// One tile of 32 positions, two halves of 16, whose K and V rows are at k and
+// v; ok: the halves that were loaded (MASK: the others may hold anything).
 template <int HD, int NT, bool MASK>
 __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, const uint8_t* v,
-                                        int pos0, int lim_max, int n_nt) {
+                                        int pos0, int lim_max, int n_nt, int ok) {
   constexpr int NB = HD / 32;
   constexpr int ROW = NB * kQ4Bytes;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   // scores
-  float s[NT][4];
+  float s[2][NT][4];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int u = 0; u < 2; ++u) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
-  const uint8_t* k0 = k + g * ROW;
-  const uint8_t* k1 = k0 + 8 * ROW;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(k0 + b * kQ4Bytes + 4 + 4 * t);
-    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(k1 + b * kQ4Bytes + 4 + 4 * t);
-    const float d0 = *reinterpret_cast<const float*>(k0 + b * kQ4Bytes);
-    const float d1 = *reinterpret_cast<const float*>(k1 + b * kQ4Bytes);
-    uint32_t a0[4], a1[4];  // dimensions (0, 4), (1, 5), (2, 6), (3, 7) of the lane's eight
-    codes4(w0, a0);
-    codes4(w1, a1);
+      for (int i = 0; i < 4; ++i) s[u][n][i] = 0.0f;
+    const uint8_t* k0 = k + (16 * u + g) * ROW;
+    const uint8_t* k1 = k0 + 8 * ROW;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (NT > 1 && n >= n_nt) break;
-      // the small parts first: an MMA truncates its sum, and a truncation next
-      // to the small sums is worth nothing
-      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      mma_f16(c, a0[0], a1[0], a0[1], a1[1], st.q[n][b][0][2], st.q[n][b][0][3]);
-      mma_f16(c, a0[2], a1[2], a0[3], a1[3], st.q[n][b][1][2], st.q[n][b][1][3]);
-      mma_f16(c, a0[0], a1[0], a0[1], a1[1], st.q[n][b][0][0], st.q[n][b][0][1]);
-      mma_f16(c, a0[2], a1[2], a0[3], a1[3], st.q[n][b][1][0], st.q[n][b][1][1]);
-      s[n][0] = fmaf(c[0], d0, s[n][0]);
-      s[n][1] = fmaf(c[1], d0, s[n][1]);
-      s[n][2] = fmaf(c[2], d1, s[n][2]);
-      s[n][3] = fmaf(c[3], d1, s[n][3]);
+    for (int b = 0; b < NB; ++b) {
+      uint32_t a0[4], a1[4];  // dimensions (0, 4), (1, 5), (2, 6), (3, 7) of the lane's eight
+      codes4(*reinterpret_cast<const uint32_t*>(k0 + b * kQ4Bytes + 4 + 4 * t), a0);
+      codes4(*reinterpret_cast<const uint32_t*>(k1 + b * kQ4Bytes + 4 + 4 * t), a1);
+      const float d0 = *reinterpret_cast<const float*>(k0 + b * kQ4Bytes);
+      const float d1 = *reinterpret_cast<const float*>(k1 + b * kQ4Bytes);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (NT > 1 && n >= n_nt) break;
+        // the small parts first: an MMA truncates its sum, and a truncation next
+        // to the small sums is worth nothing
+        float c[4];
+        mma_f16_zero(c, a0[0], a1[0], a0[1], a1[1], st.q[n][b][0][2], st.q[n][b][0][3]);
+        mma_f16(c, a0[2], a1[2], a0[3], a1[3], st.q[n][b][1][2], st.q[n][b][1][3]);
+        mma_f16(c, a0[0], a1[0], a0[1], a1[1], st.q[n][b][0][0], st.q[n][b][0][1]);
+        mma_f16(c, a0[2], a1[2], a0[3], a1[3], st.q[n][b][1][0], st.q[n][b][1][1]);
+        s[u][n][0] = fmaf(c[0], d0, s[u][n][0]);
+        s[u][n][1] = fmaf(c[1], d0, s[u][n][1]);
+        s[u][n][2] = fmaf(c[2], d1, s[u][n][2]);
+        s[u][n][3] = fmaf(c[3], d1, s[u][n][3]);
+      }
     }
   }
-  // value scales of positions g and g + 8
-  const uint8_t* v0 = v + g * ROW;
-  const uint8_t* v1 = v0 + 8 * ROW;
-  float e0[NB], e1[NB];
+  // value scales of positions g and g + 8 of each half
+  float e[2][2][NB];
   float emax = 0.0f;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    e0[b] = *reinterpret_cast<const float*>(v0 + b * kQ4Bytes);
-    e1[b] = *reinterpret_cast<const float*>(v1 + b * kQ4Bytes);
-    if (MASK) {  // what no column sees may be anything
-      if (pos0 + g >= lim_max) e0[b] = 0.0f;
-      if (pos0 + g + 8 >= lim_max) e1[b] = 0.0f;
-    }
-    // infinite and NaN scales stay out of the reference
-    emax = fmaxf(emax, fabsf(e0[b]) < INFINITY ? fabsf(e0[b]) : 0.0f);
-    emax = fmaxf(emax, fabsf(e1[b]) < INFINITY ? fabsf(e1[b]) : 0.0f);
-  }
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float x = *reinterpret_cast<const float*>(v + (16 * u + 8 * y + g) * ROW + b * kQ4Bytes);
+        // what no column sees may be anything
+        if (MASK && (!((ok >> u) & 1) || pos0 + 16 * u + 8 * y + g >= lim_max)) x = 0.0f;
+        e[u][y][b] = x;
+        emax = fmaxf(emax, fabsf(x));
+      }
   if (__any_sync(0xffffffffu, emax >= 2.0f * st.vref)) {
+    emax = 0.0f;  // infinite and NaN scales stay out of the reference
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          emax = fmaxf(emax, fabsf(e[u][y][b]) < INFINITY ? fabsf(e[u][y][b]) : 0.0f);
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) emax = fmaxf(emax, __shfl_xor_sync(0xffffffffu, emax, o));
     const float ref = fmaxf(__uint_as_float(__float_as_uint(emax) & 0x7f800000u), st.vref);
@@ -355,24 +375,28 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, c
           for (int i = 0; i < 4; ++i) st.o[n][b][j][i] *= f;
   }
   // softmax: x = z - m in log2 units
-  bool move = false;
+  float most = -INFINITY;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     if (NT > 1 && n >= n_nt) break;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[n][i] = fmaf(s[n][i], st.cn[n][i & 1], -st.m[n][i & 1]);
-      if (MASK && pos0 + g + (i >> 1) * 8 >= st.lim[n][i & 1]) s[n][i] = -INFINITY;
-      move |= s[n][i] > 4.0f;
-    }
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = fmaf(s[u][n][i], st.cn[n][i & 1], -st.m[n][i & 1]);
+        if (MASK && (!((ok >> u) & 1) || pos0 + 16 * u + g + (i >> 1) * 8 >= st.lim[n][i & 1]))
+          x = -INFINITY;
+        s[u][n][i] = x;
+        most = fmaxf(most, x);
+      }
   }
-  if (st.first || __any_sync(0xffffffffu, move)) {
+  if (st.first || __any_sync(0xffffffffu, most > 4.0f)) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (NT > 1 && n >= n_nt) break;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float x = fmaxf(s[n][c], s[n][c + 2]);
+        float x = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
 #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
         // the first tile sets the maximum (a column that sees none of it sees
@@ -384,8 +408,11 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, c
         const float a = st.first ? 1.0f : ex2(-x);
         st.m[n][c] += x;
         st.l[n][c] *= a;
-        s[n][c] -= x;
-        s[n][c + 2] -= x;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          s[u][n][c] -= x;
+          s[u][n][c + 2] -= x;
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -401,49 +428,62 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, c
   for (int n = 0; n < NT; ++n) {
     if (NT > 1 && n >= n_nt) break;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[n][i] = ex2(s[n][i]);
-    st.l[n][0] += s[n][0] + s[n][2];
-    st.l[n][1] += s[n][1] + s[n][3];
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[n][i] *= st.vinv;
+      for (int i = 0; i < 4; ++i) s[u][n][i] = ex2(s[u][n][i]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      st.l[n][c] += (s[0][n][c] + s[0][n][c + 2]) + (s[1][n][c] + s[1][n][c + 2]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[u][n][i] *= st.vinv;
   }
   // o^T += V^T p^T: lane g holds 4 dimensions of a block (its half word),
-  // positions 2t, 2t + 1, 2t + 8, 2t + 9
-  const uint8_t* vw = v + 2 * t * ROW + 4 + 2 * g;
+  // positions 2t, 2t + 1, 2t + 8, 2t + 9 of each half
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const uint32_t h0 = *reinterpret_cast<const uint16_t*>(vw + b * kQ4Bytes);
-    const uint32_t h1 = *reinterpret_cast<const uint16_t*>(vw + b * kQ4Bytes + ROW);
-    const uint32_t h2 = *reinterpret_cast<const uint16_t*>(vw + b * kQ4Bytes + 8 * ROW);
-    const uint32_t h3 = *reinterpret_cast<const uint16_t*>(vw + b * kQ4Bytes + 9 * ROW);
-    const uint32_t xl = __byte_perm(h0, h1, 0x5410), xh = __byte_perm(h2, h3, 0x5410);
-    uint32_t y[2][4];  // [pair of positions][dimension]
-    codes4(xl, y[0]);
-    codes4(xh, y[1]);
+    uint32_t y[2][2][4];  // [half][pair of positions][dimension]
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* w = v + (16 * u + 8 * h + 2 * t) * ROW + b * kQ4Bytes + 4 + 2 * g;
+        const uint32_t x0 = *reinterpret_cast<const uint16_t*>(w);
+        const uint32_t x1 = *reinterpret_cast<const uint16_t*>(w + ROW);
+        codes4(__byte_perm(x0, x1, 0x5410), y[u][h]);
+      }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (NT > 1 && n >= n_nt) break;
-      float p0 = s[n][0] * e0[b], p1 = s[n][1] * e0[b], p2 = s[n][2] * e1[b], p3 = s[n][3] * e1[b];
-      if (MASK) {  // a weight of zero stays zero whatever the scale is
-        p0 = s[n][0] == 0.0f ? 0.0f : p0;
-        p1 = s[n][1] == 0.0f ? 0.0f : p1;
-        p2 = s[n][2] == 0.0f ? 0.0f : p2;
-        p3 = s[n][3] == 0.0f ? 0.0f : p3;
-      }
-      uint32_t hi0, lo0, hi1, lo1;
-      split2(p0, p1, hi0, lo0);
-      split2(p2, p3, hi1, lo1);
-      hi0 = transpose8x8(hi0);
-      hi1 = transpose8x8(hi1);
-      lo0 = transpose8x8(lo0);
-      lo1 = transpose8x8(lo1);
+      uint32_t hi[2][2], lo[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float w0 = s[u][n][2 * h], w1 = s[u][n][2 * h + 1];
+          float p0 = w0 * e[u][h][b], p1 = w1 * e[u][h][b];
+          if (MASK) {  // a weight of zero stays zero whatever the scale is
+            p0 = w0 == 0.0f ? 0.0f : p0;
+            p1 = w1 == 0.0f ? 0.0f : p1;
+          }
+          split2(p0, p1, hi[u][h], lo[u][h]);
+          hi[u][h] = transpose8x8(hi[u][h]);
+          lo[u][h] = transpose8x8(lo[u][h]);
+        }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         // the tile's sum by itself, then added with rounding: MMAs into the
         // running sum would truncate it once each, always towards zero
-        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        mma_f16(c, y[0][2 * j], y[0][2 * j + 1], y[1][2 * j], y[1][2 * j + 1], lo0, lo1);
-        mma_f16(c, y[0][2 * j], y[0][2 * j + 1], y[1][2 * j], y[1][2 * j + 1], hi0, hi1);
+        float c[4];
+        mma_f16_zero(c, y[0][0][2 * j], y[0][0][2 * j + 1], y[0][1][2 * j], y[0][1][2 * j + 1],
+                     lo[0][0], lo[0][1]);
+        mma_f16(c, y[1][0][2 * j], y[1][0][2 * j + 1], y[1][1][2 * j], y[1][1][2 * j + 1],
+                lo[1][0], lo[1][1]);
+        mma_f16(c, y[0][0][2 * j], y[0][0][2 * j + 1], y[0][1][2 * j], y[0][1][2 * j + 1],
+                hi[0][0], hi[0][1]);
+        mma_f16(c, y[1][0][2 * j], y[1][0][2 * j + 1], y[1][1][2 * j], y[1][1][2 * j + 1],
+                hi[1][0], hi[1][1]);
         add2(st.o[n][b][j], c);
         add2(st.o[n][b][j] + 2, c + 2);
       }
@@ -452,7 +492,7 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, c
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
     kv4_attend_kernel(const __grid_constant__ Kv4AttnParams p) {
   using GM = KvGeom<HD, NT>;
   constexpr int NB = GM::NB, COLS = GM::COLS;
@@ -466,8 +506,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 2 : 1)
   const int g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x;
   uint8_t* ring = ring_all + warp * GM::PER_WARP;
-  uint64_t* bar = bars + warp * kKvStages;
-  if (lane < kKvStages) mbar_init(&bar[lane], 1);
+  uint64_t* bar = bars + warp * GM::STAGES;
+  if (lane < GM::STAGES) mbar_init(&bar[lane], 1);
   mbar_fence_init();
   pdl_wait();
   pdl_launch_dependents();
@@ -479,7 +519,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 2 : 1)
     const KvReq q = kv_req(p, r);
     total += H * kv_cum(q, p.tpt, q.J);
   }
-  const long long mine = total;  // with n_req <= 256: request tid's weight
+  const long long mine = total;  // with at most one round: request tid's weight
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_red[warp] = total;
@@ -635,62 +675,77 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 2 : 1)
     const size_t row0 = ((size_t)kvh << p.page_shift) * GM::ROW;
     const size_t page_bytes = ((size_t)p.nkv << p.page_shift) * GM::ROW;
     const int* tab = p.table + (size_t)rq.r * p.table_stride;
-    // page ids of this warp's next 32 tiles, one per lane
-    int ids = -1, ids_next = -1;
+    // page ids of the halves of this warp's next 16 tiles, one per lane; -1
+    // behind the last position
+    auto tile_pos = [&](int i) { return (ta + warp + (long long)i * kKvWarps) * kKvTile; };
     auto load_ids = [&](int i0) {
-      const int i = i0 + lane;
-      if (i >= my) return -1;
-      const long long pos = (ta + warp + (long long)i * kKvWarps) * kKvTile;
-      return tab[pos >> p.page_shift];
+      const int i = i0 + (lane >> 1);
+      const long long pos = tile_pos(i) + 16 * (lane & 1);
+      int id = -1;
+      if (i < my && pos < lim_max) id = tab[pos >> p.page_shift];
+      return id < p.n_pages ? id : -1;
     };
-    auto issue = [&](int i, int id) {  // lane 0
-      const uint32_t sidx = fill % kKvStages;
-      if (id >= 0 && id < p.n_pages) {
-        const long long pos = (ta + warp + (long long)i * kKvWarps) * kKvTile;
-        const size_t off = (size_t)id * page_bytes + row0 +
-                           (size_t)(pos & ((1ll << p.page_shift) - 1)) * GM::ROW;
-        uint8_t* dst = ring + sidx * 2 * GM::SIDE;
-        mbar_arrive_expect_tx(&bar[sidx], 2 * GM::SIDE);
+    int ids = load_ids(0), ids_next = load_ids(16);
+    auto issue = [&](int i, int id0, int id1) {  // lane 0
+      const uint32_t sidx = fill % GM::STAGES;
+      const long long pos = tile_pos(i);
+      const size_t in_page = (size_t)(pos & ((1ll << p.page_shift) - 1));
+      uint8_t* dst = ring + sidx * 2 * GM::SIDE;
+      const uint32_t n = (id0 >= 0) + (id1 >= 0);
+      if (n == 0) {
+        mbar_arrive(&bar[sidx]);
+        return;
+      }
+      mbar_arrive_expect_tx(&bar[sidx], n * 2 * GM::HALF);
+      if (n == 2 && p.page_shift > 4) {  // both halves in one page
+        const size_t off = (size_t)id0 * page_bytes + row0 + in_page * GM::ROW;
         bulk_g2s(dst, p.k_pages + off, GM::SIDE, &bar[sidx]);
         bulk_g2s(dst + GM::SIDE, p.v_pages + off, GM::SIDE, &bar[sidx]);
       } else {
-        mbar_arrive(&bar[sidx]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int id = x ? id1 : id0;
+          if (id < 0) continue;
+          const size_t off = (size_t)id * page_bytes + row0 +
+                             (p.page_shift > 4 ? in_page + 16 * x : 0) * GM::ROW;
+          bulk_g2s(dst + x * GM::HALF, p.k_pages + off, GM::HALF, &bar[sidx]);
+          bulk_g2s(dst + GM::SIDE + x * GM::HALF, p.v_pages + off, GM::HALF, &bar[sidx]);
+        }
       }
     };
-    ids = load_ids(0);
-    ids_next = load_ids(32);
-    // tile i's id: lane i % 32 of the current or the next group of 32
-    const int first = min(my, kKvStages);
+    const int first = min(my, GM::STAGES);
     for (int i = 0; i < first; ++i) {
-      const int id = __shfl_sync(0xffffffffu, ids, i);
-      if (lane == 0 && alive) issue(i, id);
+      const int a = __shfl_sync(0xffffffffu, ids, 2 * i);
+      const int b = __shfl_sync(0xffffffffu, ids, 2 * i + 1);
+      if (lane == 0 && alive) issue(i, a, b);
       ++fill;
     }
     for (int i = 0; i < my; ++i) {
-      const uint32_t sidx = used % kKvStages;
-      if (alive) alive = mbar_wait_timed(&bar[sidx], (used / kKvStages) & 1, &g_kv4_status);
+      const uint32_t sidx = used % GM::STAGES;
+      if (alive) alive = mbar_wait_timed(&bar[sidx], (used / GM::STAGES) & 1, &g_kv4_status);
       alive = __all_sync(0xffffffffu, alive);
       ++used;
-      const int id = __shfl_sync(0xffffffffu, ids, i & 31);
-      if (alive && id >= 0 && id < p.n_pages) {
-        const int pos0 = (int)((ta + warp + (long long)i * kKvWarps) * kKvTile);
+      const int ok = (int)(__ballot_sync(0xffffffffu, ids >= 0) >> (2 * (i & 15))) & 3;
+      if (alive && ok) {
+        const int pos0 = (int)tile_pos(i);
         const uint8_t* kt = ring + sidx * 2 * GM::SIDE;
-        if (pos0 + kKvTile > lim_min)
-          kv_tile<HD, NT, true>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt);
+        if (pos0 + kKvTile > lim_min || ok != 3)
+          kv_tile<HD, NT, true>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
         else
-          kv_tile<HD, NT, false>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt);
+          kv_tile<HD, NT, false>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
       }
       __syncwarp();
-      if (i + kKvStages < my) {
-        const int nx = i + kKvStages;
-        const int a = __shfl_sync(0xffffffffu, ids, nx & 31);
-        const int b = __shfl_sync(0xffffffffu, ids_next, nx & 31);
-        if (lane == 0 && alive) issue(nx, (nx >> 5) == (i >> 5) ? a : b);
+      if (i + GM::STAGES < my) {
+        const int nx = i + GM::STAGES, src = 2 * (nx & 15);
+        const int from = (nx >> 4) == (i >> 4) ? ids : ids_next;
+        const int a = __shfl_sync(0xffffffffu, from, src);
+        const int b = __shfl_sync(0xffffffffu, from, src + 1);
+        if (lane == 0 && alive) issue(nx, a, b);
         ++fill;
       }
-      if ((i & 31) == 31) {
+      if ((i & 15) == 15) {
         ids = ids_next;
-        ids_next = load_ids(i + 33);
+        ids_next = load_ids(i + 17);
       }
     }
 
@@ -819,7 +874,7 @@ KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_
   if ((hd != 64 && hd != 128) || n_kv == 0 || n_req == 0) return k;
   const size_t G = n_heads / n_kv;
   k.nt = G > 8 || n_tokens > n_req ? 2 : 1;
-  k.n_cta = sm_count() * (k.nt == 1 ? 2 : 1);
+  k.n_cta = sm_count() * (k.nt == 1 ? 4 : 2);
   k.ws = (size_t)k.n_cta * (2 * 8 * k.nt * (hd + 2) * 4 + sizeof(int4));
   return k;
 }

@@ -8,7 +8,13 @@ e = 2^-24: a score is a sum of head_dim products and has an error of at most
 the softmax's argument); a weight p_j is off by the factor exp(2 ds) and a few
 e of the exponential (counted as 16 e); the sums over n positions run in
 partial sums of at most n / 16 + 64 terms. So
-    |out - ref| <= (2 ds + (80 + n / 16) e) sum_j p_j |v_j|.
+    |out - ref| <= (2 ds + (80 + n / 16) e) sum_j p_j |v_j| + n 2^-35 a.
+The last term is the smallest step of a weight's low half. The kernel holds
+p_j d_j (d: V's scales) in units of vref / 2^10 with vref <= max d, as two f16
+values whose smallest step is 2^-24: off by at most 2^-25 2^-10 max d, times a
+code of at most 8. The weights are relative to a maximum that one position
+has, so their sum is at least 1, and a position adds at most 2^-35 (8 max d);
+a = 8 max d <= 8/7 max |v|, because a block's largest code is -8 or 7.
 """
 import ctypes as C
 import random
@@ -338,7 +344,8 @@ def _reference(torch, q, start, lens, table, page, kv, vv, scale, seen=None):
             p = torch.softmax(s, 0)
             out[t] = (p[..., None] * v).sum(0)
             spread = (p[..., None] * v.abs()).sum(0)
-            tol[t] = (2 * ds[:, None] + (80 + int(m.sum()) / 16) * E) * spread
+            step = int(m.sum()) * 2.0 ** -35 * 8 / 7 * v.abs().amax((0, 2))
+            tol[t] = (2 * ds[:, None] + (80 + int(m.sum()) / 16) * E) * spread + step[:, None]
     return out, tol
 
 
