@@ -220,6 +220,18 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = h2_bits(__floats2half2_rn(-a, -b));
 }
 
+// The part of (x, y) that a lane holds: round(x), or with neg = -1.0 (f16)
+// round(x - round(x)).
+__device__ __forceinline__ uint32_t part2(float x, float y, uint32_t neg) {
+  const uint32_t hi = h2_bits(__floats2half2_rn(x, y));
+  float a, b;
+  asm("{\n\t.reg .f16 l, h, m, z;\n\tmov.b32 {l, h}, %2;\n\tmov.b32 {m, z}, %5;\n\t"
+      "fma.rn.f32.f16 %0, l, m, %3;\n\tfma.rn.f32.f16 %1, h, m, %4;\n\t}"
+      : "=f"(a), "=f"(b)
+      : "r"(hi), "f"(x), "f"(y), "r"(neg));
+  return h2_bits(__floats2half2_rn(a, b));
+}
+
 // The codes in nibbles 0..3 of both halves of x as exact signed integers:
 // 0x6400 | c is 1024 + c in f16, and 0x6400 | 16 c is 1024 + 16 c.
 __device__ __forceinline__ void codes4(uint32_t x, uint32_t* y) {
@@ -281,22 +293,25 @@ struct KvGeom {
 };
 
 // One warp's state for an item.
-template <int HD, int NT>
+template <int HD, int NT, bool SPLIT>
 struct KvState {
   static constexpr int NB = HD / 32;
-  uint32_t q[NT][NB][2][4];  // [..][k step]: b0 b1 of the high, b0 b1 of the low part
+  // [..][k step]: b0 b1 of the high, b0 b1 of the low part; SPLIT: of the
+  // part that the lane's column g holds (high for g < 4, low of column g - 4)
+  uint32_t q[NT][NB][2][SPLIT ? 2 : 4];
   float cn[NT][2];           // scores to log2 units
   int lim[NT][2];            // positions the column sees
   float m[NT][2], l[NT][2];
   float o[NT][NB][2][4];
   float vref, vinv;          // 2^floor(log2 max value scale), 2^10 / vref
+  uint32_t neg_hi;           // SPLIT: f16 -1 where the lane's columns are low parts, else 0
   bool first;                // no tile seen yet (uniform over the warp)
 };
 
 // One tile of 32 positions, two halves of 16, whose K and V rows are at k and
 // v; ok: the halves that were loaded (MASK: the others may hold anything).
-template <int HD, int NT, bool MASK>
-__device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, const uint8_t* v,
+template <int HD, int NT, bool SPLIT, bool MASK>
+__device__ __forceinline__ void kv_tile(KvState<HD, NT, SPLIT>& st, const uint8_t* k, const uint8_t* v,
                                         int pos0, int lim_max, int n_nt, int ok) {
   constexpr int NB = HD / 32;
   constexpr int ROW = NB * kQ4Bytes;
@@ -321,19 +336,30 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, c
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (NT > 1 && n >= n_nt) break;
-        // the small parts first: an MMA truncates its sum, and a truncation next
-        // to the small sums is worth nothing
         float c[4];
-        mma_f16_zero(c, a0[0], a1[0], a0[1], a1[1], st.q[n][b][0][2], st.q[n][b][0][3]);
-        mma_f16(c, a0[2], a1[2], a0[3], a1[3], st.q[n][b][1][2], st.q[n][b][1][3]);
-        mma_f16(c, a0[0], a1[0], a0[1], a1[1], st.q[n][b][0][0], st.q[n][b][0][1]);
-        mma_f16(c, a0[2], a1[2], a0[3], a1[3], st.q[n][b][1][0], st.q[n][b][1][1]);
+        const auto& q = st.q[n][b];
+        if constexpr (SPLIT) {
+          mma_f16_zero(c, a0[0], a1[0], a0[1], a1[1], q[0][0], q[0][1]);
+        } else {
+          // the small parts first: an MMA truncates its terms, and a truncation
+          // next to the small sums is worth nothing
+          mma_f16_zero(c, a0[0], a1[0], a0[1], a1[1], q[0][2], q[0][3]);
+          mma_f16(c, a0[2], a1[2], a0[3], a1[3], q[1][2], q[1][3]);
+          mma_f16(c, a0[0], a1[0], a0[1], a1[1], q[0][0], q[0][1]);
+        }
+        mma_f16(c, a0[2], a1[2], a0[3], a1[3], q[1][0], q[1][1]);
         s[u][n][0] = fmaf(c[0], d0, s[u][n][0]);
         s[u][n][1] = fmaf(c[1], d0, s[u][n][1]);
         s[u][n][2] = fmaf(c[2], d1, s[u][n][2]);
         s[u][n][3] = fmaf(c[3], d1, s[u][n][3]);
       }
     }
+  }
+  if (SPLIT) {  // columns n and n + 4 are the two parts of one
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[u][0][i] += __shfl_xor_sync(0xffffffffu, s[u][0][i], 2);
   }
   // value scales of positions g and g + 8 of each half
   float e[2][2][NB];
@@ -456,7 +482,7 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, c
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (NT > 1 && n >= n_nt) break;
-      uint32_t hi[2][2], lo[2][2];
+      uint32_t hi[2][2], lo[2][2];  // SPLIT: hi holds the lane's part
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -467,21 +493,30 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, c
             p0 = w0 == 0.0f ? 0.0f : p0;
             p1 = w1 == 0.0f ? 0.0f : p1;
           }
-          split2(p0, p1, hi[u][h], lo[u][h]);
-          hi[u][h] = transpose8x8(hi[u][h]);
-          lo[u][h] = transpose8x8(lo[u][h]);
+          if (SPLIT) {
+            hi[u][h] = transpose8x8(part2(p0, p1, st.neg_hi));
+          } else {
+            split2(p0, p1, hi[u][h], lo[u][h]);
+            hi[u][h] = transpose8x8(hi[u][h]);
+            lo[u][h] = transpose8x8(lo[u][h]);
+          }
         }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         // the tile's sum by itself, then added with rounding: MMAs into the
         // running sum would truncate it once each, always towards zero
         float c[4];
-        mma_f16_zero(c, y[0][0][2 * j], y[0][0][2 * j + 1], y[0][1][2 * j], y[0][1][2 * j + 1],
-                     lo[0][0], lo[0][1]);
-        mma_f16(c, y[1][0][2 * j], y[1][0][2 * j + 1], y[1][1][2 * j], y[1][1][2 * j + 1],
-                lo[1][0], lo[1][1]);
-        mma_f16(c, y[0][0][2 * j], y[0][0][2 * j + 1], y[0][1][2 * j], y[0][1][2 * j + 1],
-                hi[0][0], hi[0][1]);
+        if (SPLIT) {
+          mma_f16_zero(c, y[0][0][2 * j], y[0][0][2 * j + 1], y[0][1][2 * j], y[0][1][2 * j + 1],
+                       hi[0][0], hi[0][1]);
+        } else {  // the small parts first: a truncation next to them costs nothing
+          mma_f16_zero(c, y[0][0][2 * j], y[0][0][2 * j + 1], y[0][1][2 * j], y[0][1][2 * j + 1],
+                       lo[0][0], lo[0][1]);
+          mma_f16(c, y[1][0][2 * j], y[1][0][2 * j + 1], y[1][1][2 * j], y[1][1][2 * j + 1],
+                  lo[1][0], lo[1][1]);
+          mma_f16(c, y[0][0][2 * j], y[0][0][2 * j + 1], y[0][1][2 * j], y[0][1][2 * j + 1],
+                  hi[0][0], hi[0][1]);
+        }
         mma_f16(c, y[1][0][2 * j], y[1][0][2 * j + 1], y[1][1][2 * j], y[1][1][2 * j + 1],
                 hi[1][0], hi[1][1]);
         add2(st.o[n][b][j], c);
@@ -491,7 +526,7 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT>& st, const uint8_t* k, c
   }
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
     kv4_attend_kernel(const __grid_constant__ Kv4AttnParams p) {
   using GM = KvGeom<HD, NT>;
@@ -592,7 +627,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
   uint32_t fill = 0, used = 0;  // tiles issued / consumed by this warp so far
   int4 rec = make_int4(0, 0, 0, 0);
   bool alive = true;
-  KvState<HD, NT> st;
+  KvState<HD, NT, SPLIT> st;
   long long u = u0;
   while (u < u1) {
     const long long w = rq.base + (j + 1) * p.tpt;
@@ -613,7 +648,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
     int lim_min = lim_max;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int col = n * 8 + g, ct = col / p.gsz, ch = col - ct * p.gsz;
+      const int col = SPLIT ? g & 3 : n * 8 + g, ct = col / p.gsz, ch = col - ct * p.gsz;
       const bool on = ct < ntok && ch < nhead;
       const float* qp = p.q + (size_t)(rq.t0 + tok0 + (on ? ct : 0)) * p.q_stride +
                         (size_t)(h0 + (on ? ch : 0)) * HD + 8 * t;
@@ -633,14 +668,21 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
       const float f = __uint_as_float((uint32_t)(264 - ex) << 23);
       const float cn = p.scale * 1.4426950408889634f * (1.0f / f);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float* e = v[b] + 2 * x;
-          split2(e[0] * f, e[4] * f, st.q[n][b][x][0], st.q[n][b][x][2]);
-          split2(e[1] * f, e[5] * f, st.q[n][b][x][1], st.q[n][b][x][3]);
-        }
-      }
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float* e = v[b] + 2 * x + y;
+            uint32_t hi, lo;
+            split2(e[0] * f, e[4] * f, hi, lo);
+            if constexpr (SPLIT) {
+              st.q[n][b][x][y] = g < 4 ? hi : lo;
+            } else {
+              st.q[n][b][x][y] = hi;
+              st.q[n][b][x][y + 2] = lo;
+            }
+          }
       st.cn[n][0] = __shfl_sync(0xffffffffu, cn, 8 * t);
       st.cn[n][1] = __shfl_sync(0xffffffffu, cn, 8 * t + 4);
       long long lim = on ? (long long)prior + tok0 + ct + 1 : 0;
@@ -664,6 +706,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
     st.vref = 7.8886091e-31f;  // 2^-100
     st.vinv = 1024.0f / st.vref;
     st.first = true;
+    st.neg_hi = SPLIT && t >= 2 ? 0xbc00bc00u : 0u;
 
     // --- tiles [ta, tb) of the item, every kKvWarps-th from this warp's
     const long long n_tiles = (lim_max + kKvTile - 1) / kKvTile;
@@ -730,9 +773,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
         const int pos0 = (int)tile_pos(i);
         const uint8_t* kt = ring + sidx * 2 * GM::SIDE;
         if (pos0 + kKvTile > lim_min || ok != 3)
-          kv_tile<HD, NT, true>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
+          kv_tile<HD, NT, SPLIT, true>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
         else
-          kv_tile<HD, NT, false>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
+          kv_tile<HD, NT, SPLIT, false>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
       }
       __syncwarp();
       if (i + GM::STAGES < my) {
@@ -789,7 +832,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
     for (int i = tid; i < COLS * HD; i += kKvWarps * 32) {
       const int col = i / HD, d = i - col * HD;
       const int ct = col / p.gsz, ch = col - ct * p.gsz;
-      if (ct >= ntok || ch >= nhead) continue;
+      if (ct >= ntok || ch >= nhead || (SPLIT && col >= 4)) continue;
       float M = -3.0e38f, L = 0.0f, sum = 0.0f;
 #pragma unroll
       for (int x = 0; x < kKvWarps; ++x) M = fmaxf(M, s_ml[x * COLS + col].x);
@@ -797,7 +840,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
       for (int x = 0; x < kKvWarps; ++x) {
         const float2 ml = s_ml[x * COLS + col];
         L += ml.y * ex2(ml.x - M);
-        sum += reinterpret_cast<const float*>(ring_all + x * GM::PER_WARP)[col * GM::OP + d];
+        const float* a = reinterpret_cast<const float*>(ring_all + x * GM::PER_WARP);
+        sum += a[col * GM::OP + d];
+        if (SPLIT) sum += a[(col + 4) * GM::OP + d];
       }
       if (whole) {
         p.out[(size_t)(rq.t0 + tok0 + ct) * p.out_stride + (size_t)(h0 + ch) * HD + d] =
@@ -833,40 +878,56 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
 }
 
 // Joins the pieces of the item that starts in CTA blockIdx.x and goes on in
-// the next ones, in their order. One block per column.
+// the next ones. One block per column; warp w sums the pieces w, w + 4, ..
+// (a long history has a hundred), then the four sums are added in order.
 template <int HD>
-__global__ void __launch_bounds__(HD) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
+__global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
+  constexpr int PER = HD / 32;  // values per lane
+  __shared__ float s_o[4][HD];
+  __shared__ float s_l[4];
   pdl_wait();
-  const int c = blockIdx.x, col = blockIdx.y, cols = gridDim.y, d = threadIdx.x;
+  pdl_launch_dependents();
+  const int c = blockIdx.x, col = blockIdx.y, cols = gridDim.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int4 rec = p.rec[c];
   const int parts = min(rec.w, p.n_cta - c);
-  if (parts >= 2) {
-    const KvReq q = kv_req(p, rec.x);
-    const int kvh = rec.y / p.hgroups, hg = rec.y % p.hgroups;
-    const int ct = col / p.gsz, ch = col - ct * p.gsz;
-    const int tok = rec.z * p.tpt + ct, head = hg * p.gsz + ch;
-    if (tok < q.n && ct < p.tpt && head < p.nh / p.nkv) {
-      auto at = [&](int i) { return ((size_t)(c + i) * 2 + (i == 0 ? 1 : 0)) * cols + col; };
-      float M = -3.0e38f;
-      for (int i = 0; i < parts; ++i) M = fmaxf(M, p.part_ml[at(i) * 2]);
-      float L = 0.0f, sum = 0.0f;
+  if (parts < 2) return;
+  const KvReq q = kv_req(p, rec.x);
+  const int kvh = rec.y / p.hgroups, hg = rec.y % p.hgroups;
+  const int ct = col / p.gsz, ch = col - ct * p.gsz;
+  const int tok = rec.z * p.tpt + ct, head = hg * p.gsz + ch;
+  if (tok >= q.n || ct >= p.tpt || head >= p.nh / p.nkv) return;
+  auto at = [&](int i) { return ((size_t)(c + i) * 2 + (i == 0 ? 1 : 0)) * cols + col; };
+  float M = -3.0e38f;
+  for (int i = lane; i < parts; i += 32) M = fmaxf(M, p.part_ml[at(i) * 2]);
+  M = warp_max(M);
+  float L = 0.0f, sum[PER] = {};
 #pragma unroll 4
-      for (int i = 0; i < parts; ++i) {
-        const float f = ex2(p.part_ml[at(i) * 2] - M);
-        L += p.part_ml[at(i) * 2 + 1] * f;
-        sum += p.part_o[at(i) * HD + d] * f;
-      }
-      p.out[(size_t)(q.t0 + tok) * p.out_stride +
-            (size_t)(kvh * (p.nh / p.nkv) + head) * HD + d] = L != 0.0f ? sum / L : 0.0f;
-    }
+  for (int i = warp; i < parts; i += 4) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(i) * 2);
+    const float f = ex2(ml.x - M);
+    L += ml.y * f;
+    const float* o = p.part_o + at(i) * HD + PER * lane;
+#pragma unroll
+    for (int d = 0; d < PER; ++d) sum[d] += o[d] * f;
   }
-  pdl_launch_dependents();
+#pragma unroll
+  for (int d = 0; d < PER; ++d) s_o[warp][PER * lane + d] = sum[d];
+  if (lane == 0) s_l[warp] = L;
+  __syncthreads();
+  L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  for (int d = threadIdx.x; d < HD; d += 128) {
+    const float o = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]);
+    p.out[(size_t)(q.t0 + tok) * p.out_stride + (size_t)(kvh * (p.nh / p.nkv) + head) * HD + d] =
+        L != 0.0f ? o / L : 0.0f;
+  }
 }
 
 // How the tensor-core kernel is launched for a call, or n_cta = 0 where the
 // rows kernel serves it.
 struct KvPlan {
   int nt, n_cta;
+  bool split;  // columns hold the two parts of q: up to 4 columns a tile
   size_t ws;
 };
 KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_t hd) {
@@ -874,18 +935,19 @@ KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_
   if ((hd != 64 && hd != 128) || n_kv == 0 || n_req == 0) return k;
   const size_t G = n_heads / n_kv;
   k.nt = G > 8 || n_tokens > n_req ? 2 : 1;
+  k.split = k.nt == 1 && G <= 4;
   k.n_cta = sm_count() * (k.nt == 1 ? 4 : 2);
   k.ws = (size_t)k.n_cta * (2 * 8 * k.nt * (hd + 2) * 4 + sizeof(int4));
   return k;
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool SPLIT>
 minq_status launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
   using GM = KvGeom<HD, NT>;
-  MINQ_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kv4_attend_kernel<HD, NT>), GM::SMEM));
-  MINQ_CUDA_TRY(launch_k(kv4_attend_kernel<HD, NT>, dim3(p.n_cta), dim3(kKvWarps * 32), GM::SMEM, s,
+  MINQ_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kv4_attend_kernel<HD, NT, SPLIT>), GM::SMEM));
+  MINQ_CUDA_TRY(launch_k(kv4_attend_kernel<HD, NT, SPLIT>, dim3(p.n_cta), dim3(kKvWarps * 32), GM::SMEM, s,
                          p));
-  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3(p.n_cta, GM::COLS), dim3(HD), 0, s, p));
+  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3(p.n_cta, GM::COLS), dim3(128), 0, s, p));
   return MINQ_OK;
 }
 
@@ -963,18 +1025,22 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
   p.out = out;
   p.out_stride = out_stride;
   if (plan.ws) {
-    const int G = (int)(n_heads / n_kv), cols = 8 * plan.nt;
-    p.gsz = G < cols ? G : cols;
+    const int G = (int)(n_heads / n_kv), cols = 8 * plan.nt, most = plan.split ? 4 : cols;
+    p.gsz = G < most ? G : most;
     p.hgroups = (G + p.gsz - 1) / p.gsz;
-    p.tpt = cols / p.gsz;
+    p.tpt = most / p.gsz;
     p.n_cta = plan.n_cta;
     p.rec = static_cast<int4*>(workspace);
     p.part_o = reinterpret_cast<float*>(p.rec + plan.n_cta);
     p.part_ml = p.part_o + (size_t)plan.n_cta * 2 * cols * head_dim;
     cudaStream_t s = (cudaStream_t)stream;
     if (head_dim == 64)
-      return plan.nt == 1 ? launch_kv4_attend<64, 1>(p, s) : launch_kv4_attend<64, 2>(p, s);
-    return plan.nt == 1 ? launch_kv4_attend<128, 1>(p, s) : launch_kv4_attend<128, 2>(p, s);
+      return plan.split     ? launch_kv4_attend<64, 1, true>(p, s)
+             : plan.nt == 1 ? launch_kv4_attend<64, 1, false>(p, s)
+                            : launch_kv4_attend<64, 2, false>(p, s);
+    return plan.split     ? launch_kv4_attend<128, 1, true>(p, s)
+           : plan.nt == 1 ? launch_kv4_attend<128, 1, false>(p, s)
+                          : launch_kv4_attend<128, 2, false>(p, s);
   }
   const size_t rows = n_tokens * n_heads;
   MINQ_CUDA_TRY(launch_k(kv4_attend_rows_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0,
