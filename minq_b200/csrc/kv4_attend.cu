@@ -31,8 +31,8 @@
 // has its positions along k; two positions' codes are paired by one byte
 // permutation of their words.
 //
-// Each warp owns every NW-th tile of 32 positions and keeps its own running
-// maximum, sum and accumulator; its K and V rows (16 or 32 rows of one
+// Each warp works through its own tiles of 32 positions and keeps its own
+// running maximum, sum and accumulator; its K and V rows (16 or 32 rows of one
 // page: a contiguous run each) come by bulk copies into a private ring, so no warp waits
 // for another until the item's end. The maximum is only moved when a weight
 // would exceed 2^4 (one vote a tile), which leaves the accumulator alone
@@ -40,11 +40,12 @@
 //
 // Work split. An item is (request, kv head, column tile); its weight is its
 // number of positions plus a constant for its start and end. The items of the
-// step lie on one line, and CTA c takes the c-th of equal pieces of it,
-// computed on the device from the lengths (no host synchronisation, graphs
-// replay over changing lengths). An item that lies in one CTA is written out
-// directly; the pieces of the others go to the workspace and a second small
-// launch joins them in a fixed order, so results repeat bit for bit.
+// step lie on one line, and every warp takes an equal piece of it, computed on
+// the device from the lengths (no host synchronisation, graphs replay over
+// changing lengths). An item inside one warp's piece is written out directly;
+// the pieces of the others go to the workspace, one per warp, or one per CTA
+// where an item fills it, and a second small launch joins them in a fixed
+// order, so results repeat bit for bit.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -57,6 +58,12 @@
 namespace minq {
 
 namespace {
+
+// The item that starts in a warp's piece of the line and goes on behind it.
+struct KvRec {
+  int parts, r, h, j;  // number of pieces (0: no item), request, head tile, column tile
+  int a, n_first, n_mid, z0;  // first piece and pieces in its CTA, CTAs between, first in the last
+};
 
 struct Kv4AttnParams {
   const float* q;  // token t, head h at q + t * q_stride + h * hd
@@ -75,12 +82,12 @@ struct Kv4AttnParams {
   float* out;
   size_t out_stride;
   // tensor-core kernel
-  int gsz, hgroups, tpt;  // columns: heads per group tile, tiles per kv head, tokens per tile
+  // columns of a tile (room for), heads per tile, head tiles per kv head, tokens per tile
+  int cols, gsz, hgroups, tpt;
   int n_cta;
-  float* part_o;   // [n_cta][2][cols][hd] unnormalised partial outputs
-  float* part_ml;  // [n_cta][2][cols][2] their maxima and sums
-  int4* rec;       // [n_cta] the split item that starts in this CTA: (request, head tile, column
-                   // tile, parts)
+  float* part_o;   // [n_cta * warps][2][cols][hd] unnormalised partial outputs
+  float* part_ml;  // [n_cta * warps][2][cols][2] their maxima and sums
+  KvRec* rec;      // [n_cta * warps]
 };
 
 // Request of token t, or -1 where t lies behind the last sequence (or the
@@ -177,8 +184,8 @@ __device__ int g_kv4_status;
 
 constexpr int kKvWarps = 4;
 constexpr int kKvTile = 32;     // positions per tile
-constexpr int kKvItem = 256;    // an item's start and end, in positions
-constexpr int kKvMinPiece = 128;  // positions per CTA below which an item is not split further
+constexpr int kKvItem = 64;     // an item's start and end, in positions
+constexpr int kKvMinPiece = 96;  // smallest piece of the line per warp
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -220,6 +227,13 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = h2_bits(__floats2half2_rn(-a, -b));
 }
 
+// (x & m) | o as one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(m), "r"(o));
+  return d;
+}
+
 // The part of (x, y) that a lane holds: round(x), or with neg = -1.0 (f16)
 // round(x - round(x)).
 __device__ __forceinline__ uint32_t part2(float x, float y, uint32_t neg) {
@@ -238,10 +252,10 @@ __device__ __forceinline__ void codes4(uint32_t x, uint32_t* y) {
   const __half2 m8 = __float2half2_rn(-1032.0f), m72 = __float2half2_rn(-72.0f),
                 r16 = __float2half2_rn(0.0625f);
   const uint32_t z = x >> 8;
-  y[0] = h2_bits(__hadd2(bits_h2((x & 0x000f000fu) | 0x64006400u), m8));
-  y[1] = h2_bits(__hfma2(bits_h2((x & 0x00f000f0u) | 0x64006400u), r16, m72));
-  y[2] = h2_bits(__hadd2(bits_h2((z & 0x000f000fu) | 0x64006400u), m8));
-  y[3] = h2_bits(__hfma2(bits_h2((z & 0x00f000f0u) | 0x64006400u), r16, m72));
+  y[0] = h2_bits(__hadd2(bits_h2(and_or(x, 0x000f000fu, 0x64006400u)), m8));
+  y[1] = h2_bits(__hfma2(bits_h2(and_or(x, 0x00f000f0u, 0x64006400u)), r16, m72));
+  y[2] = h2_bits(__hadd2(bits_h2(and_or(z, 0x000f000fu, 0x64006400u)), m8));
+  y[3] = h2_bits(__hfma2(bits_h2(and_or(z, 0x00f000f0u, 0x64006400u)), r16, m72));
 }
 
 // o[0..1] += c[0..1], one packed addition.
@@ -526,28 +540,293 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT, SPLIT>& st, const uint8_
   }
 }
 
+// One item: tokens [tok0, tok0 + ntok) of a request for the heads [h0, h0 +
+// nhead), at [start, start + w) on the line.
+struct KvItem {
+  KvReq rq;
+  int h;        // head tile
+  long long j;  // column tile
+  long long start, w;
+  int kvh, h0, nhead, tok0, ntok, prior, lim_max;
+  long long cap;
+  long long x0, x1;  // the part of it that this warp (or CTA) takes
+};
+__device__ __forceinline__ void kv_item_set(const Kv4AttnParams& p, KvItem& it) {
+  const int G = p.nh / p.nkv, hg = it.h % p.hgroups;
+  it.w = it.rq.base + (it.j + 1) * p.tpt;
+  it.kvh = it.h / p.hgroups;
+  it.h0 = it.kvh * G + hg * p.gsz;
+  it.nhead = min(p.gsz, G - hg * p.gsz);
+  it.tok0 = (int)(it.j * p.tpt);
+  it.ntok = min(p.tpt, it.rq.n - it.tok0);
+  it.prior = it.rq.len - it.rq.n;
+  // positions of the table row (tile ends stay inside 31 bits)
+  it.cap = min((long long)p.table_stride << p.page_shift, 0x7fffff00ll);
+  // positions that the last token sees
+  const long long lim = min((long long)it.prior + it.tok0 + it.ntok, it.cap);
+  it.lim_max = lim > 0 ? (int)lim : 0;
+}
+// The item at u, in the request r that starts at `start` on the line.
+__device__ __forceinline__ void kv_item_at(const Kv4AttnParams& p, KvItem& it, int r,
+                                           long long start, long long u) {
+  it.rq = kv_req(p, r);
+  const long long W = kv_cum(it.rq, p.tpt, it.rq.J), off = u - start;
+  it.h = (int)(off / W);
+  const long long x = off - it.h * W;
+  long long lo = 0, hi = it.rq.J;
+  while (hi - lo > 1) {
+    const long long mid = (lo + hi) >> 1;
+    if (kv_cum(it.rq, p.tpt, mid) <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  it.j = lo;
+  it.start = start + it.h * W + kv_cum(it.rq, p.tpt, lo);
+  kv_item_set(p, it);
+}
+// The next item on the line; false behind the last one.
+__device__ __forceinline__ bool kv_item_next(const Kv4AttnParams& p, KvItem& it) {
+  it.start += it.w;
+  if (++it.j == it.rq.J) {
+    it.j = 0;
+    if (++it.h == p.nkv * p.hgroups) {
+      it.h = 0;
+      int r = it.rq.r;
+      do {
+        if (++r >= p.n_req) return false;
+        it.rq = kv_req(p, r);
+      } while (it.rq.J == 0);
+    }
+  }
+  kv_item_set(p, it);
+  return true;
+}
+
+// The pieces of an item that starts in piece a: the warps' in the first and the
+// last CTA that it touches, and one per CTA that it fills.
+__device__ __forceinline__ KvRec kv_parts(const KvItem& it, int a, long long per, long long total) {
+  const long long end = it.start + it.w, cta = per * kKvWarps;
+  const int z = (int)((end - 1) / per), ca = a / kKvWarps, cz = z / kKvWarps;
+  auto full = [&](int c) { return cta * c >= it.start && min(cta * (c + 1), total) <= end; };
+  KvRec k;
+  k.r = it.rq.r;
+  k.h = it.h;
+  k.j = (int)it.j;
+  k.a = a;
+  k.z0 = cz * kKvWarps;
+  k.n_first = full(ca) ? 1 : min(z, ca * kKvWarps + kKvWarps - 1) - a + 1;
+  k.n_mid = cz > ca ? cz - ca - 1 : 0;
+  k.parts = k.n_first + k.n_mid + (cz > ca ? (full(cz) ? 1 : z - k.z0 + 1) : 0);
+  return k;
+}
+
+// A warp's ring of tiles in flight.
+struct KvRing {
+  uint8_t* buf;
+  uint64_t* bar;
+  uint32_t fill, used;  // tiles issued and consumed so far
+  bool alive;           // no wait has given up
+};
+
+// One warp's share of the part [x0, x1) of an item: every step-th of its tiles
+// from tile `lead` on.
+template <int HD, int NT, bool SPLIT>
+__device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it, int lead, int step,
+                                       KvRing& ring, KvState<HD, NT, SPLIT>& st) {
+  using GM = KvGeom<HD, NT>;
+  constexpr int NB = GM::NB;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n_tiles = (it.lim_max + kKvTile - 1) / kKvTile;
+  auto tile_at = [](long long x) { return x > kKvItem ? (x - kKvItem + kKvTile - 1) / kKvTile : 0; };
+  const long long xa = tile_at(it.x0), xb = it.x1 == it.w ? n_tiles : tile_at(it.x1);
+  const int ta = (int)min(xa, (long long)n_tiles) + lead, tb = (int)min(xb, (long long)n_tiles);
+  const int my = tb > ta ? (tb - ta + step - 1) / step : 0;
+  const int lim_max = it.lim_max;
+  const size_t row0 = ((size_t)it.kvh << p.page_shift) * GM::ROW;
+  const size_t page_bytes = ((size_t)p.nkv << p.page_shift) * GM::ROW;
+  const int* tab = p.table + (size_t)it.rq.r * p.table_stride;
+  // page ids of the halves of this warp's next 16 tiles, one per lane; -1
+  // behind the last position
+  auto tile_pos = [&](int i) { return (ta + i * step) * kKvTile; };
+  auto load_ids = [&](int i0) {
+    const int i = i0 + (lane >> 1);
+    const int pos = tile_pos(i) + 16 * (lane & 1);
+    int id = -1;
+    if (i < my && pos < lim_max) id = tab[pos >> p.page_shift];
+    return id < p.n_pages ? id : -1;
+  };
+  int ids = load_ids(0);
+  // the columns' queries
+  float v[NT][NB][8];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = SPLIT ? g & 3 : n * 8 + g, ct = col / p.gsz, ch = col - ct * p.gsz;
+    const bool on = ct < it.ntok && ch < it.nhead;
+    const float* qp = p.q + (size_t)(it.rq.t0 + it.tok0 + (on ? ct : 0)) * p.q_stride +
+                      (size_t)(it.h0 + (on ? ch : 0)) * HD + 8 * t;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[n][b][e] = on ? qp[b * 32 + e] : 0.0f;
+  }
+  auto issue = [&](int i, int id0, int id1) {  // lane 0
+    const uint32_t sidx = ring.fill % GM::STAGES;
+    uint64_t* bar = &ring.bar[sidx];
+    const int in_page = tile_pos(i) & ((1 << p.page_shift) - 1);
+    uint8_t* dst = ring.buf + sidx * 2 * GM::SIDE;
+    const uint32_t n = (id0 >= 0) + (id1 >= 0);
+    if (n == 0) {
+      mbar_arrive(bar);
+      return;
+    }
+    mbar_arrive_expect_tx(bar, n * 2 * GM::HALF);
+    if (n == 2 && p.page_shift > 4) {  // both halves in one page
+      const size_t off = (size_t)id0 * page_bytes + row0 + in_page * GM::ROW;
+      bulk_g2s(dst, p.k_pages + off, GM::SIDE, bar);
+      bulk_g2s(dst + GM::SIDE, p.v_pages + off, GM::SIDE, bar);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int id = x ? id1 : id0;
+        if (id < 0) continue;
+        const size_t off = (size_t)id * page_bytes + row0 +
+                           (p.page_shift > 4 ? in_page + 16 * x : 0) * GM::ROW;
+        bulk_g2s(dst + x * GM::HALF, p.k_pages + off, GM::HALF, bar);
+        bulk_g2s(dst + GM::SIDE + x * GM::HALF, p.v_pages + off, GM::HALF, bar);
+      }
+    }
+  };
+  const int first = min(my, GM::STAGES);
+  for (int i = 0; i < first; ++i) {
+    const int a = __shfl_sync(0xffffffffu, ids, 2 * i);
+    const int b = __shfl_sync(0xffffffffu, ids, 2 * i + 1);
+    if (lane == 0 && ring.alive) issue(i, a, b);
+    ++ring.fill;
+  }
+  int ids_next = my > 16 ? load_ids(16) : -1;
+
+  // q as f16 parts, limits
+  const int n_nt = (it.ntok * p.gsz + 7) / 8;
+  int lim_min = it.lim_max;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = SPLIT ? g & 3 : n * 8 + g, ct = col / p.gsz, ch = col - ct * p.gsz;
+    const bool on = ct < it.ntok && ch < it.nhead;
+    float amax = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[n][b][e]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // f: a power of two with amax * f in [2^10, 2^11)
+    const int ex = min(max((int)(__float_as_uint(amax) >> 23), 24), 254);
+    const float f = __uint_as_float((uint32_t)(264 - ex) << 23);
+    const float cn = p.scale * 1.4426950408889634f * (1.0f / f);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float* e = v[n][b] + 2 * x + y;
+          uint32_t hi, lo;
+          split2(e[0] * f, e[4] * f, hi, lo);
+          if constexpr (SPLIT) {
+            st.q[n][b][x][y] = g < 4 ? hi : lo;
+          } else {
+            st.q[n][b][x][y] = hi;
+            st.q[n][b][x][y + 2] = lo;
+          }
+        }
+    st.cn[n][0] = __shfl_sync(0xffffffffu, cn, 8 * t);
+    st.cn[n][1] = __shfl_sync(0xffffffffu, cn, 8 * t + 4);
+    long long lim = on ? (long long)it.prior + it.tok0 + ct + 1 : 0;
+    lim = lim < 0 ? 0 : lim < it.cap ? lim : it.cap;
+    st.lim[n][0] = __shfl_sync(0xffffffffu, (int)lim, 8 * t);
+    st.lim[n][1] = __shfl_sync(0xffffffffu, (int)lim, 8 * t + 4);
+    if (on) lim_min = min(lim_min, (int)lim);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      st.m[n][c] = 0.0f;
+      st.l[n][c] = 0.0f;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[n][b][y][i] = 0.0f;
+  }
+  lim_min = (int)__reduce_min_sync(0xffffffffu, (unsigned)lim_min);
+  st.vref = 7.8886091e-31f;  // 2^-100
+  st.vinv = 1024.0f / st.vref;
+  st.first = true;
+  st.neg_hi = SPLIT && t >= 2 ? 0xbc00bc00u : 0u;
+
+  for (int i = 0; i < my; ++i) {
+    const uint32_t sidx = ring.used % GM::STAGES;
+    if (ring.alive)
+      ring.alive = mbar_wait_timed(&ring.bar[sidx], (ring.used / GM::STAGES) & 1, &g_kv4_status);
+    ring.alive = __all_sync(0xffffffffu, ring.alive);
+    ++ring.used;
+    const int ok = (int)(__ballot_sync(0xffffffffu, ids >= 0) >> (2 * (i & 15))) & 3;
+    if (ring.alive && ok) {
+      const int pos0 = tile_pos(i);
+      const uint8_t* kt = ring.buf + sidx * 2 * GM::SIDE;
+      if (pos0 + kKvTile > lim_min || ok != 3)
+        kv_tile<HD, NT, SPLIT, true>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
+      else
+        kv_tile<HD, NT, SPLIT, false>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
+    }
+    __syncwarp();
+    if (i + GM::STAGES < my) {
+      const int nx = i + GM::STAGES, src = 2 * (nx & 15);
+      const int from = (nx >> 4) == (i >> 4) ? ids : ids_next;
+      const int a = __shfl_sync(0xffffffffu, from, src);
+      const int b = __shfl_sync(0xffffffffu, from, src + 1);
+      if (lane == 0 && ring.alive) issue(nx, a, b);
+      ++ring.fill;
+    }
+    if ((i & 15) == 15) {
+      ids = ids_next;
+      ids_next = load_ids(i + 17);
+    }
+  }
+  // sums over the positions' lanes
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int o = 4; o <= 16; o <<= 1)
+        st.l[n][c] += __shfl_xor_sync(0xffffffffu, st.l[n][c], o);
+      if (st.l[n][c] == 0.0f) st.m[n][c] = -3.0e38f;  // saw nothing
+    }
+}
+
 template <int HD, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
     kv4_attend_kernel(const __grid_constant__ Kv4AttnParams p) {
   using GM = KvGeom<HD, NT>;
   constexpr int NB = GM::NB, COLS = GM::COLS;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* ring_all = smem;
   float2* s_ml = reinterpret_cast<float2*>(smem + kKvWarps * GM::PER_WARP);  // [warp][cols]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_ml + kKvWarps * COLS);
   __shared__ long long s_red[kKvWarps];
-  __shared__ long long s_find[2];  // request and offset at this CTA's start
+  __shared__ long long s_start[kKvWarps];  // the request at each warp's start: its place
+  __shared__ int s_req[kKvWarps];          // and its number
+  __shared__ KvItem s_item[kKvWarps];      // the warps' items
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int cta = blockIdx.x;
-  uint8_t* ring = ring_all + warp * GM::PER_WARP;
-  uint64_t* bar = bars + warp * GM::STAGES;
-  if (lane < GM::STAGES) mbar_init(&bar[lane], 1);
+  KvRing ring{smem + warp * GM::PER_WARP, bars + warp * GM::STAGES, 0, 0, true};
+  if (lane < GM::STAGES) mbar_init(&ring.bar[lane], 1);
   mbar_fence_init();
   pdl_wait();
   pdl_launch_dependents();
 
-  // where this CTA's piece of the line starts
+  // the line's length, and where the warps' pieces start
   const int H = p.nkv * p.hgroups;
   long long total = 0;
   for (int r = tid; r < p.n_req; r += kKvWarps * 32) {
@@ -558,17 +837,18 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_red[warp] = total;
-  if (tid == 0) s_find[0] = -1;
+  if (tid < kKvWarps) s_req[tid] = -1;
   __syncthreads();
   total = 0;
 #pragma unroll
   for (int w = 0; w < kKvWarps; ++w) total += s_red[w];
-  long long per = (total + p.n_cta - 1) / p.n_cta;
-  const long long least = kKvMinPiece + kKvItem;
-  if (per < least) per = least;
-  const long long u0 = per * cta, u1 = u0 + per < total ? u0 + per : total;
-  if (u0 >= u1) {
-    if (tid == 0) p.rec[cta] = make_int4(0, 0, 0, 0);
+  const int n_piece = p.n_cta * kKvWarps;
+  long long per = (total + n_piece - 1) / n_piece;
+  if (per < kKvMinPiece) per = kKvMinPiece;
+  const long long c0 = per * kKvWarps * blockIdx.x, c1 = min(c0 + per * kKvWarps, total);
+  KvRec* rec = p.rec + blockIdx.x * kKvWarps;
+  if (c0 >= c1) {
+    if (tid < kKvWarps) rec[tid].parts = 0;
     return;
   }
   long long before = 0;  // weight of the requests of earlier rounds
@@ -596,330 +876,229 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
       if (x < warp) start += s_red[x];
       before += s_red[x];
     }
-    if (r < p.n_req && start <= u0 && u0 < start + w) {
-      s_find[0] = r;
-      s_find[1] = start;
-    }
-    if (before > u0) break;  // uniform
+    if (r < p.n_req)
+#pragma unroll
+      for (int x = 0; x < kKvWarps; ++x) {
+        const long long u = c0 + per * x;
+        if (start <= u && u < start + w) {
+          s_req[x] = r;
+          s_start[x] = start;
+        }
+      }
+    if (before > c1) break;  // uniform
   }
   __syncthreads();
-  if (s_find[0] < 0) return;  // cannot happen: the line's pieces cover it
-  KvReq rq = kv_req(p, (int)s_find[0]);
-  long long s0;  // start of the current item on the line
-  int h;         // its head tile
-  long long j;   // its column tile
-  {
-    const long long W = kv_cum(rq, p.tpt, rq.J), off = u0 - s_find[1];
-    h = (int)(off / W);
-    const long long x = off - h * W;
-    long long lo = 0, hi = rq.J;
-    while (hi - lo > 1) {
-      const long long mid = (lo + hi) >> 1;
-      if (kv_cum(rq, p.tpt, mid) <= x)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    j = lo;
-    s0 = s_find[1] + h * W + kv_cum(rq, p.tpt, j);
-  }
+  if (s_req[0] < 0) return;  // cannot happen: the items cover the line
 
-  uint32_t fill = 0, used = 0;  // tiles issued / consumed by this warp so far
-  int4 rec = make_int4(0, 0, 0, 0);
-  bool alive = true;
   KvState<HD, NT, SPLIT> st;
-  long long u = u0;
-  while (u < u1) {
-    const long long w = rq.base + (j + 1) * p.tpt;
-    const long long x0 = u - s0, x1 = (u1 - s0 < w ? u1 - s0 : w);
-    const int kvh = h / p.hgroups, h0 = kvh * (p.nh / p.nkv) + (h % p.hgroups) * p.gsz;
-    const int nhead = min(p.gsz, p.nh / p.nkv - (h % p.hgroups) * p.gsz);
-    const int tok0 = (int)(j * p.tpt), ntok = min(p.tpt, rq.n - tok0);
-    const int prior = rq.len - rq.n;
-    // positions of the table row (tile ends stay inside 31 bits)
-    const long long cap = min((long long)p.table_stride << p.page_shift, 0x7fffff00ll);
-    // positions that the tile's last token sees
-    long long lim_all = (long long)prior + tok0 + ntok;
-    lim_all = lim_all < cap ? lim_all : cap;
-    const int lim_max = lim_all > 0 ? (int)lim_all : 0;
-    const int n_nt = (ntok * p.gsz + 7) / 8;
-
-    // --- columns: q as f16 parts, limits
-    int lim_min = lim_max;
+  KvItem& it = s_item[warp];
+  // One item that fills the whole CTA: the warps take turns at its tiles and
+  // join in shared memory. Otherwise every warp takes its own piece of the line.
+  bool joint;
+  long long end;
+  {
+    KvItem x;
+    kv_item_at(p, x, s_req[0], s_start[0], c0);
+    joint = x.start + x.w >= c1;
+    const long long u = joint ? c0 : c0 + per * warp;
+    end = joint ? c1 : min(u + per, total);
+    if (lane == 0) rec[warp].parts = 0;
+    if (!joint && warp) {
+      if (u >= end || s_req[warp] < 0) return;
+      kv_item_at(p, x, s_req[warp], s_start[warp], u);
+    }
+    x.x0 = u - x.start;
+    x.x1 = min(end - x.start, x.w);
+    if (lane == 0) it = x;
+    __syncwarp();
+  }
+  for (;;) {
+    kv_run<HD, NT, SPLIT>(p, it, joint ? warp : 0, joint ? kKvWarps : 1, ring, st);
+    const bool whole = it.x0 == 0 && it.x1 == it.w;
+    const int slot = it.x0 > 0 ? 0 : 1;
+    if (!whole && slot == 1 && lane == 0 && (!joint || warp == 0))
+      rec[warp] = kv_parts(it, blockIdx.x * kKvWarps + warp, per, total);
+    if (joint) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int col = SPLIT ? g & 3 : n * 8 + g, ct = col / p.gsz, ch = col - ct * p.gsz;
-      const bool on = ct < ntok && ch < nhead;
-      const float* qp = p.q + (size_t)(rq.t0 + tok0 + (on ? ct : 0)) * p.q_stride +
-                        (size_t)(h0 + (on ? ch : 0)) * HD + 8 * t;
-      float v[NB][8];
-      float amax = 0.0f;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+        for (int c = 0; c < 2; ++c)
+          if (g == 0) s_ml[warp * COLS + n * 8 + 2 * t + c] = make_float2(st.m[n][c], st.l[n][c]);
+      __syncthreads();
+      float* area = reinterpret_cast<float*>(ring.buf);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[b][e] = on ? qp[b * 32 + e] : 0.0f;
-          amax = fmaxf(amax, fabsf(v[b][e]));
+      for (int n = 0; n < NT; ++n) {
+        float f[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float M = -3.0e38f;
+#pragma unroll
+          for (int x = 0; x < kKvWarps; ++x)
+            M = fmaxf(M, s_ml[x * COLS + n * 8 + 2 * t + c].x);
+          f[c] = ex2(st.m[n][c] - M) * (st.vref * 0.0009765625f);
         }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // f: a power of two with amax * f in [2^10, 2^11)
-      const int ex = min(max((int)(__float_as_uint(amax) >> 23), 24), 254);
-      const float f = __uint_as_float((uint32_t)(264 - ex) << 23);
-      const float cn = p.scale * 1.4426950408889634f * (1.0f / f);
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const float* e = v[b] + 2 * x + y;
-            uint32_t hi, lo;
-            split2(e[0] * f, e[4] * f, hi, lo);
-            if constexpr (SPLIT) {
-              st.q[n][b][x][y] = g < 4 ? hi : lo;
-            } else {
-              st.q[n][b][x][y] = hi;
-              st.q[n][b][x][y + 2] = lo;
-            }
+            float* a = area + (n * 8 + 2 * t) * GM::OP + b * 32 + 4 * g + 2 * y;
+            const float* o = st.o[n][b][y];
+            *reinterpret_cast<float2*>(a) = make_float2(o[0] * f[0], o[2] * f[0]);
+            *reinterpret_cast<float2*>(a + GM::OP) = make_float2(o[1] * f[1], o[3] * f[1]);
           }
-      st.cn[n][0] = __shfl_sync(0xffffffffu, cn, 8 * t);
-      st.cn[n][1] = __shfl_sync(0xffffffffu, cn, 8 * t + 4);
-      long long lim = on ? (long long)prior + tok0 + ct + 1 : 0;
-      lim = lim < 0 ? 0 : lim < cap ? lim : cap;
-      st.lim[n][0] = __shfl_sync(0xffffffffu, (int)lim, 8 * t);
-      st.lim[n][1] = __shfl_sync(0xffffffffu, (int)lim, 8 * t + 4);
-      if (on) lim_min = min(lim_min, (int)lim);
+      }
+      __syncthreads();
+      for (int i = tid; i < (SPLIT ? 4 : COLS) * HD; i += kKvWarps * 32) {
+        const int col = i / HD, d = i - col * HD;
+        const int ct = col / p.gsz, ch = col - ct * p.gsz;
+        if (ct >= it.ntok || ch >= it.nhead) continue;
+        float M = -3.0e38f, L = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kKvWarps; ++x) M = fmaxf(M, s_ml[x * COLS + col].x);
+#pragma unroll
+        for (int x = 0; x < kKvWarps; ++x) {
+          const float2 ml = s_ml[x * COLS + col];
+          L += ml.y * ex2(ml.x - M);
+          const float* a = reinterpret_cast<const float*>(smem + x * GM::PER_WARP);
+          sum += a[col * GM::OP + d];
+          if (SPLIT) sum += a[(col + 4) * GM::OP + d];
+        }
+        if (whole) {
+          p.out[(size_t)(it.rq.t0 + it.tok0 + ct) * p.out_stride + (size_t)(it.h0 + ch) * HD + d] =
+              L != 0.0f ? sum / L : 0.0f;
+        } else {
+          const size_t at = ((size_t)blockIdx.x * kKvWarps * 2 + slot) * COLS + col;
+          p.part_o[at * HD + d] = sum;
+          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
+        }
+      }
+      return;
+    }
+    const size_t at = ((size_t)(blockIdx.x * kKvWarps + warp) * 2 + slot) * COLS;
+    const float f = st.vref * 0.0009765625f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float* dst[2];
+      float r[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        st.m[n][c] = 0.0f;
-        st.l[n][c] = 0.0f;
+        const int col = SPLIT ? (2 * t + c) & 3 : n * 8 + 2 * t + c;
+        const int ct = col / p.gsz, ch = col - ct * p.gsz;
+        const float L = st.l[n][c];
+        const bool on = ct < it.ntok && ch < it.nhead && (!SPLIT || t < 2);
+        r[c] = !whole ? f : L != 0.0f ? f / L : 0.0f;
+        dst[c] = !on     ? nullptr
+                 : whole ? p.out + (size_t)(it.rq.t0 + it.tok0 + ct) * p.out_stride +
+                               (size_t)(it.h0 + ch) * HD
+                         : p.part_o + (at + col) * HD;
+        if (on && !whole && g == 0)
+          *reinterpret_cast<float2*>(p.part_ml + (at + col) * 2) = make_float2(st.m[n][c], L);
       }
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int y = 0; y < 2; ++y)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) st.o[n][b][y][i] = 0.0f;
+          for (int i = 0; i < 4; ++i) {
+            float o = st.o[n][b][y][i];
+            if (SPLIT) o += __shfl_xor_sync(0xffffffffu, o, 2);
+            if (dst[i & 1]) dst[i & 1][b * 32 + 4 * g + 2 * y + (i >> 1)] = o * r[i & 1];
+          }
     }
-    lim_min = (int)__reduce_min_sync(0xffffffffu, (unsigned)lim_min);
-    st.vref = 7.8886091e-31f;  // 2^-100
-    st.vinv = 1024.0f / st.vref;
-    st.first = true;
-    st.neg_hi = SPLIT && t >= 2 ? 0xbc00bc00u : 0u;
-
-    // --- tiles [ta, tb) of the item, every kKvWarps-th from this warp's
-    const long long n_tiles = (lim_max + kKvTile - 1) / kKvTile;
-    long long ta = x0 > kKvItem ? (x0 - kKvItem + kKvTile - 1) / kKvTile : 0;
-    long long tb = x1 == w ? n_tiles : x1 > kKvItem ? (x1 - kKvItem + kKvTile - 1) / kKvTile : 0;
-    ta = ta < n_tiles ? ta : n_tiles;
-    tb = tb < n_tiles ? tb : n_tiles;
-    const int my = tb > ta + warp ? (int)((tb - ta - warp + kKvWarps - 1) / kKvWarps) : 0;
-    const size_t row0 = ((size_t)kvh << p.page_shift) * GM::ROW;
-    const size_t page_bytes = ((size_t)p.nkv << p.page_shift) * GM::ROW;
-    const int* tab = p.table + (size_t)rq.r * p.table_stride;
-    // page ids of the halves of this warp's next 16 tiles, one per lane; -1
-    // behind the last position
-    auto tile_pos = [&](int i) { return (ta + warp + (long long)i * kKvWarps) * kKvTile; };
-    auto load_ids = [&](int i0) {
-      const int i = i0 + (lane >> 1);
-      const long long pos = tile_pos(i) + 16 * (lane & 1);
-      int id = -1;
-      if (i < my && pos < lim_max) id = tab[pos >> p.page_shift];
-      return id < p.n_pages ? id : -1;
-    };
-    int ids = load_ids(0), ids_next = load_ids(16);
-    auto issue = [&](int i, int id0, int id1) {  // lane 0
-      const uint32_t sidx = fill % GM::STAGES;
-      const long long pos = tile_pos(i);
-      const size_t in_page = (size_t)(pos & ((1ll << p.page_shift) - 1));
-      uint8_t* dst = ring + sidx * 2 * GM::SIDE;
-      const uint32_t n = (id0 >= 0) + (id1 >= 0);
-      if (n == 0) {
-        mbar_arrive(&bar[sidx]);
-        return;
-      }
-      mbar_arrive_expect_tx(&bar[sidx], n * 2 * GM::HALF);
-      if (n == 2 && p.page_shift > 4) {  // both halves in one page
-        const size_t off = (size_t)id0 * page_bytes + row0 + in_page * GM::ROW;
-        bulk_g2s(dst, p.k_pages + off, GM::SIDE, &bar[sidx]);
-        bulk_g2s(dst + GM::SIDE, p.v_pages + off, GM::SIDE, &bar[sidx]);
-      } else {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int id = x ? id1 : id0;
-          if (id < 0) continue;
-          const size_t off = (size_t)id * page_bytes + row0 +
-                             (p.page_shift > 4 ? in_page + 16 * x : 0) * GM::ROW;
-          bulk_g2s(dst + x * GM::HALF, p.k_pages + off, GM::HALF, &bar[sidx]);
-          bulk_g2s(dst + GM::SIDE + x * GM::HALF, p.v_pages + off, GM::HALF, &bar[sidx]);
-        }
-      }
-    };
-    const int first = min(my, GM::STAGES);
-    for (int i = 0; i < first; ++i) {
-      const int a = __shfl_sync(0xffffffffu, ids, 2 * i);
-      const int b = __shfl_sync(0xffffffffu, ids, 2 * i + 1);
-      if (lane == 0 && alive) issue(i, a, b);
-      ++fill;
-    }
-    for (int i = 0; i < my; ++i) {
-      const uint32_t sidx = used % GM::STAGES;
-      if (alive) alive = mbar_wait_timed(&bar[sidx], (used / GM::STAGES) & 1, &g_kv4_status);
-      alive = __all_sync(0xffffffffu, alive);
-      ++used;
-      const int ok = (int)(__ballot_sync(0xffffffffu, ids >= 0) >> (2 * (i & 15))) & 3;
-      if (alive && ok) {
-        const int pos0 = (int)tile_pos(i);
-        const uint8_t* kt = ring + sidx * 2 * GM::SIDE;
-        if (pos0 + kKvTile > lim_min || ok != 3)
-          kv_tile<HD, NT, SPLIT, true>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
-        else
-          kv_tile<HD, NT, SPLIT, false>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
-      }
-      __syncwarp();
-      if (i + GM::STAGES < my) {
-        const int nx = i + GM::STAGES, src = 2 * (nx & 15);
-        const int from = (nx >> 4) == (i >> 4) ? ids : ids_next;
-        const int a = __shfl_sync(0xffffffffu, from, src);
-        const int b = __shfl_sync(0xffffffffu, from, src + 1);
-        if (lane == 0 && alive) issue(nx, a, b);
-        ++fill;
-      }
-      if ((i & 15) == 15) {
-        ids = ids_next;
-        ids_next = load_ids(i + 17);
-      }
-    }
-
-    // --- join the warps
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int o = 4; o <= 16; o <<= 1)
-          st.l[n][c] += __shfl_xor_sync(0xffffffffu, st.l[n][c], o);
-        if (st.l[n][c] == 0.0f) st.m[n][c] = -3.0e38f;  // saw nothing
-        if (g == 0) s_ml[warp * COLS + n * 8 + 2 * t + c] = make_float2(st.m[n][c], st.l[n][c]);
-      }
-    __syncthreads();
-    float* area = reinterpret_cast<float*>(ring);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float f[2];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float M = -3.0e38f;
-#pragma unroll
-        for (int x = 0; x < kKvWarps; ++x)
-          M = fmaxf(M, s_ml[x * COLS + n * 8 + 2 * t + c].x);
-        f[c] = ex2(st.m[n][c] - M) * (st.vref * 0.0009765625f);
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float* a = area + (n * 8 + 2 * t) * GM::OP + b * 32 + 4 * g + 2 * y;
-          const float* o = st.o[n][b][y];
-          *reinterpret_cast<float2*>(a) = make_float2(o[0] * f[0], o[2] * f[0]);
-          *reinterpret_cast<float2*>(a + GM::OP) = make_float2(o[1] * f[1], o[3] * f[1]);
-        }
-    }
-    __syncthreads();
-    const bool whole = x0 == 0 && x1 == w;
-    const int slot = x0 > 0 ? 0 : 1;
-    for (int i = tid; i < COLS * HD; i += kKvWarps * 32) {
-      const int col = i / HD, d = i - col * HD;
-      const int ct = col / p.gsz, ch = col - ct * p.gsz;
-      if (ct >= ntok || ch >= nhead || (SPLIT && col >= 4)) continue;
-      float M = -3.0e38f, L = 0.0f, sum = 0.0f;
-#pragma unroll
-      for (int x = 0; x < kKvWarps; ++x) M = fmaxf(M, s_ml[x * COLS + col].x);
-#pragma unroll
-      for (int x = 0; x < kKvWarps; ++x) {
-        const float2 ml = s_ml[x * COLS + col];
-        L += ml.y * ex2(ml.x - M);
-        const float* a = reinterpret_cast<const float*>(ring_all + x * GM::PER_WARP);
-        sum += a[col * GM::OP + d];
-        if (SPLIT) sum += a[(col + 4) * GM::OP + d];
-      }
-      if (whole) {
-        p.out[(size_t)(rq.t0 + tok0 + ct) * p.out_stride + (size_t)(h0 + ch) * HD + d] =
-            L != 0.0f ? sum / L : 0.0f;
-      } else {
-        const size_t at = ((size_t)cta * 2 + slot) * COLS + col;
-        p.part_o[at * HD + d] = sum;
-        if (d == 0) {
-          p.part_ml[at * 2] = M;
-          p.part_ml[at * 2 + 1] = L;
-        }
-      }
-    }
-    if (!whole && slot == 1)
-      rec = make_int4(rq.r, h, (int)j, (int)((s0 + w - 1) / per) - cta + 1);
-    // the merge area is the ring of the next item's bulk copies
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-
-    u = s0 += w;
-    if (++j == rq.J) {
-      j = 0;
-      if (++h == H) {
-        h = 0;
-        do {
-          if (rq.r + 1 >= p.n_req) break;
-          rq = kv_req(p, rq.r + 1);
-        } while (rq.J == 0);
-      }
-    }
+    KvItem x = it;
+    __syncwarp();
+    if (x.start + x.w >= end || !kv_item_next(p, x)) break;
+    x.x0 = 0;
+    x.x1 = min(end - x.start, x.w);
+    if (lane == 0) it = x;
+    __syncwarp();
   }
-  if (tid == 0) p.rec[cta] = rec;
 }
 
-// Joins the pieces of the item that starts in CTA blockIdx.x and goes on in
-// the next ones. One block per column; warp w sums the pieces w, w + 4, ..
-// (a long history has a hundred), then the four sums are added in order.
+// Joins the pieces of the items that start in the warps of CTA blockIdx.x and
+// go on behind them, one block per column. An item of few pieces is summed by
+// one warp (four items at once), one of many by the eight warps in turn,
+// always in a fixed order.
+constexpr int kKvJoinWarps = 8;
+constexpr int kKvJoinAlone = 16;  // pieces
 template <int HD>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
+__global__ void __launch_bounds__(kKvJoinWarps * 32)
+    kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
   constexpr int PER = HD / 32;  // values per lane
-  __shared__ float s_o[4][HD];
-  __shared__ float s_l[4];
+  __shared__ float s_o[kKvJoinWarps][HD];
+  __shared__ float s_l[kKvJoinWarps];
+  __shared__ KvRec s_rec[kKvWarps];
   pdl_wait();
   pdl_launch_dependents();
-  const int c = blockIdx.x, col = blockIdx.y, cols = gridDim.y;
+  const int col = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int4 rec = p.rec[c];
-  const int parts = min(rec.w, p.n_cta - c);
-  if (parts < 2) return;
-  const KvReq q = kv_req(p, rec.x);
-  const int kvh = rec.y / p.hgroups, hg = rec.y % p.hgroups;
-  const int ct = col / p.gsz, ch = col - ct * p.gsz;
-  const int tok = rec.z * p.tpt + ct, head = hg * p.gsz + ch;
-  if (tok >= q.n || ct >= p.tpt || head >= p.nh / p.nkv) return;
-  auto at = [&](int i) { return ((size_t)(c + i) * 2 + (i == 0 ? 1 : 0)) * cols + col; };
-  float M = -3.0e38f;
-  for (int i = lane; i < parts; i += 32) M = fmaxf(M, p.part_ml[at(i) * 2]);
-  M = warp_max(M);
-  float L = 0.0f, sum[PER] = {};
-#pragma unroll 4
-  for (int i = warp; i < parts; i += 4) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(i) * 2);
-    const float f = ex2(ml.x - M);
-    L += ml.y * f;
-    const float* o = p.part_o + at(i) * HD + PER * lane;
-#pragma unroll
-    for (int d = 0; d < PER; ++d) sum[d] += o[d] * f;
-  }
-#pragma unroll
-  for (int d = 0; d < PER; ++d) s_o[warp][PER * lane + d] = sum[d];
-  if (lane == 0) s_l[warp] = L;
+  if (threadIdx.x < kKvWarps) s_rec[threadIdx.x] = p.rec[blockIdx.x * kKvWarps + threadIdx.x];
   __syncthreads();
-  L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-  for (int d = threadIdx.x; d < HD; d += 128) {
-    const float o = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]);
-    p.out[(size_t)(q.t0 + tok) * p.out_stride + (size_t)(kvh * (p.nh / p.nkv) + head) * HD + d] =
-        L != 0.0f ? o / L : 0.0f;
+  const int ct = col / p.gsz, ch = col - ct * p.gsz;
+  // the item's row of `out` for this column, or null
+  auto row = [&](const KvRec& rec) -> float* {
+    const int a = p.q_start[rec.r], n = p.q_start[rec.r + 1] - a;
+    const int kvh = rec.h / p.hgroups, head = (rec.h - kvh * p.hgroups) * p.gsz + ch;
+    const int tok = rec.j * p.tpt + ct;
+    if (tok >= n || ct >= p.tpt || ch >= p.gsz || head >= p.nh / p.nkv) return nullptr;
+    return p.out + (size_t)(a + tok) * p.out_stride + (size_t)(kvh * (p.nh / p.nkv) + head) * HD;
+  };
+  // pieces w, w + step, .. of an item: their sum relative to the maximum M of all
+  auto sum = [&](const KvRec& rec, int w, int step, float& L, float* acc) {
+    auto at = [&](int i) {
+      const int piece = i < rec.n_first             ? rec.a + i
+                        : i < rec.n_first + rec.n_mid ? (rec.a / kKvWarps + 1 + i - rec.n_first) * kKvWarps
+                                                      : rec.z0 + (i - rec.n_first - rec.n_mid);
+      return ((size_t)piece * 2 + (i == 0 ? 1 : 0)) * p.cols + col;
+    };
+    float M = -3.0e38f;
+    for (int i = lane; i < rec.parts; i += 32) M = fmaxf(M, p.part_ml[at(i) * 2]);
+    M = warp_max(M);
+    L = 0.0f;
+#pragma unroll
+    for (int d = 0; d < PER; ++d) acc[d] = 0.0f;
+#pragma unroll 4
+    for (int i = w; i < rec.parts; i += step) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(i) * 2);
+      const float f = ex2(ml.x - M);
+      L += ml.y * f;
+      const float* o = p.part_o + at(i) * HD + PER * lane;
+#pragma unroll
+      for (int d = 0; d < PER; ++d) acc[d] += o[d] * f;
+    }
+  };
+  float L, acc[PER];
+  if (warp < kKvWarps) {
+    const KvRec rec = s_rec[warp];
+    if (rec.parts && rec.parts <= kKvJoinAlone) {
+      float* out = row(rec);
+      if (out) {
+        sum(rec, 0, 1, L, acc);
+#pragma unroll
+        for (int d = 0; d < PER; ++d) out[PER * lane + d] = L != 0.0f ? acc[d] / L : 0.0f;
+      }
+    }
+  }
+  for (int k = 0; k < kKvWarps; ++k) {
+    const KvRec rec = s_rec[k];
+    if (rec.parts <= kKvJoinAlone) continue;
+    float* out = row(rec);
+    if (!out) continue;
+    sum(rec, warp, kKvJoinWarps, L, acc);
+    __syncthreads();  // the sums of the item before have been read
+#pragma unroll
+    for (int d = 0; d < PER; ++d) s_o[warp][PER * lane + d] = acc[d];
+    if (lane == 0) s_l[warp] = L;
+    __syncthreads();
+    for (int d = threadIdx.x; d < HD; d += kKvJoinWarps * 32) {
+      float o = 0.0f, l = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kKvJoinWarps; ++x) {
+        o += s_o[x][d];
+        l += s_l[x];
+      }
+      out[d] = l != 0.0f ? o / l : 0.0f;
+    }
   }
 }
 
@@ -937,7 +1116,7 @@ KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_
   k.nt = G > 8 || n_tokens > n_req ? 2 : 1;
   k.split = k.nt == 1 && G <= 4;
   k.n_cta = sm_count() * (k.nt == 1 ? 4 : 2);
-  k.ws = (size_t)k.n_cta * (2 * 8 * k.nt * (hd + 2) * 4 + sizeof(int4));
+  k.ws = (size_t)k.n_cta * kKvWarps * (2 * 8 * k.nt * (hd + 2) * 4 + sizeof(KvRec));
   return k;
 }
 
@@ -947,7 +1126,8 @@ minq_status launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
   MINQ_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kv4_attend_kernel<HD, NT, SPLIT>), GM::SMEM));
   MINQ_CUDA_TRY(launch_k(kv4_attend_kernel<HD, NT, SPLIT>, dim3(p.n_cta), dim3(kKvWarps * 32), GM::SMEM, s,
                          p));
-  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3(p.n_cta, GM::COLS), dim3(128), 0, s, p));
+  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3(p.n_cta, SPLIT ? 4 : GM::COLS),
+                         dim3(kKvJoinWarps * 32), 0, s, p));
   return MINQ_OK;
 }
 
@@ -1026,13 +1206,15 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
   p.out_stride = out_stride;
   if (plan.ws) {
     const int G = (int)(n_heads / n_kv), cols = 8 * plan.nt, most = plan.split ? 4 : cols;
+    p.cols = cols;
     p.gsz = G < most ? G : most;
     p.hgroups = (G + p.gsz - 1) / p.gsz;
     p.tpt = most / p.gsz;
     p.n_cta = plan.n_cta;
-    p.rec = static_cast<int4*>(workspace);
-    p.part_o = reinterpret_cast<float*>(p.rec + plan.n_cta);
-    p.part_ml = p.part_o + (size_t)plan.n_cta * 2 * cols * head_dim;
+    const size_t pieces = (size_t)plan.n_cta * kKvWarps;
+    p.rec = static_cast<KvRec*>(workspace);
+    p.part_o = reinterpret_cast<float*>(p.rec + pieces);
+    p.part_ml = p.part_o + pieces * 2 * cols * head_dim;
     cudaStream_t s = (cudaStream_t)stream;
     if (head_dim == 64)
       return plan.split     ? launch_kv4_attend<64, 1, true>(p, s)
