@@ -266,6 +266,23 @@ __device__ __forceinline__ void add2(float* o, const float* c) {
       : "f"(c[0]), "f"(c[1]));
 }
 
+// Four 8x8 matrices of half words, transposed: lane i gives row i's address
+// (16-byte aligned) and gets rows 2t, 2t + 1 of column g of each.
+__device__ __forceinline__ void load_trans(uint32_t* d, const uint8_t* row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(smem_u32(row))
+               : "memory");
+}
+
+// First of the 4 dimensions of block b that lane group g holds of V. With
+// head_dim 128 a row is five 16-byte chunks, which the transposing load reads
+// whole: block b's half word h lies in column (2 b + 2 + h) mod 8 of its chunk.
+template <int HD>
+__device__ __forceinline__ int kv_dim(int b, int g) {
+  return b * 32 + 4 * (HD == 128 ? (g - 2 * b - 2) & 7 : g);
+}
+
 // The line of items. Request r: n tokens in J column tiles per head tile.
 struct KvReq {
   int r, t0, n, len;  // request, first token, tokens, positions
@@ -315,9 +332,10 @@ struct KvState {
   uint32_t q[NT][NB][2][SPLIT ? 2 : 4];
   float cn[NT][2];           // scores to log2 units
   int lim[NT][2];            // positions the column sees
+  // running maximum less vlog, and sum: weights are 2^(z - m) = p 2^10 / vref
   float m[NT][2], l[NT][2];
   float o[NT][NB][2][4];
-  float vref, vinv;          // 2^floor(log2 max value scale), 2^10 / vref
+  float vref, vlog;          // 2^floor(log2 max value scale), log2(2^10 / vref)
   uint32_t neg_hi;           // SPLIT: f16 -1 where the lane's columns are low parts, else 0
   bool first;                // no tile seen yet (uniform over the warp)
 };
@@ -403,16 +421,24 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT, SPLIT>& st, const uint8_
     for (int o = 4; o <= 16; o <<= 1) emax = fmaxf(emax, __shfl_xor_sync(0xffffffffu, emax, o));
     const float ref = fmaxf(__uint_as_float(__float_as_uint(emax) & 0x7f800000u), st.vref);
     const float f = st.vref / ref;  // powers of two
+    const float up = (float)((int)(__float_as_uint(ref) >> 23) -
+                             (int)(__float_as_uint(st.vref) >> 23));
     st.vref = ref;
-    st.vinv = 1024.0f / ref;
+    st.vlog -= up;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        st.m[n][c] += up;
+        st.l[n][c] *= f;
+      }
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) st.o[n][b][j][i] *= f;
+    }
   }
   // softmax: x = z - m in log2 units
   float most = -INFINITY;
@@ -430,7 +456,7 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT, SPLIT>& st, const uint8_
         most = fmaxf(most, x);
       }
   }
-  if (st.first || __any_sync(0xffffffffu, most > 4.0f)) {
+  if (st.first || __any_sync(0xffffffffu, most > 4.0f + st.vlog)) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (NT > 1 && n >= n_nt) break;
@@ -441,6 +467,7 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT, SPLIT>& st, const uint8_
         for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
         // the first tile sets the maximum (a column that sees none of it sees
         // none of the later ones), then it only grows
+        x -= st.vlog;
         if (st.first)
           x = x == -INFINITY ? 0.0f : x;
         else
@@ -474,25 +501,41 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT, SPLIT>& st, const uint8_
 #pragma unroll
     for (int c = 0; c < 2; ++c)
       st.l[n][c] += (s[0][n][c] + s[0][n][c + 2]) + (s[1][n][c] + s[1][n][c + 2]);
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[u][n][i] *= st.vinv;
   }
-  // o^T += V^T p^T: lane g holds 4 dimensions of a block (its half word),
-  // positions 2t, 2t + 1, 2t + 8, 2t + 9 of each half
+  // o^T += V^T p^T: lane g holds 4 dimensions of a block (a half word, see
+  // kv_dim), positions 2t, 2t + 1, 2t + 8, 2t + 9 of each half
+  uint32_t chunk[4], next_chunk[4];
+  if constexpr (HD == 128) load_trans(chunk, v + lane * ROW);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     uint32_t y[2][2][4];  // [half][pair of positions][dimension]
+    if constexpr (HD == 128) {
+      // half words 10 b + 2 .. 10 b + 9 of the row: lane g takes the one in its
+      // column of 16-byte chunk b, lanes below 2 b + 2 that of chunk b + 1
+      uint32_t x[4];
+      if (b < 3) {
+        load_trans(next_chunk, v + lane * ROW + 16 * (b + 1));
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* w = v + (16 * u + 8 * h + 2 * t) * ROW + b * kQ4Bytes + 4 + 2 * g;
-        const uint32_t x0 = *reinterpret_cast<const uint16_t*>(w);
-        const uint32_t x1 = *reinterpret_cast<const uint16_t*>(w + ROW);
-        codes4(__byte_perm(x0, x1, 0x5410), y[u][h]);
+        for (int i = 0; i < 4; ++i) {
+          x[i] = g < 2 * b + 2 ? next_chunk[i] : chunk[i];
+          chunk[i] = next_chunk[i];
+        }
+      } else {
+        load_trans(x, v + lane * ROW + 64);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) codes4(x[i], y[i >> 1][i & 1]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* w = v + (16 * u + 8 * h + 2 * t) * ROW + b * kQ4Bytes + 4 + 2 * g;
+          const uint32_t x0 = *reinterpret_cast<const uint16_t*>(w);
+          const uint32_t x1 = *reinterpret_cast<const uint16_t*>(w + ROW);
+          codes4(__byte_perm(x0, x1, 0x5410), y[u][h]);
+        }
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (NT > 1 && n >= n_nt) break;
@@ -670,40 +713,33 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[n][b][e] = on ? qp[b * 32 + e] : 0.0f;
   }
-  auto issue = [&](int i, int id0, int id1) {  // lane 0
+  // tile i into the ring: lanes 0..3 copy a half of K or V each (16 rows of
+  // one page); `from` holds the ids of its group of 16 tiles
+  const int half = lane & 1;
+  const uint8_t* side = (lane & 2 ? p.v_pages : p.k_pages) + row0;
+  const int page_mask = (1 << p.page_shift) - 1;
+  auto issue = [&](int i, int from) {
     const uint32_t sidx = ring.fill % GM::STAGES;
     uint64_t* bar = &ring.bar[sidx];
-    const int in_page = tile_pos(i) & ((1 << p.page_shift) - 1);
-    uint8_t* dst = ring.buf + sidx * 2 * GM::SIDE;
-    const uint32_t n = (id0 >= 0) + (id1 >= 0);
-    if (n == 0) {
-      mbar_arrive(bar);
-      return;
+    const int id = __shfl_sync(0xffffffffu, from, 2 * (i & 15) + half);
+    const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
+    if (lane == 0 && ring.alive) {
+      const uint32_t n = (have & 1) + ((have >> 1) & 1);
+      if (n)
+        mbar_arrive_expect_tx(bar, n * 2 * GM::HALF);
+      else
+        mbar_arrive(bar);
     }
-    mbar_arrive_expect_tx(bar, n * 2 * GM::HALF);
-    if (n == 2 && p.page_shift > 4) {  // both halves in one page
-      const size_t off = (size_t)id0 * page_bytes + row0 + in_page * GM::ROW;
-      bulk_g2s(dst, p.k_pages + off, GM::SIDE, bar);
-      bulk_g2s(dst + GM::SIDE, p.v_pages + off, GM::SIDE, bar);
-    } else {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int id = x ? id1 : id0;
-        if (id < 0) continue;
-        const size_t off = (size_t)id * page_bytes + row0 +
-                           (p.page_shift > 4 ? in_page + 16 * x : 0) * GM::ROW;
-        bulk_g2s(dst + x * GM::HALF, p.k_pages + off, GM::HALF, bar);
-        bulk_g2s(dst + GM::SIDE + x * GM::HALF, p.v_pages + off, GM::HALF, bar);
-      }
+    __syncwarp();  // the bytes are expected before they can come
+    if (lane < 4 && id >= 0 && ring.alive) {
+      const int row = (tile_pos(i) + 16 * half) & page_mask;
+      bulk_g2s(ring.buf + sidx * 2 * GM::SIDE + (lane >> 1) * GM::SIDE + half * GM::HALF,
+               side + (size_t)id * page_bytes + row * GM::ROW, GM::HALF, bar);
     }
+    ++ring.fill;
   };
   const int first = min(my, GM::STAGES);
-  for (int i = 0; i < first; ++i) {
-    const int a = __shfl_sync(0xffffffffu, ids, 2 * i);
-    const int b = __shfl_sync(0xffffffffu, ids, 2 * i + 1);
-    if (lane == 0 && ring.alive) issue(i, a, b);
-    ++ring.fill;
-  }
+  for (int i = 0; i < first; ++i) issue(i, ids);
   int ids_next = my > 16 ? load_ids(16) : -1;
 
   // q as f16 parts, limits
@@ -749,7 +785,7 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
     if (on) lim_min = min(lim_min, (int)lim);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      st.m[n][c] = 0.0f;
+      st.m[n][c] = -74.0f;
       st.l[n][c] = 0.0f;
     }
 #pragma unroll
@@ -760,8 +796,8 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
         for (int i = 0; i < 4; ++i) st.o[n][b][y][i] = 0.0f;
   }
   lim_min = (int)__reduce_min_sync(0xffffffffu, (unsigned)lim_min);
-  st.vref = 7.8886091e-31f;  // 2^-100
-  st.vinv = 1024.0f / st.vref;
+  st.vref = 5.4210109e-20f;  // 2^-64: the weights' sums stay finite
+  st.vlog = 74.0f;
   st.first = true;
   st.neg_hi = SPLIT && t >= 2 ? 0xbc00bc00u : 0u;
 
@@ -781,14 +817,8 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
         kv_tile<HD, NT, SPLIT, false>(st, kt, kt + GM::SIDE, pos0, lim_max, n_nt, ok);
     }
     __syncwarp();
-    if (i + GM::STAGES < my) {
-      const int nx = i + GM::STAGES, src = 2 * (nx & 15);
-      const int from = (nx >> 4) == (i >> 4) ? ids : ids_next;
-      const int a = __shfl_sync(0xffffffffu, from, src);
-      const int b = __shfl_sync(0xffffffffu, from, src + 1);
-      if (lane == 0 && ring.alive) issue(nx, a, b);
-      ++ring.fill;
-    }
+    const int nx = i + GM::STAGES;
+    if (nx < my) issue(nx, (nx >> 4) == (i >> 4) ? ids : ids_next);
     if ((i & 15) == 15) {
       ids = ids_next;
       ids_next = load_ids(i + 17);
@@ -802,7 +832,9 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1)
         st.l[n][c] += __shfl_xor_sync(0xffffffffu, st.l[n][c], o);
-      if (st.l[n][c] == 0.0f) st.m[n][c] = -3.0e38f;  // saw nothing
+      // the plain maximum and sum; o keeps the factor 2^10 / vref
+      st.m[n][c] = st.l[n][c] == 0.0f ? -3.0e38f : st.m[n][c] + st.vlog;  // saw nothing
+      st.l[n][c] *= st.vref * 0.0009765625f;
     }
 }
 
@@ -941,7 +973,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
         for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            float* a = area + (n * 8 + 2 * t) * GM::OP + b * 32 + 4 * g + 2 * y;
+            float* a = area + (n * 8 + 2 * t) * GM::OP + kv_dim<HD>(b, g) + 2 * y;
             const float* o = st.o[n][b][y];
             *reinterpret_cast<float2*>(a) = make_float2(o[0] * f[0], o[2] * f[0]);
             *reinterpret_cast<float2*>(a + GM::OP) = make_float2(o[1] * f[1], o[3] * f[1]);
@@ -1002,7 +1034,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
           for (int i = 0; i < 4; ++i) {
             float o = st.o[n][b][y][i];
             if (SPLIT) o += __shfl_xor_sync(0xffffffffu, o, 2);
-            if (dst[i & 1]) dst[i & 1][b * 32 + 4 * g + 2 * y + (i >> 1)] = o * r[i & 1];
+            if (dst[i & 1]) dst[i & 1][kv_dim<HD>(b, g) + 2 * y + (i >> 1)] = o * r[i & 1];
           }
     }
     KvItem x = it;
