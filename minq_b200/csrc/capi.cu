@@ -179,7 +179,8 @@ minq_status minq_device_status(void) {
   const minq_status a = take_device_status();
   const minq_status b = take_static_attn_status();
   const minq_status c = take_kv4_status();
-  return a != MINQ_OK ? a : b != MINQ_OK ? b : c;
+  const minq_status d = take_sample_rows_status();
+  return a != MINQ_OK ? a : b != MINQ_OK ? b : c != MINQ_OK ? c : d;
 }
 
 minq_status minq_kernel_timer_start(const char* family) {

@@ -40,8 +40,9 @@ minq_status take_device_status();
 // Read-and-clear of minq_attend_static's file-scope status word on the
 // current device (no allocation; the caller has synchronised).
 minq_status take_static_attn_status();
-// The same of minq_kv4_attend's.
+// The same of minq_kv4_attend's and minq_sample_rows's.
 minq_status take_kv4_status();
+minq_status take_sample_rows_status();
 
 #define MINQ_CUDA_TRY(expr)                                    \
   do {                                                         \
