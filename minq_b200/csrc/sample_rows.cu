@@ -13,19 +13,22 @@
 // on, in index order otherwise. Tokens at -infinity (or NaN) have w = 0 and
 // are never drawn; a row without any other token gives token 0.
 //
-// Weights and sums carry about f64: next to a border a draw is decided by
-// digits that an f32 sum over a vocabulary does not hold (with 100,000 even
-// tokens, borders moved by 1e-7 of the mass would change one draw in a
-// hundred). The exponential is the table-driven one (Tang 1989): 2^(m/256) from
-// a table times a polynomial of degree 3 on half a step, to 1e-13.
+// Next to a border a draw is decided by digits that an f32 sum over a
+// vocabulary does not hold (with 100,000 even tokens, borders moved by 1e-7 of
+// the mass would change one draw in a hundred). So a weight is a fixed-point
+// integer, to 2^-28 of itself, and all sums are exact integers: the roundings
+// of 100,000 even tokens move a border by about 1e-6 of one token, and no
+// result depends on an order of summation. The exponent 256 log2 w comes from
+// one f64 FMA whose addend leaves 24 fractional bits; 2^(a/256) is the
+// table-driven exponential (Tang 1989), a table of 256 steps and a polynomial
+// of degree 3 for the rest, in f32 and integers.
 //
 // A cluster of up to 8 CTAs holds a row in shared memory (one pass over HBM,
 // bulk copies), so every further pass runs at shared-memory speed:
 //   1. the maximum;
 //   2. a histogram over 512 buckets of (max - x) / T, 1/32 wide: counts, and
-//      the mass as fixed-point integers in three 32-bit parts (shared-memory
-//      atomics are fast in 32 bits only; integer sums do not depend on their
-//      order). Each CTA adds up a slice of the buckets over the cluster; the
+//      the mass in two 32-bit parts, in units of the bucket (shared-memory
+//      atomics are fast in 32 bits only). Each CTA adds up a slice of the buckets over the cluster; the
 //      running sums give the bucket of the last kept token (by count and by
 //      mass alike) and, for a given mass, that of the draw;
 //   3. the tokens of that bucket are listed, sorted and summed in f64, which
@@ -50,11 +53,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kRowsThreads = 512;
+constexpr int kRowsThreads = 256;
 constexpr int kRowsWarps = kRowsThreads / 32;
-constexpr int kRowsBuckets = 512;           // one per thread
+constexpr int kRowsBuckets = 512;           // two per thread
 constexpr float kRowsPerNat = 32.0f;        // buckets per unit of (max - x) / T
-constexpr int kRowsList = 1024;             // tokens a list holds
+constexpr int kRowsList = 1024;             // tokens a list holds: four per thread
 constexpr int kRowsMaxCtas = 8;             // the portable cluster size
 constexpr uint32_t kRowsCached = 48 * 1024; // floats of a row that a CTA can hold
 constexpr int kRowsTable = 256;
@@ -64,7 +67,8 @@ struct RowsParams {
   size_t stride;
   uint32_t n, chunk;         // chunk: elements per CTA
   bool cached;
-  int part_bits, mass_bits;  // the fixed-point mass: bits per part, of w = 1
+  int part_bits, drop;       // a weight's 30 bits less `drop`, in two parts of part_bits
+  int mass_bits;             // of w = 1 in 64-bit sums
   const float* temperature;  // null: 1
   const int* top_k;          // null or <= 0: off
   const float* top_p;        // null or >= 1: off
@@ -72,6 +76,9 @@ struct RowsParams {
   const float* u;
   uint32_t* out;
 };
+
+// Whether a token can be drawn (a number above -infinity).
+__device__ __forceinline__ bool rows_real(float v) { return v > -INFINITY; }
 
 // Set when a bounded wait gave up (read and cleared by take_sample_rows_status).
 __device__ int g_rows_status;
@@ -94,26 +101,29 @@ struct RowsShared {
   // a list is only sorted after a cluster barrier that follows the last read
   // of the histogram
   union {
-    uint32_t hist[4][kRowsBuckets];
+    uint32_t hist[3][kRowsBuckets];
     unsigned long long sort[kRowsList];
   };
   unsigned long long list[2][kRowsList];
   // this CTA's slice of the cluster's buckets: running sums before each
   unsigned long long slice_m[kRowsBuckets + 1];
   uint32_t slice_c[kRowsBuckets + 2];
-  double table[kRowsTable];  // 2^(j/256)
-  double red[kRowsWarps];
+  uint2 table[kRowsTable];  // 2^(29 + j/256), and it as a float
   unsigned long long redu[kRowsWarps];
-  unsigned long long best;  // this CTA's maximum
-  double total;             // this CTA's mass (unfiltered and small top-k rows)
+  unsigned long long best;   // this CTA's maximum
+  unsigned long long total;  // this CTA's mass (unfiltered and small top-k rows)
   unsigned long long ties;  // this CTA's count of one key
   uint32_t count[2];        // entries of the lists
   uint32_t result, last;
   int pick[4];
   unsigned long long pickm;
-  double pickd;
   uint64_t bar;
 };
+
+__device__ __forceinline__ RowsShared& rows_shared() {
+  __shared__ RowsShared s;
+  return s;
+}
 
 __device__ __forceinline__ unsigned long long rows_warp_scan(unsigned long long v) {
   const int lane = threadIdx.x & 31;
@@ -124,28 +134,20 @@ __device__ __forceinline__ unsigned long long rows_warp_scan(unsigned long long 
   }
   return v;
 }
-__device__ __forceinline__ double rows_warp_scan(double v) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double x = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
-}
 // Exclusive prefix over the block; the total in every thread.
-template <class T>
-__device__ __forceinline__ T rows_scan(T v, T* red, T& total) {
+__device__ __forceinline__ unsigned long long rows_scan(unsigned long long v,
+                                                        unsigned long long* red,
+                                                        unsigned long long& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T incl = rows_warp_scan(v);
+  const unsigned long long incl = rows_warp_scan(v);
   __syncthreads();
   if (lane == 31) red[warp] = incl;
   __syncthreads();
-  T base = 0;
+  unsigned long long base = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kRowsThreads / 32; ++w) {
-    const T x = red[w];
+    const unsigned long long x = red[w];
     if (w < warp) base += x;
     total += x;
   }
@@ -154,26 +156,37 @@ __device__ __forceinline__ T rows_scan(T v, T* red, T& total) {
 
 constexpr uint32_t kRowsPad = 0xffffffffu;  // a NaN below every number: no token
 
+template <bool CACHED>
 struct Row {
   // this CTA's part of the row, four at a time: element i is token first + i,
   // ends padded with kRowsPad (cached: 16-byte aligned shared memory; else
   // `count` floats in global memory, first == base)
   const float* x;
-  bool cached;
   uint32_t first, n4;
   uint32_t base, count;  // its tokens
   uint32_t top;          // key of the maximum
-  float fmax, per;       // buckets: (fmax - x) * per
-  double dmax, scale;    // 256 log2(w) = (x - dmax) * scale
-  const double* table;
+  float fmax, per, low;  // buckets: (fmax - x) * per; what is below low weighs nothing
+  double scale, shift;   // 256 log2(w) = x * scale + shift, plus kMagic
+  int bits, drop;        // see RowsParams
+  static constexpr double kMagic = 402653184.0;  // 1.5 * 2^28: 24 fractional bits
+  bool inf;              // the maximum is infinite: it counts as 0, all else as -infinity
 
   __device__ __forceinline__ float4 load(uint32_t j) const {
-    if (cached) return reinterpret_cast<const float4*>(x)[j];
-    float v[4];
+    if constexpr (CACHED) {
+      extern __shared__ __align__(16) float s_row[];
+      return reinterpret_cast<const float4*>(s_row)[j];
+    } else {
+      float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = 4 * j + i < count ? x[4 * j + i] : __uint_as_float(kRowsPad);
-    return make_float4(v[0], v[1], v[2], v[3]);
+      for (int i = 0; i < 4; ++i)
+        v[i] = 4 * j + i < count ? at(4 * j + i) : __uint_as_float(kRowsPad);
+      return make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+  // Token base + i.
+  __device__ __forceinline__ float at(uint32_t i) const {
+    const float v = x[base - first + i];
+    return CACHED || !inf ? v : v == INFINITY ? 0.0f : -INFINITY;
   }
   // Every element of this CTA: f(value, token).
   template <class F>
@@ -187,32 +200,43 @@ struct Row {
       f(v.w, first + 4 * j + 3);
     }
   }
-  // Whether a weight can be drawn (a number above -infinity).
-  __device__ static __forceinline__ bool real(float v) { return v > -INFINITY; }
-  // 2^bits exp((v - max) / T); 0 where it is below 2^(bits - 860), or the
-  // maximum is infinite and v is not.
-  __device__ __forceinline__ double weight(float v, int bits = 0) const {
-    const double kMagic = 6755399441055744.0;  // 1.5 * 2^52: rounds to an integer
-    if (fmax == INFINITY) return v == INFINITY ? ldexp(1.0, bits) : 0.0;
-    if (!((fmax - v) * per < kRowsPerNat * 600.0f)) return 0.0;
-    const double a = ((double)v - dmax) * scale;
-    const double m = a + kMagic;
-    const int k = __double2loint(m);
-    const double f = a - (m - kMagic);         // [-1/2, 1/2] of 1/256 octave
-    // 2^(f/256) = sum (f ln2/256)^i / i!
-    double y = 3.308302680541371e-09;          // (ln2/256)^3 / 6
-    y = fma(y, f, 3.665565596910106e-06);      // (ln2/256)^2 / 2
-    y = fma(y, f, 0.0027076061740622863);      // ln2/256
-    y = fma(y, f, 1.0);
-    y *= table[k & (kRowsTable - 1)];
-    return __hiloint2double(__double2hiint(y) + (((k >> 8) + bits) << 20), __double2loint(y));
-  }
-  __device__ __forceinline__ double key_weight(uint32_t key) const {
-    return key > kKeyNone ? weight(rows_value(key)) : 0.0;
-  }
+  // Bucket of a value, in order (the nearest of (fmax - v) * per).
   __device__ __forceinline__ int bucket(float v) const {
-    const float b = (fmax - v) * per;  // NaN (both infinite): 0
-    return b >= (float)(kRowsBuckets - 1) ? kRowsBuckets - 1 : (int)b;
+    const float b = fminf((fmax - v) * per, (float)(kRowsBuckets - 1));
+    return __float_as_int(b + 12582912.0f) - 0x4b400000;  // 1.5 * 2^23: rounds to an integer
+  }
+  // Exponent of the bucket's unit: at least that of any weight in it
+  // (1/32 nat = 0.04508 octaves > 46 / 1024).
+  __device__ static __forceinline__ int unit(int bucket) { return -((bucket * 46) >> 10); }
+  // exp((v - max) / T) in units of 2^(unit(b) - 29 + drop), b = bucket(v).
+  __device__ __forceinline__ uint32_t weight(float v, int b) const {
+    const double m = fma((double)fmaxf(v, low), scale, shift);
+    // a = 256 log2 w, times 2^24, below kMagic's bits
+    const uint32_t lo = (uint32_t)__double2loint(m), hi = (uint32_t)__double2hiint(m);
+    const int k = (int)__funnelshift_r(lo, hi, 24) - kMagicK;
+    const float f = __uint_as_float(0x3f800000u | ((lo & 0xffffffu) >> 1)) - 1.0f;  // [0, 1)
+    // 2^(f/256) - 1 = sum (f ln2/256)^i / i!
+    float y = 3.3083026e-09f;        // (ln2/256)^3 / 6
+    y = fmaf(y, f, 3.6655656e-06f);  // (ln2/256)^2 / 2
+    y = fmaf(y, f, 2.7076062e-03f);  // ln2/256
+    const uint2 t = rows_shared().table[k & (kRowsTable - 1)];
+    const float up = fmaf(y * f, __uint_as_float(t.y), 12582912.0f);  // rounded to an integer
+    const uint32_t w = t.x + (uint32_t)(__float_as_int(up) - 0x4b400000);  // [2^29, 2^30]
+    return w >> min(unit(b) - (k >> 8) + drop, 31);
+  }
+  // kMagic's bits, shifted like those of m.
+  static constexpr int kMagicK = (int)((0x41b8000000000000ull >> 24) & 0xffffffffull);
+  // A sum of weights of bucket b in 64-bit units (2^-bits).
+  __device__ __forceinline__ unsigned long long wide(unsigned long long w, int b) const {
+    const int up = bits - 29 + drop + unit(b);
+    return up >= 0 ? w << up : up > -64 ? w >> -up : 0ull;
+  }
+  __device__ __forceinline__ unsigned long long value_weight(float v) const {
+    const int b = bucket(v);
+    return wide(weight(v, b), b);
+  }
+  __device__ __forceinline__ unsigned long long key_weight(uint32_t key) const {
+    return key > kKeyNone ? value_weight(rows_value(key)) : 0ull;
   }
 };
 
@@ -227,7 +251,7 @@ __device__ __forceinline__ T rows_lane(int n, F get) {
 // Where the kept prefix ends, or the draw falls.
 struct Targets {
   double k;        // tokens (infinity: none)
-  double mass;     // running sum to reach (infinity: none)
+  double mass;     // running sum to reach, in fixed-point units (infinity: none)
   uint32_t least;  // smallest key kept (0: any)
 };
 
@@ -238,7 +262,7 @@ struct Range {
   int b0, b1;
   uint32_t lo, hi;
   uint32_t count;
-  double mass;
+  unsigned long long mass;
 };
 
 struct Found {
@@ -248,62 +272,67 @@ struct Found {
   unsigned long long above_m;
 };
 
+template <bool CACHED>
 struct Search {
-  const RowsParams& p;
-  RowsShared& sh;
-  const Row& row;
+  const Row<CACHED> row;
   cg::cluster_group cl;
-  int ctas;
-  double unit;  // mass of one fixed-point step
+  const int ctas, part_bits;
 
-  // Adds up the cluster's histogram: f(value, add) calls add(bucket) for a
-  // token that counts. Afterwards every CTA's slice holds running sums.
-  template <class F>
-  __device__ void histogram(bool mass, F f) {
+  // Adds up the cluster's histogram: f(value, bucket, add) calls add(i) for a
+  // token that counts in entry i; unit(i): the bucket of entry i's units.
+  // Afterwards every CTA's slice holds running sums.
+  template <class F, class U>
+  __device__ __forceinline__ void histogram(bool mass, F f, U unit) {
+    RowsShared& sh = rows_shared();
     const int tid = threadIdx.x;
-    const int arrays = mass ? 4 : 1;
-    for (int i = tid; i < arrays * kRowsBuckets; i += kRowsThreads) (&sh.hist[0][0])[i] = 0;
+    for (int i = tid; i < (mass ? 3 : 1) * kRowsBuckets; i += kRowsThreads) (&sh.hist[0][0])[i] = 0;
     __syncthreads();
-    const uint32_t mask = (1u << p.part_bits) - 1;
+    const uint32_t mask = (1u << part_bits) - 1;
     row.each([&](float v, uint32_t) {
-      f(v, [&](int b) {
-        atomicAdd(&sh.hist[0][b], 1u);
+      if (!rows_real(v)) return;
+      const int b = row.bucket(v);
+      f(v, b, [&](int i) {
+        atomicAdd(&sh.hist[0][i], 1u);
         if (mass) {
-          // 2^52 + w rounds w to an integer in the low mantissa bits
-          const unsigned long long w =
-              (unsigned long long)__double_as_longlong(row.weight(v, p.mass_bits) + 4503599627370496.0) &
-              0xfffffffffffffull;
-          const uint32_t w0 = (uint32_t)w & mask, w1 = (uint32_t)(w >> p.part_bits) & mask,
-                         w2 = (uint32_t)(w >> (2 * p.part_bits));
-          if (w0) atomicAdd(&sh.hist[1][b], w0);
-          if (w1) atomicAdd(&sh.hist[2][b], w1);
-          if (w2) atomicAdd(&sh.hist[3][b], w2);
+          const uint32_t w = row.weight(v, b);
+          atomicAdd(&sh.hist[1][i], w & mask);
+          atomicAdd(&sh.hist[2][i], w >> part_bits);
         }
       });
     });
     cl.sync();
-    // this CTA's slice: thread i sums bucket i of it over the cluster
+    // this CTA's slice: thread i sums entries 2i, 2i + 1 of it over the cluster
     const int per = kRowsBuckets / ctas, rank = (int)cl.block_rank();
-    uint32_t c = 0;
-    unsigned long long m = 0;
-    if (tid < per) {
-      const int b = rank * per + tid;
+    uint32_t c[2] = {0, 0};
+    unsigned long long m[2] = {0, 0};
+    if (2 * tid < per) {
+      const int b = rank * per + 2 * tid;
+      unsigned long long m0 = 0, m1 = 0;
 #pragma unroll
       for (int q = 0; q < kRowsMaxCtas; ++q)
         if (q < ctas) {
           const uint32_t* h = cl.map_shared_rank(&sh.hist[0][0], q) + b;
-          c += h[0];
-          if (mass)
-            m += h[kRowsBuckets] + ((unsigned long long)h[2 * kRowsBuckets] << p.part_bits) +
-                 ((unsigned long long)h[3 * kRowsBuckets] << (2 * p.part_bits));
+          const uint2 n = *reinterpret_cast<const uint2*>(h);
+          c[0] += n.x;
+          c[1] += n.y;
+          if (mass) {
+            const uint2 l = *reinterpret_cast<const uint2*>(h + kRowsBuckets);
+            const uint2 u = *reinterpret_cast<const uint2*>(h + 2 * kRowsBuckets);
+            m0 += l.x + ((unsigned long long)u.x << part_bits);
+            m1 += l.y + ((unsigned long long)u.y << part_bits);
+          }
         }
+      m[0] = row.wide(m0, unit(b));
+      m[1] = row.wide(m1, unit(b + 1));
     }
     unsigned long long tc, tm = 0;
-    const uint32_t ec = (uint32_t)rows_scan((unsigned long long)c, sh.redu, tc);
-    const unsigned long long em = mass ? rows_scan(m, sh.redu, tm) : 0ull;
-    if (tid < per) {
-      sh.slice_c[tid] = ec;
-      sh.slice_m[tid] = em;
+    const uint32_t ec = (uint32_t)rows_scan((unsigned long long)c[0] + c[1], sh.redu, tc);
+    const unsigned long long em = mass ? rows_scan(m[0] + m[1], sh.redu, tm) : 0ull;
+    if (2 * tid < per) {
+      sh.slice_c[2 * tid] = ec;
+      sh.slice_c[2 * tid + 1] = ec + c[0];
+      sh.slice_m[2 * tid] = em;
+      sh.slice_m[2 * tid + 1] = em + m[0];
     }
     if (tid == 0) {
       sh.slice_c[per] = (uint32_t)tc;
@@ -313,7 +342,8 @@ struct Search {
   }
 
   // The row's (or range's) whole mass and count, from the slices.
-  __device__ void totals(unsigned long long& count, unsigned long long& mass) const {
+  __device__ __forceinline__ void totals(unsigned long long& count, unsigned long long& mass) const {
+    RowsShared& sh = rows_shared();
     const int per = kRowsBuckets / ctas;
     unsigned long long c = rows_lane<unsigned long long>(
         ctas, [&](int q) { return (unsigned long long)cl.map_shared_rank(sh.slice_c, q)[per]; });
@@ -332,7 +362,9 @@ struct Search {
   // is not further; `c0`, `m0`: what lies above the histogram's range.
   // meets(bucket): a border by key.
   template <class F>
-  __device__ Found find(const Targets& want, uint32_t c0, double m0, bool mass, int most, F meets) {
+  __device__ __forceinline__ Found find(const Targets& want, uint32_t c0, unsigned long long m0, bool mass, int most,
+                        F meets) {
+    RowsShared& sh = rows_shared();
     const int per = kRowsBuckets / ctas, tid = threadIdx.x, lane = tid & 31;
     // running sums of the slices, one per lane
     uint32_t sc = rows_lane<uint32_t>(ctas, [&](int q) { return cl.map_shared_rank(sh.slice_c, q)[per]; });
@@ -352,8 +384,8 @@ struct Search {
     __syncthreads();
     if (tid == 0) sh.pick[0] = most;
     __syncthreads();
-    // thread b looks at bucket b, in the slice of CTA b / per
-    const int q = tid / per, i = tid - q * per;
+    // thread i looks at buckets 2i and 2i + 1, in one CTA's slice
+    const int q = 2 * tid / per, i = 2 * tid - q * per;
     uint32_t base_c = 0;
     unsigned long long base_m = 0;
 #pragma unroll
@@ -367,23 +399,26 @@ struct Search {
     }
     const uint32_t* pc = cl.map_shared_rank(sh.slice_c, q) + i;
     const unsigned long long* pm = cl.map_shared_rank(sh.slice_m, q) + i;
-    const uint32_t a0 = base_c + pc[0], cnt = base_c + pc[1] - a0;
-    unsigned long long am = 0, mm = 0;
-    if (mass) {
-      am = base_m + pm[0];
-      mm = base_m + pm[1] - am;
-    }
-    if (cnt && ((double)(c0 + a0 + cnt) >= want.k ||
-                (mass && m0 + (double)(am + mm) * unit >= want.mass) || meets(tid)))
-      atomicMin(&sh.pick[0], tid);
+    const uint32_t ac[3] = {base_c + pc[0], base_c + pc[1], base_c + pc[2]};
+    unsigned long long am[3] = {0, 0, 0};
+    if (mass)
+#pragma unroll
+      for (int x = 0; x < 3; ++x) am[x] = base_m + pm[x];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (ac[x + 1] > ac[x] && ((double)(c0 + ac[x + 1]) >= want.k ||
+                                (mass && (double)(m0 + am[x + 1]) >= want.mass) || meets(2 * tid + x)))
+        atomicMin(&sh.pick[0], 2 * tid + x);
     __syncthreads();
     Found f;
     f.b = sh.pick[0];
-    if (tid == min(f.b, kRowsBuckets - 1)) {
-      sh.pick[1] = (int)cnt;
-      sh.pick[2] = (int)(c0 + a0);
-      sh.pickm = am;
-    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (2 * tid + x == min(f.b, kRowsBuckets - 1)) {
+        sh.pick[1] = (int)(ac[x + 1] - ac[x]);
+        sh.pick[2] = (int)(c0 + ac[x]);
+        sh.pickm = m0 + am[x];
+      }
     __syncthreads();
     f.cnt = (uint32_t)sh.pick[1];
     f.above_c = (uint32_t)sh.pick[2];
@@ -392,7 +427,7 @@ struct Search {
   }
 
   // Keys of the bucket g.b0 == g.b1, from the monotone bucket().
-  __device__ void to_keys(Range& g) const {
+  __device__ __forceinline__ void to_keys(Range& g) const {
     const int b = g.b0;
     const uint32_t first = kKeyNone + 1;
     g.hi = row.top;
@@ -418,28 +453,33 @@ struct Search {
 
   // Splits a range of keys and narrows it to the first part where a border is
   // reached (else the last with any token); returns the tokens in it.
-  __device__ uint32_t split(Range& g, const Targets& want) {
+  __device__ __forceinline__ uint32_t split(Range& g, const Targets& want) {
+    RowsShared& sh = rows_shared();
     if (!g.keyed) to_keys(g);
     int shift = 0;
     while (((g.hi - g.lo) >> shift) >= (uint32_t)kRowsBuckets) ++shift;
     const uint32_t width = (1u << shift) - 1;
     cl.sync();  // the others have read the last slices
     const uint32_t lo = g.lo, hi = g.hi;
-    histogram(true, [&](float v, auto add) {
-      const uint32_t key = rows_key(v);
-      if (key >= lo && key <= hi) add((int)((hi - key) >> shift));
-    });
+    const int inside = g.b0;  // every key of the range is in this bucket
+    histogram(
+        true,
+        [&](float v, int, auto add) {
+          const uint32_t key = rows_key(v);
+          if (key >= lo && key <= hi) add((int)((hi - key) >> shift));
+        },
+        [&](int) { return inside; });
     // without a border: the last part with any token
     Targets all{INFINITY, INFINITY, 0};
     unsigned long long c, m;
     totals(c, m);
     all.k = (double)c;
-    const int last = find(all, 0, 0.0, false, kRowsBuckets - 1, [](int) { return false; }).b;
+    const int last = find(all, 0, 0, false, kRowsBuckets - 1, [](int) { return false; }).b;
     const Found f = find(want, g.count, g.mass, true, last, [&](int b) {
       return want.least && hi - ((uint32_t)b << shift) - width <= want.least;
     });
     g.count = f.above_c;
-    g.mass += (double)f.above_m * unit;
+    g.mass = f.above_m;
     const uint32_t first_key = hi - ((uint32_t)f.b << shift);
     if (first_key - lo > width) g.lo = first_key - width;
     g.hi = first_key;
@@ -448,13 +488,14 @@ struct Search {
 
   // The cluster's tokens in the range (at most kRowsList), sorted in rank order
   // into sh.sort; returns their number. `which`: the list to use.
-  __device__ uint32_t gather(const Range& g, int which) {
+  __device__ __forceinline__ uint32_t gather(const Range& g, int which) {
+    RowsShared& sh = rows_shared();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) sh.count[which] = 0;
     __syncthreads();
     row.each([&](float v, uint32_t token) {
       const uint32_t key = rows_key(v);
-      bool in = Row::real(v);
+      bool in = rows_real(v);
       if (g.keyed) {
         in = in && key >= g.lo && key <= g.hi;
       } else {
@@ -478,13 +519,14 @@ struct Search {
       if (lane >= o) incl += x;
     }
     const uint32_t m = min(__shfl_sync(0xffffffffu, incl, kRowsMaxCtas - 1), (uint32_t)kRowsList);
-    // two warps copy each CTA's list
+    // a warp copies each CTA's list
+    static_assert(kRowsWarps == kRowsMaxCtas, "one warp per CTA");
     {
-      const int q = warp & (kRowsMaxCtas - 1);
-      const uint32_t n = __shfl_sync(0xffffffffu, k, q), base = __shfl_sync(0xffffffffu, incl, q) - n;
-      if (q < ctas) {
-        const unsigned long long* src = cl.map_shared_rank(&sh.list[which][0], q);
-        for (uint32_t i = lane + 32 * (warp / kRowsMaxCtas); i < n; i += 64)
+      const uint32_t n = __shfl_sync(0xffffffffu, k, warp);
+      const uint32_t base = __shfl_sync(0xffffffffu, incl, warp) - n;
+      if (warp < ctas) {
+        const unsigned long long* src = cl.map_shared_rank(&sh.list[which][0], warp);
+        for (uint32_t i = lane; i < n; i += 32)
           if (base + i < (uint32_t)kRowsList) sh.sort[base + i] = src[i];
       }
     }
@@ -515,14 +557,14 @@ struct Search {
 
   // Token of the t-th (1-based) element in index order with this key; in the
   // CTA that holds it.
-  __device__ uint32_t nth_tie(uint32_t key, unsigned long long t) {
+  __device__ __forceinline__ uint32_t nth_tie(uint32_t key, unsigned long long t) {
+    RowsShared& sh = rows_shared();
     const int tid = threadIdx.x;
     if (tid == 0) sh.result = 0xffffffffu;
-    const float* x = row.x + (row.base - row.first);
     const uint32_t per = (row.count + kRowsThreads - 1) / kRowsThreads;
     const uint32_t lo = min(row.count, tid * per), hi = min(row.count, lo + per);
     unsigned long long mine = 0;
-    for (uint32_t i = lo; i < hi; ++i) mine += rows_key(x[i]) == key;
+    for (uint32_t i = lo; i < hi; ++i) mine += rows_key(row.at(i)) == key;
     unsigned long long total;
     unsigned long long before = rows_scan(mine, sh.redu, total);
     if (tid == 0) sh.ties = total;
@@ -531,7 +573,7 @@ struct Search {
     for (int c = 0; c < rank; ++c) before += *cl.map_shared_rank(&sh.ties, c);
     if (before < t && t <= before + mine)
       for (uint32_t i = lo; i < hi; ++i)
-        if (rows_key(x[i]) == key && ++before == t) {
+        if (rows_key(row.at(i)) == key && ++before == t) {
           sh.result = row.base + i;
           break;
         }
@@ -540,7 +582,8 @@ struct Search {
   }
 
   // The draw of a filtered row; the token in the CTA that writes it.
-  __device__ uint32_t filtered(const Targets& borders, double top_p, double u) {
+  __device__ __forceinline__ uint32_t filtered(const Targets& borders, double top_p, double u) {
+    RowsShared& sh = rows_shared();
     const int tid = threadIdx.x, rank = (int)cl.block_rank();
     const bool by_p = top_p < 1.0;
     Targets kept = borders;
@@ -548,33 +591,33 @@ struct Search {
     // then top-p needs the row's whole mass only
     bool mass = by_p && kept.k > (double)kRowsList / 2;
     if (by_p && !mass) {
-      double mine = 0.0, total;
-      row.each([&](float v, uint32_t) { mine += Row::real(v) ? row.weight(v) : 0.0; });
-      rows_scan(mine, sh.red, total);
+      unsigned long long mine = 0, total;
+      row.each([&](float v, uint32_t) { mine += rows_real(v) ? row.value_weight(v) : 0ull; });
+      rows_scan(mine, sh.redu, total);
       if (tid == 0) sh.total = total;  // read after the histogram's barrier
     }
-    const auto whole = [&](float v, auto add) {
-      if (Row::real(v)) add(row.bucket(v));
-    };
+    const auto whole = [](float, int b, auto add) { add(b); };
+    const auto itself = [](int b) { return b; };
     const auto never = [](int) { return false; };
-    double z = 0.0;  // the row's mass (by_p or mass)
+    unsigned long long z = 0;  // the row's mass (by_p or mass)
     Found end;       // bucket of the last kept token; kRowsBuckets: every token is kept
     for (;;) {
-      histogram(mass, whole);
+      histogram(mass, whole, itself);
       unsigned long long tc, tm;
       totals(tc, tm);
       if (mass) {
-        z = (double)tm * unit;
+        z = tm;
       } else if (by_p) {
-        const double x = rows_lane<double>(ctas, [&](int q) { return *cl.map_shared_rank(&sh.total, q); });
-        z = 0.0;
+        const unsigned long long x = rows_lane<unsigned long long>(
+            ctas, [&](int q) { return *cl.map_shared_rank(&sh.total, q); });
+        z = 0;
 #pragma unroll
         for (int q = 0; q < kRowsMaxCtas; ++q) z += __shfl_sync(0xffffffffu, x, q);
       }
-      if (by_p) kept.mass = top_p * z;
+      if (by_p) kept.mass = top_p * (double)z;
       // (without a mass histogram the border by mass is found in the list)
       const int most = kept.least ? row.bucket(rows_value(kept.least)) : kRowsBuckets;
-      end = find(kept, 0, 0.0, mass, most, never);
+      end = find(kept, 0, 0, mass, most, never);
       const uint32_t n = end.b < kRowsBuckets ? end.above_c + end.cnt : (uint32_t)tc;
       if (n <= (uint32_t)kRowsList) {
         end.cnt = n;
@@ -588,7 +631,7 @@ struct Search {
       cl.sync();    // the others have read these slices
     }
     const bool one_list = end.cnt <= (uint32_t)kRowsList;
-    double kept_mass = z;
+    unsigned long long kept_mass = z;
     uint32_t end_key = kKeyNone + 1;  // no key below it is kept
     double end_ties = INFINITY;       // and of it so many
     bool fresh = true;                // the slices are those of the whole row
@@ -596,7 +639,7 @@ struct Search {
     // not among the tokens that phase 0 listed
     for (int phase = 0; phase < 2; ++phase) {
       Targets want = kept;
-      Range g{false, 0, min(end.b, kRowsBuckets - 1), 0, 0, 0, 0.0};
+      Range g{false, 0, min(end.b, kRowsBuckets - 1), 0, 0, 0, 0};
       uint32_t members = end.cnt;
       if (!one_list) {
         Found f = end;
@@ -604,16 +647,16 @@ struct Search {
           if (end.b >= kRowsBuckets) continue;  // everything is kept
           f.cnt = end.cnt - end.above_c;
         } else {
-          want = Targets{INFINITY, u * kept_mass, 0};
+          want = Targets{INFINITY, u * (double)kept_mass, 0};
           if (!fresh) {
             cl.sync();
-            histogram(true, whole);
+            histogram(true, whole, itself);
           }
-          f = find(want, 0, 0.0, true, min(end.b, kRowsBuckets - 1), never);
+          f = find(want, 0, 0, true, min(end.b, kRowsBuckets - 1), never);
         }
         g.b0 = g.b1 = f.b;
         g.count = f.above_c;
-        g.mass = (double)f.above_m * unit;
+        g.mass = f.above_m;
         members = f.cnt;
         // a crowded bucket is split by the key's bits until it fits, or is one key
         while (members > (uint32_t)kRowsList && (!g.keyed || g.lo < g.hi)) {
@@ -623,9 +666,9 @@ struct Search {
       }
       // --- settle the border among the listed tokens (or equal keys)
       if (members > (uint32_t)kRowsList) {  // `members` equal logits
-        const double w = row.key_weight(g.lo);
+        const unsigned long long w = row.key_weight(g.lo);
         double n = want.k - (double)g.count;
-        if (w > 0.0) n = fmin(n, ceil((want.mass - g.mass) / w));
+        if (w) n = fmin(n, ceil((want.mass - (double)g.mass) / (double)w));
         n = fmax(1.0, fmin(n, (double)members));
         if (phase == 1) {
           if (g.lo == end_key) n = fmin(n, end_ties);
@@ -634,58 +677,55 @@ struct Search {
         if (want.least > g.lo) n = 0.0;  // min-p ends above them
         end_key = n > 0.0 ? g.lo : g.lo + 1;
         end_ties = n > 0.0 ? n : INFINITY;
-        kept_mass = g.mass + n * w;
+        kept_mass = g.mass + (unsigned long long)n * w;
         continue;
       }
       const uint32_t m = gather(g, phase);
-      const uint32_t at = 2 * tid;
-      uint32_t key[2];
-      double w[2], tw;
+      constexpr int kOwn = kRowsList / kRowsThreads;  // consecutive entries of a thread
+      const int at = kOwn * tid;
+      uint32_t key[kOwn];
+      unsigned long long run[kOwn], mine = 0, tw;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        key[i] = at + i < m ? (uint32_t)(sh.sort[at + i] >> 32) : 0u;
-        w[i] = row.key_weight(key[i]);
+      for (int i = 0; i < kOwn; ++i) {
+        key[i] = at + i < (int)m ? (uint32_t)(sh.sort[at + i] >> 32) : 0u;
+        if (at + i < (int)m) mine += row.key_weight(key[i]);
+        run[i] = mine;
       }
-      const double ew = g.mass + rows_scan(w[0] + w[1], sh.red, tw);
-      const double run[2] = {ew + w[0], ew + w[0] + w[1]};
+      const unsigned long long before = g.mass + rows_scan(mine, sh.redu, tw);
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) run[i] += before;
       // entries that a border allows, and the first that reaches one
-      __syncthreads();
       if (tid == 0) sh.pick[0] = (int)m - 1, sh.pick[1] = 0;
       __syncthreads();
       const uint32_t floor_key = phase == 0 ? want.least : end_key;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (at + i < m) {
-          if ((double)(g.count + at + i + 1) >= want.k ||
-              ((phase == 0 || w[i] > 0.0) && run[i] >= want.mass))
-            atomicMin(&sh.pick[0], (int)(at + i));
-          if (key[i] >= floor_key) atomicMax(&sh.pick[1], (int)(at + i) + 1);
+      for (int i = 0; i < kOwn; ++i)
+        if (at + i < (int)m) {
+          if ((double)(g.count + at + i + 1) >= want.k || (double)run[i] >= want.mass)
+            atomicMin(&sh.pick[0], at + i);
+          if (key[i] >= floor_key) atomicMax(&sh.pick[1], at + i + 1);
         }
       __syncthreads();
       int e = min(sh.pick[0], sh.pick[1] - 1);  // the last kept entry, or the draw; -1: above all
       if (phase == 0) {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+          if (at + i == e) sh.pickm = run[i];
         __syncthreads();
-        if ((uint32_t)e >= at && (uint32_t)e < at + 2) sh.pickd = run[e - at];
-        __syncthreads();
-        kept_mass = e >= 0 ? sh.pickd : g.mass;
-        if (!one_list && !(u * kept_mass > g.mass)) {
+        kept_mass = e >= 0 ? sh.pickm : g.mass;
+        if (!one_list && !(u * (double)kept_mass > (double)g.mass)) {
           // above this list: no key of it may be drawn
-          uint32_t hi = g.hi;
-          if (!g.keyed) {
-            to_keys(g);
-            hi = g.hi;
-          }
-          end_key = hi + 1;
+          if (!g.keyed) to_keys(g);
+          end_key = g.hi + 1;
           continue;
         }
         // the draw is among these, too
-        const double target = u * kept_mass;
+        const double target = u * (double)kept_mass;
         if (tid == 0) sh.pick[0] = e;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if ((int)at + i < e && w[i] > 0.0 && run[i] >= target)
-            atomicMin(&sh.pick[0], (int)(at + i));
+        for (int i = 0; i < kOwn; ++i)
+          if (at + i < e && (double)run[i] >= target) atomicMin(&sh.pick[0], at + i);
         __syncthreads();
         e = sh.pick[0];
       }
@@ -696,86 +736,93 @@ struct Search {
 
   // The draw of an unfiltered row, by the running sum in index order; the
   // token in the CTA that holds it.
-  __device__ uint32_t unfiltered(double u) {
+  __device__ __forceinline__ uint32_t unfiltered(double u) {
+    RowsShared& sh = rows_shared();
     const int tid = threadIdx.x, rank = (int)cl.block_rank();
     if (tid == 0) sh.result = 0xffffffffu, sh.last = 0;
-    const float* x = row.x + (row.base - row.first);
     const uint32_t per = (row.count + kRowsThreads - 1) / kRowsThreads | 1u;  // odd: no bank twice
     const uint32_t lo = min(row.count, tid * per), hi = min(row.count, lo + per);
-    double mine = 0.0;
+    unsigned long long mine = 0;
     uint32_t last = 0xffffffffu;
     for (uint32_t i = lo; i < hi; ++i) {
-      const double w = Row::real(x[i]) ? row.weight(x[i]) : 0.0;
-      mine += w;
-      if (w > 0.0) last = i;
+      const float v = row.at(i);
+      if (!rows_real(v)) continue;
+      mine += row.value_weight(v);
+      last = i;
     }
-    double total;
-    const double before = rows_scan(mine, sh.red, total);
+    unsigned long long total;
+    const unsigned long long before = rows_scan(mine, sh.redu, total);
     if (tid == 0) sh.total = total;
+    // the last CTA with a token takes what no sum reaches (u = 1)
+    if (last != 0xffffffffu) atomicMax(&sh.last, last + 1);
     cl.sync();
-    const double xs = rows_lane<double>(ctas, [&](int q) { return *cl.map_shared_rank(&sh.total, q); });
-    double z = 0.0, base = 0.0, run = 0.0;
-    int holder = 0;  // the CTA whose sums reach the draw (else the last with any)
+    const unsigned long long xs = rows_lane<unsigned long long>(
+        ctas, [&](int q) { return *cl.map_shared_rank(&sh.total, q); });
+    const uint32_t any = rows_lane<uint32_t>(
+        ctas, [&](int q) { return *cl.map_shared_rank(&sh.last, q); });
+    unsigned long long z = 0, base = 0, run = 0;
+    int holder = 0;
     bool reached = false;
 #pragma unroll
     for (int q = 0; q < kRowsMaxCtas; ++q) z += __shfl_sync(0xffffffffu, xs, q);
-    const double target = u * z;
+    const double target = u * (double)z;
 #pragma unroll
     for (int q = 0; q < kRowsMaxCtas; ++q) {
-      const double v = __shfl_sync(0xffffffffu, xs, q);
-      if (v > 0.0 && !reached) {
+      const unsigned long long v = __shfl_sync(0xffffffffu, xs, q);
+      if (__shfl_sync(0xffffffffu, any, q) && !reached) {
         holder = q;
         base = run;
-        reached = run + v >= target;
+        reached = (double)(run + v) >= target;
       }
       run += v;
     }
     if (holder != rank) return 0xffffffffu;
-    // the first chunk that reaches the draw holds the token; where rounding at
-    // its seam leaves the inner scan short, its last one
-    if (last != 0xffffffffu) {
-      atomicMax(&sh.last, last);
-      if (base + before + mine >= target) {
-        double r = base + before;
-        uint32_t hit = last;
-        for (uint32_t i = lo; i < hi; ++i) {
-          const double w = Row::real(x[i]) ? row.weight(x[i]) : 0.0;
-          r += w;
-          if (w > 0.0 && r >= target) {
-            hit = i;
-            break;
-          }
+    // the first chunk that reaches the draw holds the token
+    if (last != 0xffffffffu && (double)(base + before + mine) >= target) {
+      unsigned long long r = base + before;
+      uint32_t hit = last;
+      for (uint32_t i = lo; i < hi; ++i) {
+        const float v = row.at(i);
+        if (!rows_real(v)) continue;
+        r += row.value_weight(v);
+        if ((double)r >= target) {
+          hit = i;
+          break;
         }
-        atomicMin(&sh.result, hit);
       }
+      atomicMin(&sh.result, hit);
     }
     __syncthreads();
-    return row.base + (sh.result != 0xffffffffu ? sh.result : sh.last);
+    return row.base + (sh.result != 0xffffffffu ? sh.result : sh.last - 1);
   }
 };
 
+template <bool CACHED>
 __global__ void __launch_bounds__(kRowsThreads, 2)
     sample_rows_kernel(const __grid_constant__ RowsParams p) {
   extern __shared__ __align__(16) float s_row[];
-  __shared__ RowsShared sh;
+  RowsShared& sh = rows_shared();
   cg::cluster_group cl = cg::this_cluster();
   const int ctas = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t r = blockIdx.x / ctas;
-  Row row;
+  Row<CACHED> row;
   row.base = min(p.n, p.chunk * (uint32_t)rank);
   row.count = min(p.n, row.base + p.chunk) - row.base;
   const float* src = p.logits + r * p.stride + row.base;
-  row.cached = p.cached;
   row.x = src;
   row.first = row.base;
   row.n4 = (row.count + 3) / 4;
+  row.inf = false;
   if (tid == 0) mbar_init(&sh.bar, 1);
   mbar_fence_init();
-  if (tid < kRowsTable) sh.table[tid] = exp2((double)tid / kRowsTable);
+  for (int i = tid; i < kRowsTable; i += kRowsThreads) {
+    const double x = exp2(29.0 + (double)i / kRowsTable);
+    sh.table[i] = make_uint2((uint32_t)(x + 0.5), __float_as_uint((float)x));
+  }
   __syncthreads();
   pdl_wait();
-  if (p.cached) {
+  if (CACHED) {
     // the 16-byte aligned middle by bulk copies, the ragged ends by loads; the
     // copy keeps the row's misalignment, the ends are padded
     const uint32_t mis = (uint32_t)((reinterpret_cast<uintptr_t>(src) >> 2) & 3);
@@ -813,9 +860,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       best = x > best ? x : best;
     });
   } else {
-    uint32_t top = 0;
-    row.each([&](float v, uint32_t) { top = max(top, rows_key(v)); });
-    best = (unsigned long long)top << 32;
+    float top = -INFINITY;
+    row.each([&](float v, uint32_t) { top = fmaxf(top, v); });  // NaN gives way
+    best = (unsigned long long)rows_key(top) << 32;
   }
   best = warp_max_u64(best);
   if (lane == 0) sh.redu[warp] = best;
@@ -832,13 +879,27 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   } else if (row.top <= kKeyNone) {
     if (rank == 0) token = 0;  // nothing to draw from
   } else {
+    if (rows_value(row.top) == INFINITY) {
+      // only infinite logits are drawn, evenly: they become 0, the others -infinity
+      row.inf = true;
+      row.top = rows_key(0.0f);
+      if (CACHED) {
+        for (uint32_t i = tid; i < 4 * row.n4; i += kRowsThreads)
+          s_row[i] = s_row[i] == INFINITY ? 0.0f : -INFINITY;
+        __syncthreads();
+      }
+    }
     row.fmax = rows_value(row.top);
-    const float tt = fmaxf(t, 1e-30f);  // (what lies below differs from it by nothing)
+    // below |max| 1e-12 every other logit's weight is 0 already
+    const float tt = fmaxf(t, fmaxf(1e-30f, fabsf(row.fmax) * 1e-12f));
     row.per = kRowsPerNat / tt;
-    row.dmax = (double)row.fmax;
+    row.low = row.fmax - 64.0f * tt;
+    row.bits = p.mass_bits;
+    row.drop = p.drop;
     row.scale = (kRowsTable * 1.4426950408889634074) / (double)tt;
-    row.table = sh.table;
-    Search s{p, sh, row, cl, ctas, ldexp(1.0, -p.mass_bits)};
+    // one rounding for the whole row: a common factor next to 1 on all weights
+    row.shift = Row<CACHED>::kMagic - (double)row.fmax * row.scale;
+    Search<CACHED> s{row, cl, ctas, p.part_bits};
     const bool by_k = k > 0 && (uint32_t)k < p.n;
     if (!by_k && !(top_p < 1.0) && !(min_p > 0.0)) {
       token = s.unfiltered(u);
@@ -849,12 +910,14 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       } else if (min_p > 0.0) {
         // smallest key with w >= min_p (w grows with the key): a search with one
         // key per lane, at most seven rounds
-        uint32_t lo = kKeyNone, hi = row.top;  // w(lo) < bar <= w(hi)
+        const double bar = log(min_p);
+        const auto log_weight = [&](float v) { return ((double)v - (double)row.fmax) / (double)tt; };
+        uint32_t lo = kKeyNone, hi = row.top;  // w(lo) < min_p <= w(hi)
         while (hi - lo > 1) {
           const uint32_t step = (hi - lo - 1) / 32 + 1;
           const uint32_t probe = min(lo + step * (lane + 1), hi);
           const uint32_t yes = __ballot_sync(
-              0xffffffffu, probe == hi || row.weight(rows_value(probe)) >= min_p);
+              0xffffffffu, probe == hi || log_weight(rows_value(probe)) >= bar);
           const uint32_t at = __ffs(yes) - 1;
           hi = min(lo + step * (at + 1), hi);
           lo = lo + step * at;
@@ -920,11 +983,13 @@ minq_status minq_sample_rows(const float* logits, size_t row_stride, size_t n_ro
   int chunk_bits = 0, n_bits = 0;
   while ((1u << chunk_bits) < p.chunk) ++chunk_bits;
   while ((1u << n_bits) < p.n) ++n_bits;
-  p.part_bits = 32 - chunk_bits < 16 ? 32 - chunk_bits : 16;
-  p.mass_bits = 3 * p.part_bits - 1 < 62 - n_bits ? 3 * p.part_bits - 1 : 62 - n_bits;
-  if (p.mass_bits > 47) p.mass_bits = 47;
+  // sums of a chunk's parts fit 32 bits, those of the row 63
+  p.part_bits = 32 - chunk_bits < 15 ? 32 - chunk_bits : 15;
+  p.drop = 30 - 2 * p.part_bits;
+  p.mass_bits = 62 - n_bits < 47 ? 62 - n_bits : 47;
   const size_t smem = p.cached ? ((size_t)p.chunk + 8) * sizeof(float) : 0;
-  const void* fn = reinterpret_cast<const void*>(sample_rows_kernel);
+  auto kernel = p.cached ? sample_rows_kernel<true> : sample_rows_kernel<false>;
+  const void* fn = reinterpret_cast<const void*>(kernel);
   MINQ_TRY(ensure_dynamic_smem(fn, smem));
   prefer_max_shared(fn);
   cudaLaunchConfig_t cfg = {};
@@ -941,7 +1006,7 @@ minq_status minq_sample_rows(const float* logits, size_t row_stride, size_t n_ro
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   count_launch();
-  MINQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_rows_kernel, p));
+  MINQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
   return MINQ_OK;
 }
 
