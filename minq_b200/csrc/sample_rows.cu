@@ -188,16 +188,15 @@ struct Row {
     const float v = x[base - first + i];
     return CACHED || !inf ? v : v == INFINITY ? 0.0f : -INFINITY;
   }
-  // Every element of this CTA: f(value, token).
+  // Every element of this CTA, four at a time: f(values, first token). The
+  // bodies keep to straight-line code, so that four elements' chains overlap.
   template <class F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each4(F f) const {
 #pragma unroll 2
     for (uint32_t j = threadIdx.x; j < n4; j += kRowsThreads) {
-      const float4 v = load(j);
-      f(v.x, first + 4 * j);
-      f(v.y, first + 4 * j + 1);
-      f(v.z, first + 4 * j + 2);
-      f(v.w, first + 4 * j + 3);
+      const float4 q = load(j);
+      const float v[4] = {q.x, q.y, q.z, q.w};
+      f(v, first + 4 * j);
     }
   }
   // Bucket of a value, in order (the nearest of (fmax - v) * per).
@@ -228,8 +227,8 @@ struct Row {
   static constexpr int kMagicK = (int)((0x41b8000000000000ull >> 24) & 0xffffffffull);
   // A sum of weights of bucket b in 64-bit units (2^-bits).
   __device__ __forceinline__ unsigned long long wide(unsigned long long w, int b) const {
-    const int up = bits - 29 + drop + unit(b);
-    return up >= 0 ? w << up : up > -64 ? w >> -up : 0ull;
+    const int up = bits - 29 + drop + unit(b);  // -22 .. 22
+    return up >= 0 ? w << up : w >> -up;
   }
   __device__ __forceinline__ unsigned long long value_weight(float v) const {
     const int b = bucket(v);
@@ -278,28 +277,44 @@ struct Search {
   cg::cluster_group cl;
   const int ctas, part_bits;
 
-  // Adds up the cluster's histogram: f(value, bucket, add) calls add(i) for a
-  // token that counts in entry i; unit(i): the bucket of entry i's units.
-  // Afterwards every CTA's slice holds running sums.
+  // Adds up the cluster's histogram: entry(value, bucket) gives a token's entry,
+  // -1 for none; unit(i): the bucket of entry i's units. Afterwards
+  // every CTA's slice holds running sums.
   template <class F, class U>
-  __device__ __forceinline__ void histogram(bool mass, F f, U unit) {
+  __device__ __forceinline__ void histogram(bool mass, F entry, U unit) {
     RowsShared& sh = rows_shared();
     const int tid = threadIdx.x;
     for (int i = tid; i < (mass ? 3 : 1) * kRowsBuckets; i += kRowsThreads) (&sh.hist[0][0])[i] = 0;
     __syncthreads();
     const uint32_t mask = (1u << part_bits) - 1;
-    row.each([&](float v, uint32_t) {
-      if (!rows_real(v)) return;
-      const int b = row.bucket(v);
-      f(v, b, [&](int i) {
-        atomicAdd(&sh.hist[0][i], 1u);
-        if (mass) {
-          const uint32_t w = row.weight(v, b);
-          atomicAdd(&sh.hist[1][i], w & mask);
-          atomicAdd(&sh.hist[2][i], w >> part_bits);
+    if (mass) {
+      row.each4([&](const float* v, uint32_t) {
+        int at[4];
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int b = row.bucket(v[i]);
+          w[i] = row.weight(v[i], b);
+          at[i] = rows_real(v[i]) ? entry(v[i], b) : -1;
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (at[i] >= 0) {
+            atomicAdd(&sh.hist[0][at[i]], 1u);
+            atomicAdd(&sh.hist[1][at[i]], w[i] & mask);
+            atomicAdd(&sh.hist[2][at[i]], w[i] >> part_bits);
+          }
       });
-    });
+    } else {
+      row.each4([&](const float* v, uint32_t) {
+        int at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = rows_real(v[i]) ? entry(v[i], row.bucket(v[i])) : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (at[i] >= 0) atomicAdd(&sh.hist[0][at[i]], 1u);
+      });
+    }
     cl.sync();
     // this CTA's slice: thread i sums entries 2i, 2i + 1 of it over the cluster
     const int per = kRowsBuckets / ctas, rank = (int)cl.block_rank();
@@ -464,9 +479,9 @@ struct Search {
     const int inside = g.b0;  // every key of the range is in this bucket
     histogram(
         true,
-        [&](float v, int, auto add) {
+        [&](float v, int) {
           const uint32_t key = rows_key(v);
-          if (key >= lo && key <= hi) add((int)((hi - key) >> shift));
+          return key >= lo && key <= hi ? (int)((hi - key) >> shift) : -1;
         },
         [&](int) { return inside; });
     // without a border: the last part with any token
@@ -493,19 +508,31 @@ struct Search {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) sh.count[which] = 0;
     __syncthreads();
-    row.each([&](float v, uint32_t token) {
-      const uint32_t key = rows_key(v);
-      bool in = rows_real(v);
+    row.each4([&](const float* v, uint32_t token) {
+      uint32_t in = 0;
       if (g.keyed) {
-        in = in && key >= g.lo && key <= g.hi;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t key = rows_key(v[i]);
+          in |= (uint32_t)(key >= g.lo && key <= g.hi) << i;
+        }
       } else {
-        const int b = row.bucket(v);
-        in = in && b >= g.b0 && b <= g.b1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int b = row.bucket(v[i]);
+          in |= (uint32_t)(rows_real(v[i]) && b >= g.b0 && b <= g.b1) << i;
+        }
       }
       if (in) {
-        const uint32_t at = atomicAdd(&sh.count[which], 1u);
-        if (at < (uint32_t)kRowsList)
-          sh.list[which][at] = ((unsigned long long)key << 32) | (uint32_t)~token;
+        uint32_t at = atomicAdd(&sh.count[which], (uint32_t)__popc(in));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((in >> i) & 1) {
+            if (at < (uint32_t)kRowsList)
+              sh.list[which][at] =
+                  ((unsigned long long)rows_key(v[i]) << 32) | (uint32_t)~(token + i);
+            ++at;
+          }
       }
     });
     cl.sync();
@@ -592,11 +619,17 @@ struct Search {
     bool mass = by_p && kept.k > (double)kRowsList / 2;
     if (by_p && !mass) {
       unsigned long long mine = 0, total;
-      row.each([&](float v, uint32_t) { mine += rows_real(v) ? row.value_weight(v) : 0ull; });
+      row.each4([&](const float* v, uint32_t) {
+        unsigned long long w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = row.value_weight(v[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += rows_real(v[i]) ? w[i] : 0ull;
+      });
       rows_scan(mine, sh.redu, total);
       if (tid == 0) sh.total = total;  // read after the histogram's barrier
     }
-    const auto whole = [](float, int b, auto add) { add(b); };
+    const auto whole = [](float, int b) { return b; };
     const auto itself = [](int b) { return b; };
     const auto never = [](int) { return false; };
     unsigned long long z = 0;  // the row's mass (by_p or mass)
@@ -855,13 +888,18 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   // minq_argmax (the padding comes last in it)
   unsigned long long best = 0;
   if (greedy) {
-    row.each([&](float v, uint32_t token) {
-      const unsigned long long x = argmax_pack(v, token);
-      best = x > best ? x : best;
+    row.each4([&](const float* v, uint32_t token) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned long long x = argmax_pack(v[i], token + i);
+        best = x > best ? x : best;
+      }
     });
   } else {
     float top = -INFINITY;
-    row.each([&](float v, uint32_t) { top = fmaxf(top, v); });  // NaN gives way
+    row.each4([&](const float* v, uint32_t) {  // NaN gives way
+      top = fmaxf(top, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+    });
     best = (unsigned long long)rows_key(top) << 32;
   }
   best = warp_max_u64(best);
