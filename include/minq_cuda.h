@@ -456,7 +456,8 @@ minq_status minq_generate_sampled(minq_model* m, minq_sampler* s, const uint32_t
 /* captured into a CUDA graph. All pointers are device memory.                */
 
 /* What a pages call found (info[0]): 0, or the bits below. A call that finds
- * anything changes neither tables nor lengths nor the free list. */
+ * anything changes neither tables nor lengths nor the free list (the first
+ * *n_free entries of free_pages; what lies above them is scratch). */
 enum {
   MINQ_PAGES_SHORT = 1,           /* too few free pages: info[1] more are needed */
   MINQ_PAGES_ROW_FULL = 2,        /* a request does not fit its table row */

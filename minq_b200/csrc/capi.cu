@@ -114,10 +114,13 @@ minq_status take_device_status() {
 }
 
 minq_status require_device() {
+  static std::atomic<bool> seen{false};  // devices do not go away
+  if (seen.load(std::memory_order_relaxed)) return MINQ_OK;
   int n = 0;
   cudaError_t e = cudaGetDeviceCount(&n);
   if (e != cudaSuccess || n == 0)
     return fail(MINQ_ERR_CUDA, "no CUDA device available (the CUDA path has no CPU fallback)");
+  seen.store(true, std::memory_order_relaxed);
   return MINQ_OK;
 }
 

@@ -41,7 +41,7 @@ constexpr int kPagesMaxCtas = 8;  // the portable cluster size
 struct PagesParams {
   const int* lens;
   const int* arg;  // new tokens (extend) or lengths to keep (trim)
-  int n_req, page_size;
+  int n_req, page_shift;
   int* table;
   size_t table_stride;
   int* free_pages;
@@ -111,20 +111,24 @@ __device__ __forceinline__ int find_last(const int* start, int n, int x) {
 }
 
 // Pages of `len` positions.
-__device__ __forceinline__ long long pages_of(long long len, int P) { return (len + P - 1) / P; }
+__device__ __forceinline__ int pages_of(int len, int shift) {
+  return (int)(((unsigned)len + ((1u << shift) - 1)) >> shift);
+}
 
 template <bool EXTEND>
 __global__ void __launch_bounds__(kPagesThreads) pages_kernel(PagesParams p) {
   extern __shared__ int dyn[];
-  int* s_tok = dyn;                  // [n_req] first token (extend)
-  int* s_page = dyn + p.n_req;       // [n_req] first moved page
+  int* s_page = dyn;                  // [n_req] first moved page
+  int* s_base = dyn + p.n_req;        // [n_req] its column in the request's table row
+  int* s_tok = dyn + 2 * p.n_req;     // [n_req] first token (extend)
+  int* s_len = dyn + 3 * p.n_req;     // [n_req] length before (extend)
   __shared__ PagesShared sh;
   pdl_wait();
   cg::cluster_group cl = cg::this_cluster();
   const int ncta = (int)cl.num_blocks(), cta = (int)cl.block_rank();
   const int tid = threadIdx.x, nthreads = blockDim.x;
   const int gid = cta * nthreads + tid, gthreads = ncta * nthreads;
-  const int P = p.page_size;
+  const int shift = p.page_shift, mask = (1 << shift) - 1;
   if (tid == 0) sh.flags = 0;
   __syncthreads();
   cl.barrier_arrive();  // this CTA's flags word may be written by the others
@@ -132,30 +136,42 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(PagesParams p) {
   // every CTA: all requests' lengths, checked and scanned
   const int n_free = *p.n_free;
   int flags = n_free < 0 || n_free > p.n_pages ? MINQ_PAGES_BAD_PAGE : 0;
-  const long long cap = (long long)p.table_stride * P;
+  const long long cap = (long long)p.table_stride << shift;
   long long tokens = 0, pages = 0;
   for (int base = 0; base < p.n_req; base += nthreads) {
     const int r = base + tid;
     long long t = 0, g = 0;
+    int len = 0, from = 0;
     if (r < p.n_req) {
-      const long long len = p.lens[r], arg = p.arg[r];
+      len = p.lens[r];
+      const int arg = p.arg[r];
       if (len < 0 || arg < 0) {
         flags |= MINQ_PAGES_BAD_LENGTH;
       } else if (EXTEND) {
+        const long long after = (long long)len + arg;
+        if (after > cap || after > 0x7fffffffll) {
+          flags |= MINQ_PAGES_ROW_FULL;
+        } else {
+          from = pages_of(len, shift);
+          g = pages_of((int)after, shift) - from;
+        }
         t = arg;
-        g = pages_of(len + arg, P) - pages_of(len, P);
-        if (len + arg > cap || len + arg > 0x7fffffffll) flags |= MINQ_PAGES_ROW_FULL;
       } else {
         if (len > cap) flags |= MINQ_PAGES_ROW_FULL;
-        g = pages_of(len, P) - pages_of(arg < len ? arg : len, P);
+        from = pages_of(min(arg, len), shift);
+        g = pages_of(len, shift) - from;
       }
     }
     long long tt, tg;
     scan2(t, g, tt, tg, sh);
     // offsets past 2^31 only occur in a step that is refused below
     if (r < p.n_req) {
-      if (EXTEND) s_tok[r] = (int)(tokens + t);
       s_page[r] = (int)(pages + g);
+      s_base[r] = from;
+      if (EXTEND) {
+        s_tok[r] = (int)(tokens + t);
+        s_len[r] = len;
+      }
     }
     tokens += tt;
     pages += tg;
@@ -170,70 +186,60 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(PagesParams p) {
   cl.barrier_wait();
 
   // the ids that move must be pages of the pool (spread over the cluster)
-  if (flags == 0) {
+  const int moved = flags ? 0 : (int)pages;
+  if (moved) {
     int bad = 0;
-    for (long long j = gid; j < pages; j += gthreads) {
+    for (int j = gid; j < moved; j += gthreads) {
       int id;
       if (EXTEND) {
         id = p.free_pages[n_free - 1 - j];
       } else {
-        const int r = find_last(s_page, p.n_req, (int)j);
-        const long long len = p.lens[r], keep = p.arg[r];
-        id = p.table[(size_t)r * p.table_stride + pages_of(keep < len ? keep : len, P) +
-                     (j - s_page[r])];
+        const int r = find_last(s_page, p.n_req, j);
+        id = p.table[(size_t)r * p.table_stride + s_base[r] + (j - s_page[r])];
+        // (above the free pages: no part of the list until n_free_out says so)
+        p.free_pages[n_free + moved - 1 - j] = id;
       }
       bad |= id < 0 || id >= p.n_pages;
     }
     if (bad)
       for (int c = 0; c < ncta; ++c) atomicOr(cl.map_shared_rank(&sh.flags, c), MINQ_PAGES_BAD_PAGE);
   }
-  // after this barrier every length and the free count have been read for the
-  // decision; what is still needed of them below is read before they change
+  // after this barrier every length and the free count have been read: they may
+  // be overwritten in place
   cl.sync();
   flags = sh.flags;
-
   const bool ok = flags == 0;
   if (EXTEND) {
-    if (!ok) tokens = 0;
+    const int n_tok = ok ? (int)tokens : 0;
     for (int t = gid; t < p.max_tokens; t += gthreads) {
       long long slot = -1;
       int pos = 0;
-      if (t < tokens) {
+      if (t < n_tok) {
         const int r = find_last(s_tok, p.n_req, t);
-        pos = p.lens[r] + (t - s_tok[r]);
-        const long long held = pages_of(p.lens[r], P);
-        const int col = pos / P;
-        const int id = col < held ? p.table[(size_t)r * p.table_stride + col]
-                                  : p.free_pages[n_free - 1 - (s_page[r] + (col - held))];
-        slot = id < 0 || id >= p.n_pages ? -1 : (long long)id * P + (pos - col * P);
+        pos = s_len[r] + (t - s_tok[r]);
+        const int col = pos >> shift;
+        const int id = col < s_base[r] ? p.table[(size_t)r * p.table_stride + col]
+                                       : p.free_pages[n_free - 1 - (s_page[r] + (col - s_base[r]))];
+        slot = id < 0 || id >= p.n_pages ? -1 : ((long long)id << shift) + (pos & mask);
       }
       p.slots[t] = slot;
       if (p.positions) p.positions[t] = pos;
     }
-  }
-  if (ok) {
-    for (long long j = gid; j < pages; j += gthreads) {
-      const int r = find_last(s_page, p.n_req, (int)j);
-      const long long len = p.lens[r];
-      if (EXTEND) {
-        p.table[(size_t)r * p.table_stride + pages_of(len, P) + (j - s_page[r])] =
+    if (ok)
+      for (int j = gid; j < moved; j += gthreads) {
+        const int r = find_last(s_page, p.n_req, j);
+        p.table[(size_t)r * p.table_stride + s_base[r] + (j - s_page[r])] =
             p.free_pages[n_free - 1 - j];
-      } else {
-        const long long keep = p.arg[r] < len ? p.arg[r] : len;
-        p.free_pages[n_free + pages - 1 - j] =
-            p.table[(size_t)r * p.table_stride + pages_of(keep, P) + (j - s_page[r])];
       }
-    }
   }
-  cl.sync();  // every read of lens is done: they may be overwritten in place
   for (int r = gid; r < p.n_req; r += gthreads) {
     const int len = p.lens[r], arg = p.arg[r];
     p.lens_out[r] = !ok ? len : EXTEND ? len + arg : min(len, arg);
     if (EXTEND) p.q_start[r] = ok ? s_tok[r] : 0;
   }
   if (gid == 0) {
-    *p.n_free_out = !ok ? n_free : EXTEND ? n_free - (int)pages : n_free + (int)pages;
-    if (EXTEND) p.q_start[p.n_req] = (int)tokens;
+    *p.n_free_out = !ok ? n_free : EXTEND ? n_free - moved : n_free + moved;
+    if (EXTEND) p.q_start[p.n_req] = ok ? (int)tokens : 0;
     p.info[0] = flags;
     const long long lack = EXTEND && n_free >= 0 ? pages - n_free : 0;
     p.info[1] = (flags & MINQ_PAGES_SHORT) ? (int)(lack > 0x7fffffffll ? 0x7fffffffll : lack) : 0;
@@ -243,12 +249,13 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(PagesParams p) {
 
 template <bool EXTEND>
 minq_status launch_pages(const PagesParams& p, cudaStream_t s) {
-  // one thread a token (or request); 8 CTAs only when there is work for them
-  const int items = EXTEND ? (p.max_tokens > p.n_req ? p.max_tokens : p.n_req) : p.n_req;
+  // one thread a token, or a few pages a request (trim's are not known here); 8
+  // CTAs only when there is work for them
+  const int items = EXTEND ? (p.max_tokens > p.n_req ? p.max_tokens : p.n_req) : 32 * p.n_req;
   const int threads = items <= 128 ? 128 : items <= 512 ? 512 : kPagesThreads;
   int ctas = 1;
   while (ctas < kPagesMaxCtas && ctas * threads < items) ctas *= 2;
-  const size_t smem = 2 * (size_t)p.n_req * sizeof(int);
+  const size_t smem = (EXTEND ? 4 : 2) * (size_t)p.n_req * sizeof(int);
   const void* fn = reinterpret_cast<const void*>(pages_kernel<EXTEND>);
   MINQ_TRY(ensure_dynamic_smem(fn, smem));
   prefer_max_shared(fn);
@@ -310,7 +317,7 @@ minq_status minq_pages_extend(const int32_t* lens, const int32_t* new_tokens, si
   p.lens = lens;
   p.arg = new_tokens;
   p.n_req = (int)n_req;
-  p.page_size = (int)page_size;
+  while ((size_t(1) << p.page_shift) < page_size) ++p.page_shift;
   p.table = table;
   p.table_stride = table_stride;
   p.free_pages = const_cast<int32_t*>(free_pages);  // only read when extending
@@ -339,7 +346,7 @@ minq_status minq_pages_trim(const int32_t* lens, const int32_t* keep, size_t n_r
   p.lens = lens;
   p.arg = keep;
   p.n_req = (int)n_req;
-  p.page_size = (int)page_size;
+  while ((size_t(1) << p.page_shift) < page_size) ++p.page_shift;
   p.table = const_cast<int32_t*>(table);  // only read when trimming
   p.table_stride = table_stride;
   p.free_pages = free_pages;

@@ -57,7 +57,7 @@ constexpr int kRowsThreads = 256;
 constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsBuckets = 512;           // two per thread
 constexpr float kRowsPerNat = 32.0f;        // buckets per unit of (max - x) / T
-constexpr int kRowsList = 1024;             // tokens a list holds: four per thread
+constexpr int kRowsList = 4 * kRowsThreads; // tokens a list holds: four per thread
 constexpr int kRowsMaxCtas = 8;             // the portable cluster size
 constexpr uint32_t kRowsCached = 48 * 1024; // floats of a row that a CTA can hold
 constexpr int kRowsTable = 256;
@@ -102,9 +102,10 @@ struct RowsShared {
   // of the histogram
   union {
     uint32_t hist[3][kRowsBuckets];
-    unsigned long long sort[kRowsList];
+    alignas(16) unsigned long long sort[kRowsList];
   };
   unsigned long long list[2][kRowsList];
+  uint32_t place[kRowsList];
   // this CTA's slice of the cluster's buckets: running sums before each
   unsigned long long slice_m[kRowsBuckets + 1];
   uint32_t slice_c[kRowsBuckets + 2];
@@ -254,11 +255,10 @@ struct Targets {
   uint32_t least;  // smallest key kept (0: any)
 };
 
-// What the search has narrowed the border down to: buckets [b0, b1] of the
-// row, or (keyed) keys [lo, hi]; `count` tokens and `mass` lie above.
+// What the search has narrowed the border down to: keys [lo, hi] (of bucket b,
+// where it is split); `count` tokens and `mass` lie above.
 struct Range {
-  bool keyed;
-  int b0, b1;
+  int b;
   uint32_t lo, hi;
   uint32_t count;
   unsigned long long mass;
@@ -287,6 +287,11 @@ struct Search {
     for (int i = tid; i < (mass ? 3 : 1) * kRowsBuckets; i += kRowsThreads) (&sh.hist[0][0])[i] = 0;
     __syncthreads();
     const uint32_t mask = (1u << part_bits) - 1;
+    // the last entry (everything far below the maximum) is often crowded, and
+    // adds to one word run one after the other: it is summed in registers
+    uint32_t last_c = 0;
+    unsigned long long last_m = 0;
+    constexpr int kLast = kRowsBuckets - 1;
     if (mass) {
       row.each4([&](const float* v, uint32_t) {
         int at[4];
@@ -298,12 +303,15 @@ struct Search {
           at[i] = rows_real(v[i]) ? entry(v[i], b) : -1;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (at[i] >= 0) {
+        for (int i = 0; i < 4; ++i) {
+          last_c += at[i] == kLast ? 1u : 0u;
+          last_m += at[i] == kLast ? w[i] : 0u;
+          if ((uint32_t)at[i] < (uint32_t)kLast) {
             atomicAdd(&sh.hist[0][at[i]], 1u);
             atomicAdd(&sh.hist[1][at[i]], w[i] & mask);
             atomicAdd(&sh.hist[2][at[i]], w[i] >> part_bits);
           }
+        }
       });
     } else {
       row.each4([&](const float* v, uint32_t) {
@@ -311,9 +319,23 @@ struct Search {
 #pragma unroll
         for (int i = 0; i < 4; ++i) at[i] = rows_real(v[i]) ? entry(v[i], row.bucket(v[i])) : -1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (at[i] >= 0) atomicAdd(&sh.hist[0][at[i]], 1u);
+        for (int i = 0; i < 4; ++i) {
+          last_c += at[i] == kLast ? 1u : 0u;
+          if ((uint32_t)at[i] < (uint32_t)kLast) atomicAdd(&sh.hist[0][at[i]], 1u);
+        }
       });
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      last_c += __shfl_xor_sync(0xffffffffu, last_c, o);
+      last_m += __shfl_xor_sync(0xffffffffu, last_m, o);
+    }
+    if ((tid & 31) == 0 && last_c) {
+      atomicAdd(&sh.hist[0][kLast], last_c);
+      if (mass) {  // (the high part takes what its 32 bits hold of the chunk's sum)
+        atomicAdd(&sh.hist[1][kLast], (uint32_t)last_m & mask);
+        atomicAdd(&sh.hist[2][kLast], (uint32_t)(last_m >> part_bits));
+      }
     }
     cl.sync();
     // this CTA's slice: thread i sums entries 2i, 2i + 1 of it over the cluster
@@ -441,42 +463,32 @@ struct Search {
     return f;
   }
 
-  // Keys of the bucket g.b0 == g.b1, from the monotone bucket().
-  __device__ __forceinline__ void to_keys(Range& g) const {
-    const int b = g.b0;
-    const uint32_t first = kKeyNone + 1;
-    g.hi = row.top;
-    g.lo = first;
-    if (b > 0) {  // largest key with bucket >= b
-      uint32_t x = first, y = row.top;  // bucket(x) >= b > bucket(y)
-      while (y - x > 1) {
-        const uint32_t m = x + (y - x) / 2;
-        (row.bucket(rows_value(m)) >= b ? x : y) = m;
-      }
-      g.hi = x;
+  // Smallest key above -infinity whose bucket is at most b (row.top's is 0): a
+  // search with one key per lane.
+  __device__ __forceinline__ uint32_t key_of(int b) const {
+    const int lane = threadIdx.x & 31;
+    uint32_t lo = kKeyNone, hi = row.top;  // bucket(lo) > b >= bucket(hi)
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo - 1) / 32 + 1;
+      const uint32_t probe = min(lo + step * (lane + 1), hi);
+      const uint32_t at =
+          __ffs(__ballot_sync(0xffffffffu, probe == hi || row.bucket(rows_value(probe)) <= b)) - 1;
+      hi = min(lo + step * (at + 1), hi);
+      lo = lo + step * at;
     }
-    if (row.bucket(rows_value(first)) > b) {  // smallest key with bucket <= b
-      uint32_t x = first, y = row.top;  // bucket(x) > b >= bucket(y)
-      while (y - x > 1) {
-        const uint32_t m = x + (y - x) / 2;
-        (row.bucket(rows_value(m)) > b ? x : y) = m;
-      }
-      g.lo = y;
-    }
-    g.keyed = true;
+    return hi;
   }
 
   // Splits a range of keys and narrows it to the first part where a border is
   // reached (else the last with any token); returns the tokens in it.
   __device__ __forceinline__ uint32_t split(Range& g, const Targets& want) {
     RowsShared& sh = rows_shared();
-    if (!g.keyed) to_keys(g);
     int shift = 0;
     while (((g.hi - g.lo) >> shift) >= (uint32_t)kRowsBuckets) ++shift;
     const uint32_t width = (1u << shift) - 1;
     cl.sync();  // the others have read the last slices
     const uint32_t lo = g.lo, hi = g.hi;
-    const int inside = g.b0;  // every key of the range is in this bucket
+    const int inside = g.b;  // every key of the range is in this bucket
     histogram(
         true,
         [&](float v, int) {
@@ -501,28 +513,18 @@ struct Search {
     return f.cnt;
   }
 
-  // The cluster's tokens in the range (at most kRowsList), sorted in rank order
-  // into sh.sort; returns their number. `which`: the list to use.
+  // The cluster's tokens with keys in [lo, hi] (at most kRowsList), sorted in rank
+  // order into sh.list[which ^ 1]; returns their number. `which`: the list to use.
   __device__ __forceinline__ uint32_t gather(const Range& g, int which) {
     RowsShared& sh = rows_shared();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) sh.count[which] = 0;
     __syncthreads();
+    const float lo = rows_value(g.lo), hi = rows_value(g.hi);
     row.each4([&](const float* v, uint32_t token) {
       uint32_t in = 0;
-      if (g.keyed) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t key = rows_key(v[i]);
-          in |= (uint32_t)(key >= g.lo && key <= g.hi) << i;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int b = row.bucket(v[i]);
-          in |= (uint32_t)(rows_real(v[i]) && b >= g.b0 && b <= g.b1) << i;
-        }
-      }
+      for (int i = 0; i < 4; ++i) in |= (uint32_t)(v[i] >= lo && v[i] <= hi) << i;
       if (in) {
         uint32_t at = atomicAdd(&sh.count[which], (uint32_t)__popc(in));
 #pragma unroll
@@ -557,28 +559,49 @@ struct Search {
           if (base + i < (uint32_t)kRowsList) sh.sort[base + i] = src[i];
       }
     }
-    uint32_t N = 2;
-    while (N < m) N <<= 1;
-    for (uint32_t i = m + tid; i < N; i += kRowsThreads) sh.sort[i] = 0ull;
+    if (tid == 0 && (m & 1)) sh.sort[m] = 0ull;
     __syncthreads();
-    // bitonic, descending; pairs less than 64 apart stay within one warp's 64
-    // entries
-    for (uint32_t kk = 2; kk <= N; kk <<= 1)
-      for (uint32_t j = kk >> 1; j > 0; j >>= 1) {
-        for (uint32_t i = tid; i < N / 2; i += kRowsThreads) {
-          const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;  // pairs j apart
-          const unsigned long long x = sh.sort[a], y = sh.sort[b];
-          if ((a & kk) == 0 ? x < y : x > y) {
-            sh.sort[a] = y;
-            sh.sort[b] = x;
-          }
-        }
-        if (j > 32 || (j == 1 && kk >= 64))
-          __syncthreads();
-        else
-          __syncwarp();
+    // an entry's place is the number of larger ones (they all differ); a long
+    // list's entries are dealt out over the cluster
+    unsigned long long* sorted = sh.list[which ^ 1];
+    const bool dealt = ctas > 1 && m > (uint32_t)kRowsThreads;
+    const uint32_t share = dealt ? (m + ctas - 1) / ctas : m;
+    const uint32_t e0 = dealt ? min(m, share * cl.block_rank()) : 0u, e1 = min(m, e0 + share);
+    for (uint32_t e = tid; e < e1 - e0; e += kRowsThreads) sh.place[e] = 0;
+    __syncthreads();
+    // each warp compares with its part of the list, four entries per lane at a time
+    const uint32_t part = ((m + kRowsWarps - 1) / kRowsWarps + 1) & ~1u;
+    const uint32_t j0 = min(m, part * warp), j1 = min(m, j0 + part);
+    for (uint32_t e = e0; e < e1; e += 128) {
+      unsigned long long x[4];
+      uint32_t place[4] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[i] = e + 32 * i + lane < e1 ? sh.sort[e + 32 * i + lane] : ~0ull;
+#pragma unroll 2
+      for (uint32_t j = j0; j < j1; j += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.sort[j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) place[i] += (o.x > x[i] ? 1u : 0u) + (o.y > x[i] ? 1u : 0u);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (place[i]) atomicAdd(&sh.place[e - e0 + 32 * i + lane], place[i]);
+    }
     __syncthreads();
+    for (uint32_t e = tid; e < e1 - e0; e += kRowsThreads) {
+      const unsigned long long x = sh.sort[e0 + e];
+      const uint32_t place = sh.place[e];
+      if (dealt) {
+        for (int q = 0; q < ctas; ++q) cl.map_shared_rank(sorted, q)[place] = x;
+      } else {
+        sorted[place] = x;
+      }
+    }
+    if (dealt)
+      cl.sync();
+    else
+      __syncthreads();
     return m;
   }
 
@@ -672,9 +695,11 @@ struct Search {
     // not among the tokens that phase 0 listed
     for (int phase = 0; phase < 2; ++phase) {
       Targets want = kept;
-      Range g{false, 0, min(end.b, kRowsBuckets - 1), 0, 0, 0, 0};
+      Range g{0, kKeyNone + 1, row.top, 0, 0};
       uint32_t members = end.cnt;
-      if (!one_list) {
+      if (one_list) {
+        g.lo = key_of(min(end.b, kRowsBuckets - 1));
+      } else {
         Found f = end;
         if (phase == 0) {
           if (end.b >= kRowsBuckets) continue;  // everything is kept
@@ -687,12 +712,14 @@ struct Search {
           }
           f = find(want, 0, 0, true, min(end.b, kRowsBuckets - 1), never);
         }
-        g.b0 = g.b1 = f.b;
+        g.b = f.b;
+        g.lo = key_of(f.b);
+        g.hi = f.b > 0 ? key_of(f.b - 1) - 1 : row.top;
         g.count = f.above_c;
         g.mass = f.above_m;
         members = f.cnt;
         // a crowded bucket is split by the key's bits until it fits, or is one key
-        while (members > (uint32_t)kRowsList && (!g.keyed || g.lo < g.hi)) {
+        while (members > (uint32_t)kRowsList && g.lo < g.hi) {
           members = split(g, want);
           fresh = false;
         }
@@ -714,13 +741,14 @@ struct Search {
         continue;
       }
       const uint32_t m = gather(g, phase);
+      const unsigned long long* sorted = sh.list[phase ^ 1];
       constexpr int kOwn = kRowsList / kRowsThreads;  // consecutive entries of a thread
       const int at = kOwn * tid;
       uint32_t key[kOwn];
       unsigned long long run[kOwn], mine = 0, tw;
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
-        key[i] = at + i < (int)m ? (uint32_t)(sh.sort[at + i] >> 32) : 0u;
+        key[i] = at + i < (int)m ? (uint32_t)(sorted[at + i] >> 32) : 0u;
         if (at + i < (int)m) mine += row.key_weight(key[i]);
         run[i] = mine;
       }
@@ -748,7 +776,6 @@ struct Search {
         kept_mass = e >= 0 ? sh.pickm : g.mass;
         if (!one_list && !(u * (double)kept_mass > (double)g.mass)) {
           // above this list: no key of it may be drawn
-          if (!g.keyed) to_keys(g);
           end_key = g.hi + 1;
           continue;
         }
@@ -762,7 +789,7 @@ struct Search {
         __syncthreads();
         e = sh.pick[0];
       }
-      return rank == 0 ? ~(uint32_t)sh.sort[max(0, e)] : 0xffffffffu;
+      return rank == 0 ? ~(uint32_t)sorted[max(0, e)] : 0xffffffffu;
     }
     return 0xffffffffu;  // not reached: phase 1 returns
   }
@@ -948,14 +975,14 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       } else if (min_p > 0.0) {
         // smallest key with w >= min_p (w grows with the key): a search with one
         // key per lane, at most seven rounds
-        const double bar = log(min_p);
-        const auto log_weight = [&](float v) { return ((double)v - (double)row.fmax) / (double)tt; };
+        const double bar = log(min_p) * (double)tt;
         uint32_t lo = kKeyNone, hi = row.top;  // w(lo) < min_p <= w(hi)
+        if (tt == INFINITY) hi = lo + 1;       // every weight is 1
         while (hi - lo > 1) {
           const uint32_t step = (hi - lo - 1) / 32 + 1;
           const uint32_t probe = min(lo + step * (lane + 1), hi);
           const uint32_t yes = __ballot_sync(
-              0xffffffffu, probe == hi || log_weight(rows_value(probe)) >= bar);
+              0xffffffffu, probe == hi || (double)rows_value(probe) - (double)row.fmax >= bar);
           const uint32_t at = __ffs(yes) - 1;
           hi = min(lo + step * (at + 1), hi);
           lo = lo + step * at;

@@ -14,7 +14,7 @@ converted.
 """
 from __future__ import annotations
 
-import contextlib
+import functools
 import math
 from typing import NamedTuple
 
@@ -52,9 +52,16 @@ class PageTrim(NamedTuple):
     info: object
 
 
+@functools.cache
 def _torch():
     import torch
     return torch
+
+
+@functools.cache
+def _call(name):
+    """The library's function of that name."""
+    return getattr(lib(), name)
 
 
 def _arg(msg: str) -> MinqError:
@@ -65,12 +72,12 @@ def _shape(msg: str) -> MinqError:
     return MinqError(_lib.ERR_SHAPE, msg)
 
 
-def _take(name, t, dtype, device, shape=None, contiguous=True):
-    """Check a tensor argument; returns its address."""
+def _take(name, t, dtype, dev, shape=None, contiguous=True):
+    """Check a tensor argument on CUDA device `dev`; returns its address."""
     if t.dtype is not dtype:
         raise _arg(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise _arg(f"{name} is on {t.device}, expected {device}")
+    if t.get_device() != dev:
+        raise _arg(f"{name} is on {t.device}, expected cuda:{dev}")
     if shape is not None and t.shape != shape:
         raise _shape(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
     if contiguous and not t.is_contiguous():
@@ -78,29 +85,35 @@ def _take(name, t, dtype, device, shape=None, contiguous=True):
     return t.data_ptr()
 
 
-def _cuda(name, t):
+def _cuda(name, t) -> int:
+    """Index of the CUDA device that a tensor is on."""
     if not getattr(t, "is_cuda", False):
         raise MinqError(_lib.ERR_CUDA, f"{name} must be a CUDA tensor (there is no CPU path)")
-    return t.device
+    return t.get_device()
 
 
-def _on(device):
-    """The tensors' device made current (for the launch and its stream)."""
-    torch = _torch()
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+@functools.cache
+def _on(dev: int):
+    return _torch().device("cuda", dev)
 
 
-def _stream(device) -> int:
-    return _torch().cuda.current_stream(device).cuda_stream
+def _run(dev: int, name: str, *args) -> None:
+    """Call the library on the current stream of device `dev`, with that device
+    current."""
+    cuda = _torch()._C
+    stream = cuda._cuda_getCurrentRawStream(dev)
+    if cuda._cuda_getDevice() == dev:
+        check(_call(name)(*args, stream))
+    else:
+        with _torch().cuda.device(dev):
+            check(_call(name)(*args, stream))
 
 
-def _table(table, device, n_req):
+def _table(table, dev, n_req):
     torch = _torch()
     if table.dim() != 2 or table.shape[0] != n_req:
         raise _shape(f"table must have shape [{n_req}, width], got {list(table.shape)}")
-    return _take("table", table, torch.int32, device)
+    return _take("table", table, torch.int32, dev)
 
 
 def pages_extend(lens, new_tokens, table, free_pages, n_free, page_size: int, max_tokens: int,
@@ -124,9 +137,9 @@ def pages_extend(lens, new_tokens, table, free_pages, n_free, page_size: int, ma
     i32 = torch.int32
     if out is None:
         # one allocation for the small outputs
-        buf = torch.empty(2 * n + 4 + max_tokens, dtype=i32, device=dev)
-        lo, nf, qs, info, pos = buf.split([n, 1, n + 1, 2, max_tokens])
-        out = PageStep(lo, nf, qs, torch.empty(max_tokens, dtype=torch.int64, device=dev), pos,
+        buf = torch.empty(2 * n + 4 + max_tokens, dtype=i32, device=_on(dev))
+        lo, nf, qs, info, pos = buf.split_with_sizes([n, 1, n + 1, 2, max_tokens])
+        out = PageStep(lo, nf, qs, torch.empty(max_tokens, dtype=torch.int64, device=_on(dev)), pos,
                        info)
     o = [_take("out.lens", out.lens, i32, dev, (n,)),
          _take("out.n_free", out.n_free, i32, dev, (1,)),
@@ -134,9 +147,8 @@ def pages_extend(lens, new_tokens, table, free_pages, n_free, page_size: int, ma
          _take("out.slots", out.slots, torch.int64, dev, (max_tokens,)),
          _take("out.positions", out.positions, i32, dev, (max_tokens,)),
          _take("out.info", out.info, i32, dev, (2,))]
-    with _on(dev):
-        check(lib().minq_pages_extend(a[0], a[1], n, page_size, tp, table.shape[1], fp,
-                                      free_pages.numel(), np_, max_tokens, *o, _stream(dev)))
+    _run(dev, "minq_pages_extend", a[0], a[1], n, page_size, tp, table.shape[1], fp,
+         free_pages.numel(), np_, max_tokens, *o)
     return out
 
 
@@ -152,13 +164,12 @@ def pages_trim(lens, keep, table, free_pages, n_free, page_size: int,
     fp = _take("free_pages", free_pages, i32, dev, (free_pages.numel(),))
     np_ = _take("n_free", n_free, i32, dev, (1,))
     if out is None:
-        out = PageTrim(*torch.empty(n + 3, dtype=i32, device=dev).split([n, 1, 2]))
+        out = PageTrim(*torch.empty(n + 3, dtype=i32, device=_on(dev)).split([n, 1, 2]))
     o = [_take("out.lens", out.lens, i32, dev, (n,)),
          _take("out.n_free", out.n_free, i32, dev, (1,)),
          _take("out.info", out.info, i32, dev, (2,))]
-    with _on(dev):
-        check(lib().minq_pages_trim(a[0], a[1], n, page_size, tp, table.shape[1], fp,
-                                    free_pages.numel(), np_, *o, _stream(dev)))
+    _run(dev, "minq_pages_trim", a[0], a[1], n, page_size, tp, table.shape[1], fp,
+         free_pages.numel(), np_, *o)
     return out
 
 
@@ -208,8 +219,7 @@ def kv4_write(k, v, slots, k_pages, v_pages) -> None:
     if v.shape[0] != T:
         raise _shape("k and v must hold the same tokens")
     s = _take("slots", slots, torch.int64, dev, (T,))
-    with _on(dev):
-        check(lib().minq_kv4_write(a, b, sa, sb, s, T, nkv, hd, kp, vp, n, page, _stream(dev)))
+    _run(dev, "minq_kv4_write", a, b, sa, sb, s, T, nkv, hd, kp, vp, n, page)
 
 
 def kv4_read(slots, k_pages, v_pages, out=None):
@@ -220,15 +230,20 @@ def kv4_read(slots, k_pages, v_pages, out=None):
     T = slots.numel()
     s = _take("slots", slots, torch.int64, dev, (T,))
     if out is None:
-        out = tuple(torch.empty(2, T, nkv, hd, dtype=torch.float32, device=dev).unbind(0))
+        out = tuple(torch.empty(2, T, nkv, hd, dtype=torch.float32, device=_on(dev)).unbind(0))
     k, v = out
     a, sa = _rows("out[0]", k, nkv, hd, dev)
     b, sb = _rows("out[1]", v, nkv, hd, dev)
     if k.shape[0] != T or v.shape[0] != T:
         raise _shape(f"out must hold {T} tokens")
-    with _on(dev):
-        check(lib().minq_kv4_read(kp, vp, n, page, s, T, nkv, hd, a, b, sa, sb, _stream(dev)))
+    _run(dev, "minq_kv4_read", kp, vp, n, page, s, T, nkv, hd, a, b, sa, sb)
     return k, v
+
+
+@functools.lru_cache(1024)
+def _workspace(dev, n_req, n_tokens, n_heads, n_kv, hd) -> int:
+    with _torch().cuda.device(dev):
+        return lib().minq_kv4_attend_workspace_bytes(n_req, n_tokens, n_heads, n_kv, hd)
 
 
 def kv4_attend(q, q_start, lens, table, k_pages, v_pages, scale: float | None = None, out=None,
@@ -249,18 +264,16 @@ def kv4_attend(q, q_start, lens, table, k_pages, v_pages, scale: float | None = 
     sp = _take("q_start", q_start, torch.int32, dev, (R + 1,))
     tp = _table(table, dev, R)
     if out is None:
-        out = torch.empty(T, nh, hd, dtype=torch.float32, device=dev)
+        out = torch.empty(T, nh, hd, dtype=torch.float32, device=_on(dev))
     op, os_ = _rows("out", out, nh, hd, dev)
     if out.shape[0] != T:
         raise _shape(f"out must hold {T} tokens")
-    with _on(dev):
-        need = lib().minq_kv4_attend_workspace_bytes(R, T, nh, nkv, hd)
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        wp = _take("workspace", workspace, torch.uint8, dev)
-        check(lib().minq_kv4_attend(qp, qs, sp, T, lp, R, tp, table.shape[1], kp, vp, n, page, nh,
-                                    nkv, hd, 1.0 / math.sqrt(hd) if scale is None else scale, op,
-                                    os_, wp, workspace.numel(), _stream(dev)))
+    need = _workspace(dev, R, T, nh, nkv, hd)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=_on(dev))
+    wp = _take("workspace", workspace, torch.uint8, dev)
+    _run(dev, "minq_kv4_attend", qp, qs, sp, T, lp, R, tp, table.shape[1], kp, vp, n, page, nh, nkv,
+         hd, 1.0 / math.sqrt(hd) if scale is None else scale, op, os_, wp, workspace.numel())
     return out
 
 
@@ -278,15 +291,12 @@ def sample_rows(logits, uniforms, temperature=None, top_k=None, top_p=None, min_
     if logits.stride(1) != 1 and n > 1:
         raise _arg("logits: a row must be contiguous")
     if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=dev)
+        out = torch.empty(rows, dtype=torch.int32, device=_on(dev))
     one = (rows,)
-    with _on(dev):
-        check(lib().minq_sample_rows(
-            lp, logits.stride(0) if rows > 1 else n, rows, n,
-            None if temperature is None else _take("temperature", temperature, f32, dev, one),
-            None if top_k is None else _take("top_k", top_k, torch.int32, dev, one),
-            None if top_p is None else _take("top_p", top_p, f32, dev, one),
-            None if min_p is None else _take("min_p", min_p, f32, dev, one),
-            _take("uniforms", uniforms, f32, dev, one), _take("out", out, torch.int32, dev, one),
-            _stream(dev)))
+    _run(dev, "minq_sample_rows", lp, logits.stride(0) if rows > 1 else n, rows, n,
+         None if temperature is None else _take("temperature", temperature, f32, dev, one),
+         None if top_k is None else _take("top_k", top_k, torch.int32, dev, one),
+         None if top_p is None else _take("top_p", top_p, f32, dev, one),
+         None if min_p is None else _take("min_p", min_p, f32, dev, one),
+         _take("uniforms", uniforms, f32, dev, one), _take("out", out, torch.int32, dev, one))
     return out
