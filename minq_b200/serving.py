@@ -136,17 +136,20 @@ def pages_extend(lens, new_tokens, table, free_pages, n_free, page_size: int, ma
         raise _shape("max_tokens must not be negative")
     i32 = torch.int32
     if out is None:
-        # one allocation for the small outputs
+        # one allocation for the 32-bit outputs
         buf = torch.empty(2 * n + 4 + max_tokens, dtype=i32, device=_on(dev))
+        slots = torch.empty(max_tokens, dtype=torch.int64, device=_on(dev))
         lo, nf, qs, info, pos = buf.split_with_sizes([n, 1, n + 1, 2, max_tokens])
-        out = PageStep(lo, nf, qs, torch.empty(max_tokens, dtype=torch.int64, device=_on(dev)), pos,
-                       info)
-    o = [_take("out.lens", out.lens, i32, dev, (n,)),
-         _take("out.n_free", out.n_free, i32, dev, (1,)),
-         _take("out.q_start", out.q_start, i32, dev, (n + 1,)),
-         _take("out.slots", out.slots, torch.int64, dev, (max_tokens,)),
-         _take("out.positions", out.positions, i32, dev, (max_tokens,)),
-         _take("out.info", out.info, i32, dev, (2,))]
+        out = PageStep(lo, nf, qs, slots, pos, info)
+        b = buf.data_ptr()
+        o = (b, b + 4 * n, b + 4 * n + 4, slots.data_ptr(), b + 8 * n + 16, b + 8 * n + 8)
+    else:
+        o = (_take("out.lens", out.lens, i32, dev, (n,)),
+             _take("out.n_free", out.n_free, i32, dev, (1,)),
+             _take("out.q_start", out.q_start, i32, dev, (n + 1,)),
+             _take("out.slots", out.slots, torch.int64, dev, (max_tokens,)),
+             _take("out.positions", out.positions, i32, dev, (max_tokens,)),
+             _take("out.info", out.info, i32, dev, (2,)))
     _run(dev, "minq_pages_extend", a[0], a[1], n, page_size, tp, table.shape[1], fp,
          free_pages.numel(), np_, max_tokens, *o)
     return out
@@ -164,10 +167,14 @@ def pages_trim(lens, keep, table, free_pages, n_free, page_size: int,
     fp = _take("free_pages", free_pages, i32, dev, (free_pages.numel(),))
     np_ = _take("n_free", n_free, i32, dev, (1,))
     if out is None:
-        out = PageTrim(*torch.empty(n + 3, dtype=i32, device=_on(dev)).split([n, 1, 2]))
-    o = [_take("out.lens", out.lens, i32, dev, (n,)),
-         _take("out.n_free", out.n_free, i32, dev, (1,)),
-         _take("out.info", out.info, i32, dev, (2,))]
+        buf = torch.empty(n + 3, dtype=i32, device=_on(dev))
+        out = PageTrim(*buf.split_with_sizes([n, 1, 2]))
+        b = buf.data_ptr()
+        o = (b, b + 4 * n, b + 4 * n + 4)
+    else:
+        o = (_take("out.lens", out.lens, i32, dev, (n,)),
+             _take("out.n_free", out.n_free, i32, dev, (1,)),
+             _take("out.info", out.info, i32, dev, (2,)))
     _run(dev, "minq_pages_trim", a[0], a[1], n, page_size, tp, table.shape[1], fp,
          free_pages.numel(), np_, *o)
     return out
@@ -230,14 +237,15 @@ def kv4_read(slots, k_pages, v_pages, out=None):
     T = slots.numel()
     s = _take("slots", slots, torch.int64, dev, (T,))
     if out is None:
-        out = tuple(torch.empty(2, T, nkv, hd, dtype=torch.float32, device=_on(dev)).unbind(0))
-    k, v = out
-    a, sa = _rows("out[0]", k, nkv, hd, dev)
-    b, sb = _rows("out[1]", v, nkv, hd, dev)
-    if k.shape[0] != T or v.shape[0] != T:
-        raise _shape(f"out must hold {T} tokens")
+        out = torch.empty(2, T, nkv, hd, dtype=torch.float32, device=_on(dev)).unbind(0)
+        a, b, sa, sb = out[0].data_ptr(), out[1].data_ptr(), nkv * hd, nkv * hd
+    else:
+        a, sa = _rows("out[0]", out[0], nkv, hd, dev)
+        b, sb = _rows("out[1]", out[1], nkv, hd, dev)
+        if out[0].shape[0] != T or out[1].shape[0] != T:
+            raise _shape(f"out must hold {T} tokens")
     _run(dev, "minq_kv4_read", kp, vp, n, page, s, T, nkv, hd, a, b, sa, sb)
-    return k, v
+    return out
 
 
 @functools.lru_cache(1024)
@@ -265,9 +273,11 @@ def kv4_attend(q, q_start, lens, table, k_pages, v_pages, scale: float | None = 
     tp = _table(table, dev, R)
     if out is None:
         out = torch.empty(T, nh, hd, dtype=torch.float32, device=_on(dev))
-    op, os_ = _rows("out", out, nh, hd, dev)
-    if out.shape[0] != T:
-        raise _shape(f"out must hold {T} tokens")
+        op, os_ = out.data_ptr(), nh * hd
+    else:
+        op, os_ = _rows("out", out, nh, hd, dev)
+        if out.shape[0] != T:
+            raise _shape(f"out must hold {T} tokens")
     need = _workspace(dev, R, T, nh, nkv, hd)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=_on(dev))
