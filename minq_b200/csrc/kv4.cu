@@ -14,6 +14,10 @@
 // each: two 16-byte loads, a maximum over the four lanes by two shuffles, and
 // one 4-byte word of codes per lane, the scale by the first; a warp covers
 // 256 consecutive values, so every global access of it is one contiguous run.
+// A value costs seven instructions (with roundf and an integer conversion each
+// it is twenty, and the write then waits for the arithmetic): the rounding half
+// away from zero is two additions rounded towards zero, and four codes are
+// added up in one float before a single conversion.
 #include <string>
 
 #include "common.cuh"
@@ -30,7 +34,9 @@ struct Kv4RowsParams {
   float* v_out;
   size_t k_stride, v_stride;  // floats between tokens
   const long long* slots;
-  size_t n_tokens;
+  uint32_t n_units;           // units of eight values on one side (below 2^31)
+  uint32_t token_m, row_m;    // u / (units per token), u / (units per row) as a product
+  int token_s, row_s;
   int n_kv, hd, page_shift;
   long long n_slots;
   uint8_t* k_pages;
@@ -51,47 +57,80 @@ __device__ __forceinline__ void load8(const float* x, float* v) {
   }
 }
 
-// One unit = eight values of one token, kv head and side (K or V): unit u =
-// ((token * 2 + side) * n_kv + head) * (hd / 8) + eighth.
+// One unit = eight values of one token and kv head: unit u = (token * n_kv +
+// head) * (hd / 8) + eighth; blockIdx.y is the side (K or V).
 struct Kv4Unit {
-  size_t token;
-  int side, head, e;
+  uint32_t token;
+  int head, e;
   uint8_t* block;  // the block's bytes, or null: a slot outside the pool
 };
 
-__device__ __forceinline__ Kv4Unit kv4_unit(const Kv4RowsParams& p, size_t u) {
+__device__ __forceinline__ Kv4Unit kv4_unit(const Kv4RowsParams& p, uint32_t u) {
   Kv4Unit c;
-  const int per_row = p.hd / 8;
-  const size_t row = u / per_row;
-  c.e = (int)(u - row * per_row);
-  const size_t ts = row / p.n_kv;
-  c.head = (int)(row - ts * p.n_kv);
-  c.token = ts >> 1;
-  c.side = (int)(ts & 1);
+  const uint32_t per_row = (uint32_t)p.hd / 8;
+  c.token = __umulhi(u, p.token_m) >> p.token_s;
+  const uint32_t in = u - c.token * p.n_kv * per_row;
+  c.head = (int)(__umulhi(in, p.row_m) >> p.row_s);
+  c.e = (int)(in - c.head * per_row);
   const long long slot = p.slots[c.token];
   c.block = nullptr;
   if (slot >= 0 && slot < p.n_slots) {
     const size_t page = (size_t)(slot >> p.page_shift);
     const size_t off = (size_t)(slot & ((1ll << p.page_shift) - 1));
     const size_t rrow = ((page * p.n_kv + c.head) << p.page_shift) + off;
-    c.block = (c.side ? p.v_pages : p.k_pages) + (rrow * (p.hd / kBlock) + c.e / 4) * kQ4Bytes;
+    c.block = (blockIdx.y ? p.v_pages : p.k_pages) +
+              (rrow * (p.hd / kBlock) + c.e / 4) * kQ4Bytes;
   }
   return c;
+}
+
+// Codes of eight values times 1 / d, in quant.cu's steps.
+__device__ __noinline__ uint32_t kv4_codes_slow(const float* v, float id) {
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = roundf(__fmul_rn(v[i], id));
+    const int q = isnan(y) ? 0 : (int)fminf(fmaxf(y, -8.0f), 7.0f);
+    word |= (uint32_t)(q + 8) << (4 * i);
+  }
+  return word;
+}
+__device__ __forceinline__ uint32_t kv4_codes(const float* v, float id) {
+  float sum[2] = {0.0f, 0.0f};  // codes less 8, in base 16
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = __fmul_rn(v[i], id);
+    // floor(|y| + 1/2): the sum is exact, but for 1/2 - 2^-25, which rounds to 1
+    // unless towards zero; 2^23 then leaves the integer
+    const float m = __fadd_rz(__fadd_rz(fabsf(y), 0.5f), 8388608.0f) - 8388608.0f;
+    float q = copysignf(m, y);
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(q) : "f"(7.0f));
+    sum[i >> 2] = fmaf(q, (float)(1 << (4 * (i & 3))), sum[i >> 2]);
+  }
+  // NaN anywhere, or an infinite product (a denormal scale's reciprocal)
+  if (!(fabsf(sum[0]) + fabsf(sum[1]) < 1048576.0f)) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v[i];
+    return kv4_codes_slow(x, id);
+  }
+  // + 0x8888: the codes' offset of 8
+  const uint32_t a = __float_as_uint(sum[0] + (8388608.0f + 34952.0f));
+  const uint32_t b = __float_as_uint(sum[1] + (8388608.0f + 34952.0f));
+  return __byte_perm(a, b, 0x5410);
 }
 
 template <bool VEC>
 __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4RowsParams p) {
   pdl_wait();
-  const size_t n_units = p.n_tokens * 2 * p.n_kv * (p.hd / 8);
   // whole warps take whole steps (n_units is a multiple of 4, not of 32)
-  const size_t step = (size_t)gridDim.x * blockDim.x;
-  for (size_t u0 = (size_t)blockIdx.x * blockDim.x + (threadIdx.x & ~31u); u0 < n_units;
-       u0 += step) {
-    const size_t u = u0 + (threadIdx.x & 31);
-    const bool on = u < n_units;
-    const Kv4Unit c = kv4_unit(p, on ? u : n_units - 1);
+  const uint32_t step = gridDim.x * 256;
+  for (uint32_t u0 = blockIdx.x * 256 + (threadIdx.x & ~31u); u0 < p.n_units; u0 += step) {
+    const uint32_t u = u0 + (threadIdx.x & 31);
+    const bool on = u < p.n_units;
+    const Kv4Unit c = kv4_unit(p, on ? u : p.n_units - 1);
     float v[8];
-    const float* x = (c.side ? p.v_in + c.token * p.v_stride : p.k_in + c.token * p.k_stride) +
+    const float* x = (blockIdx.y ? p.v_in + c.token * p.v_stride : p.k_in + c.token * p.k_stride) +
                      (size_t)c.head * p.hd + c.e * 8;
     load8<VEC>(x, v);
     float a = 0.0f;
@@ -100,16 +139,7 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4RowsParams p) {
     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
     const float d = a / 8.0f;
-    uint32_t word = 0;
-    if (d != 0.0f) {
-      const float id = 1.0f / d;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = roundf(__fmul_rn(v[i], id));
-        const int q = isnan(y) ? 0 : (int)fminf(fmaxf(y, -8.0f), 7.0f);
-        word |= (uint32_t)(q + 8) << (4 * i);
-      }
-    }
+    const uint32_t word = d != 0.0f ? kv4_codes(v, 1.0f / d) : 0u;
     if (on && c.block) {
       // blocks are 20 bytes: 4-byte aligned words
       *reinterpret_cast<uint32_t*>(c.block + 4 + 4 * (c.e & 3)) = word;
@@ -122,9 +152,7 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4RowsParams p) {
 template <bool VEC>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4RowsParams p) {
   pdl_wait();
-  const size_t n_units = p.n_tokens * 2 * p.n_kv * (p.hd / 8);
-  for (size_t u = (size_t)blockIdx.x * blockDim.x + threadIdx.x; u < n_units;
-       u += (size_t)gridDim.x * blockDim.x) {
+  for (uint32_t u = blockIdx.x * 256 + threadIdx.x; u < p.n_units; u += gridDim.x * 256) {
     const Kv4Unit c = kv4_unit(p, u);
     float v[8] = {};
     if (c.block) {
@@ -133,7 +161,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4RowsParams p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = __fmul_rn((float)((int)((w >> (4 * i)) & 15u) - 8), d);
     }
-    float* o = (c.side ? p.v_out + c.token * p.v_stride : p.k_out + c.token * p.k_stride) +
+    float* o = (blockIdx.y ? p.v_out + c.token * p.v_stride : p.k_out + c.token * p.k_stride) +
                (size_t)c.head * p.hd + c.e * 8;
     if (VEC) {
       reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -162,9 +190,32 @@ minq_status kv4_rows_check(const char* what, size_t n_tokens, size_t n_kv, size_
   return MINQ_OK;
 }
 
-unsigned kv4_grid(size_t units) {
-  const size_t g = (units + 255) / 256, cap = (size_t)sm_count() * 32;
-  return (unsigned)(g < cap ? g : cap);
+// u / d == umulhi(u, m) >> s for u < 2^31 and d >= 2.
+void divisor(uint32_t d, uint32_t* m, int* s) {
+  int bits = 1;
+  while ((1u << bits) < d) ++bits;
+  *m = (uint32_t)((1ull << (31 + bits)) / d + 1);
+  *s = bits - 1;
+}
+
+// Both sides of all tokens, in as many launches as keep the units below 2^31.
+template <class K>
+minq_status launch_rows(K kernel, Kv4RowsParams p, size_t n_tokens, cudaStream_t s) {
+  const uint32_t per_row = (uint32_t)p.hd / 8, per_token = per_row * (uint32_t)p.n_kv;
+  divisor(per_token, &p.token_m, &p.token_s);
+  divisor(per_row, &p.row_m, &p.row_s);
+  const size_t most = ((1u << 31) - 1024) / per_token, cap = (size_t)sm_count() * 16;
+  for (size_t t = 0; t < n_tokens; t += most) {
+    const size_t n = n_tokens - t < most ? n_tokens - t : most;
+    p.n_units = (uint32_t)(n * per_token);
+    const size_t g = (p.n_units + 255) / 256;
+    MINQ_CUDA_TRY(
+        launch_k(kernel, dim3((unsigned)(g < cap ? g : cap), 2), dim3(256), 0, s, p));
+    p.slots += n;
+    if (p.k_in) p.k_in += n * p.k_stride, p.v_in += n * p.v_stride;
+    if (p.k_out) p.k_out += n * p.k_stride, p.v_out += n * p.v_stride;
+  }
+  return MINQ_OK;
 }
 
 int page_shift_of(size_t P) {
@@ -201,18 +252,15 @@ minq_status minq_kv4_write(const float* k, const float* v, size_t k_stride, size
   p.k_stride = k_stride;
   p.v_stride = v_stride;
   p.slots = reinterpret_cast<const long long*>(slots);
-  p.n_tokens = n_tokens;
   p.n_kv = (int)n_kv;
   p.hd = (int)head_dim;
   p.page_shift = page_shift_of(page_size);
   p.n_slots = (long long)n_pages << p.page_shift;
   p.k_pages = static_cast<uint8_t*>(k_pages);
   p.v_pages = static_cast<uint8_t*>(v_pages);
-  const dim3 grid(kv4_grid(n_tokens * 2 * n_kv * (head_dim / 8)));
   const bool vec = al16(k) && al16(v) && (k_stride | v_stride) % 4 == 0;
-  MINQ_CUDA_TRY(launch_k(vec ? kv4_write_kernel<true> : kv4_write_kernel<false>, grid, dim3(256), 0,
-                         (cudaStream_t)stream, p));
-  return MINQ_OK;
+  return launch_rows(vec ? kv4_write_kernel<true> : kv4_write_kernel<false>, p, n_tokens,
+                     (cudaStream_t)stream);
 }
 
 minq_status minq_kv4_read(const void* k_pages, const void* v_pages, size_t n_pages,
@@ -233,18 +281,15 @@ minq_status minq_kv4_read(const void* k_pages, const void* v_pages, size_t n_pag
   p.k_stride = k_stride;
   p.v_stride = v_stride;
   p.slots = reinterpret_cast<const long long*>(slots);
-  p.n_tokens = n_tokens;
   p.n_kv = (int)n_kv;
   p.hd = (int)head_dim;
   p.page_shift = page_shift_of(page_size);
   p.n_slots = (long long)n_pages << p.page_shift;
   p.k_pages = const_cast<uint8_t*>(static_cast<const uint8_t*>(k_pages));
   p.v_pages = const_cast<uint8_t*>(static_cast<const uint8_t*>(v_pages));
-  const dim3 grid(kv4_grid(n_tokens * 2 * n_kv * (head_dim / 8)));
   const bool vec = al16(k) && al16(v) && (k_stride | v_stride) % 4 == 0;
-  MINQ_CUDA_TRY(launch_k(vec ? kv4_read_kernel<true> : kv4_read_kernel<false>, grid, dim3(256), 0,
-                         (cudaStream_t)stream, p));
-  return MINQ_OK;
+  return launch_rows(vec ? kv4_read_kernel<true> : kv4_read_kernel<false>, p, n_tokens,
+                     (cudaStream_t)stream);
 }
 
 }  // extern "C"
