@@ -84,7 +84,7 @@ struct Kv4AttnParams {
   // tensor-core kernel
   // columns of a tile (room for), heads per tile, head tiles per kv head, tokens per tile
   int cols, gsz, hgroups, tpt;
-  int n_cta;
+  int n_cta, join_ctas;  // CTAs of the first kernel, and those that a block of the second joins
   float* part_o;   // [n_cta * warps][2][cols][hd] unnormalised partial outputs
   float* part_ml;  // [n_cta * warps][2][cols][2] their maxima and sums
   KvRec* rec;      // [n_cta * warps]
@@ -1047,40 +1047,59 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
   }
 }
 
-// Joins the pieces of the items that start in the warps of CTA blockIdx.x and
-// go on behind them, one block per column. An item of few pieces is summed by
-// one warp (four items at once), one of many by the eight warps in turn,
-// always in a fixed order.
+// Joins the pieces of the items that start in the warps of join_ctas CTAs and
+// go on behind them, always in a fixed order. An item of few pieces is summed
+// by a warp per column, the (item, column) pairs dealt out to the eight warps;
+// one of many by all eight warps, column by column. A long step of few items
+// has its columns spread over gridDim.y blocks.
 constexpr int kKvJoinWarps = 8;
 constexpr int kKvJoinAlone = 16;  // pieces
+constexpr int kKvJoinCtas = 4;    // most per block
+constexpr int kKvJoinRecs = kKvJoinCtas * kKvWarps;
 template <int HD>
 __global__ void __launch_bounds__(kKvJoinWarps * 32)
     kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
   constexpr int PER = HD / 32;  // values per lane
   __shared__ float s_o[kKvJoinWarps][HD];
   __shared__ float s_l[kKvJoinWarps];
-  __shared__ KvRec s_rec[kKvWarps];
+  __shared__ KvRec s_rec[kKvJoinRecs];
+  __shared__ int2 s_tok[kKvJoinRecs];  // the request's first token, its tokens
+  __shared__ int s_n;
   pdl_wait();
   pdl_launch_dependents();
-  const int col = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x < kKvWarps) s_rec[threadIdx.x] = p.rec[blockIdx.x * kKvWarps + threadIdx.x];
+  if (warp == 0) {  // the items that there are, in order
+    const int per = p.join_ctas * kKvWarps, c = blockIdx.x * per + lane;
+    KvRec rec{};
+    if (lane < per && c < p.n_cta * kKvWarps) rec = p.rec[c];
+    const uint32_t some = __ballot_sync(0xffffffffu, rec.parts > 0);
+    const int at = __popc(some & ((1u << lane) - 1));
+    if (rec.parts > 0) {
+      s_rec[at] = rec;
+      const int a = p.q_start[rec.r];
+      s_tok[at] = make_int2(a, p.q_start[rec.r + 1] - a);
+    }
+    if (lane == 0) s_n = __popc(some);
+  }
   __syncthreads();
-  const int ct = col / p.gsz, ch = col - ct * p.gsz;
-  // the item's row of `out` for this column, or null
-  auto row = [&](const KvRec& rec) -> float* {
-    const int a = p.q_start[rec.r], n = p.q_start[rec.r + 1] - a;
+  const int n_rec = s_n;
+  const int G = p.nh / p.nkv, used = p.tpt * p.gsz;  // columns that hold anything
+  // the item's row of `out` for a column, or null
+  auto row = [&](int k, int col) -> float* {
+    const KvRec& rec = s_rec[k];
+    const int ct = col / p.gsz, ch = col - ct * p.gsz;
     const int kvh = rec.h / p.hgroups, head = (rec.h - kvh * p.hgroups) * p.gsz + ch;
     const int tok = rec.j * p.tpt + ct;
-    if (tok >= n || ct >= p.tpt || ch >= p.gsz || head >= p.nh / p.nkv) return nullptr;
-    return p.out + (size_t)(a + tok) * p.out_stride + (size_t)(kvh * (p.nh / p.nkv) + head) * HD;
+    if (tok >= s_tok[k].y || head >= G) return nullptr;
+    return p.out + (size_t)(s_tok[k].x + tok) * p.out_stride + (size_t)(kvh * G + head) * HD;
   };
   // pieces w, w + step, .. of an item: their sum relative to the maximum M of all
-  auto sum = [&](const KvRec& rec, int w, int step, float& L, float* acc) {
+  auto sum = [&](const KvRec& rec, int col, int w, int step, float& L, float* acc) {
     auto at = [&](int i) {
-      const int piece = i < rec.n_first             ? rec.a + i
-                        : i < rec.n_first + rec.n_mid ? (rec.a / kKvWarps + 1 + i - rec.n_first) * kKvWarps
-                                                      : rec.z0 + (i - rec.n_first - rec.n_mid);
+      const int piece = i < rec.n_first ? rec.a + i
+                        : i < rec.n_first + rec.n_mid
+                            ? (rec.a / kKvWarps + 1 + i - rec.n_first) * kKvWarps
+                            : rec.z0 + (i - rec.n_first - rec.n_mid);
       return ((size_t)piece * 2 + (i == 0 ? 1 : 0)) * p.cols + col;
     };
     float M = -3.0e38f;
@@ -1089,47 +1108,53 @@ __global__ void __launch_bounds__(kKvJoinWarps * 32)
     L = 0.0f;
 #pragma unroll
     for (int d = 0; d < PER; ++d) acc[d] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = w; i < rec.parts; i += step) {
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(i) * 2);
       const float f = ex2(ml.x - M);
       L += ml.y * f;
       const float* o = p.part_o + at(i) * HD + PER * lane;
+      float v[PER];
 #pragma unroll
-      for (int d = 0; d < PER; ++d) acc[d] += o[d] * f;
+      for (int d = 0; d < PER; d += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(o + d);
+        v[d] = x.x;
+        v[d + 1] = x.y;
+      }
+#pragma unroll
+      for (int d = 0; d < PER; ++d) acc[d] += v[d] * f;
     }
   };
   float L, acc[PER];
-  if (warp < kKvWarps) {
-    const KvRec rec = s_rec[warp];
-    if (rec.parts && rec.parts <= kKvJoinAlone) {
-      float* out = row(rec);
-      if (out) {
-        sum(rec, 0, 1, L, acc);
-#pragma unroll
-        for (int d = 0; d < PER; ++d) out[PER * lane + d] = L != 0.0f ? acc[d] / L : 0.0f;
-      }
-    }
-  }
-  for (int k = 0; k < kKvWarps; ++k) {
-    const KvRec rec = s_rec[k];
-    if (rec.parts <= kKvJoinAlone) continue;
-    float* out = row(rec);
+  for (int i = warp * gridDim.y + blockIdx.y; i < n_rec * used; i += kKvJoinWarps * gridDim.y) {
+    const int k = i / used, col = i - k * used;
+    if (s_rec[k].parts > kKvJoinAlone) continue;
+    float* out = row(k, col);
     if (!out) continue;
-    sum(rec, warp, kKvJoinWarps, L, acc);
-    __syncthreads();  // the sums of the item before have been read
+    sum(s_rec[k], col, 0, 1, L, acc);
 #pragma unroll
-    for (int d = 0; d < PER; ++d) s_o[warp][PER * lane + d] = acc[d];
-    if (lane == 0) s_l[warp] = L;
-    __syncthreads();
-    for (int d = threadIdx.x; d < HD; d += kKvJoinWarps * 32) {
-      float o = 0.0f, l = 0.0f;
+    for (int d = 0; d < PER; ++d) out[PER * lane + d] = L != 0.0f ? acc[d] / L : 0.0f;
+  }
+  for (int k = 0; k < n_rec; ++k) {
+    if (s_rec[k].parts <= kKvJoinAlone) continue;
+    for (int col = blockIdx.y; col < used; col += gridDim.y) {
+      float* out = row(k, col);
+      if (!out) continue;
+      sum(s_rec[k], col, warp, kKvJoinWarps, L, acc);
+      __syncthreads();  // the sums before have been read
 #pragma unroll
-      for (int x = 0; x < kKvJoinWarps; ++x) {
-        o += s_o[x][d];
-        l += s_l[x];
+      for (int d = 0; d < PER; ++d) s_o[warp][PER * lane + d] = acc[d];
+      if (lane == 0) s_l[warp] = L;
+      __syncthreads();
+      for (int d = threadIdx.x; d < HD; d += kKvJoinWarps * 32) {
+        float o = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kKvJoinWarps; ++x) {
+          o += s_o[x][d];
+          l += s_l[x];
+        }
+        out[d] = l != 0.0f ? o / l : 0.0f;
       }
-      out[d] = l != 0.0f ? o / l : 0.0f;
     }
   }
 }
@@ -1158,8 +1183,17 @@ minq_status launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
   MINQ_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kv4_attend_kernel<HD, NT, SPLIT>), GM::SMEM));
   MINQ_CUDA_TRY(launch_k(kv4_attend_kernel<HD, NT, SPLIT>, dim3(p.n_cta), dim3(kKvWarps * 32), GM::SMEM, s,
                          p));
-  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3(p.n_cta, SPLIT ? 4 : GM::COLS),
-                         dim3(kKvJoinWarps * 32), 0, s, p));
+  // With few items (of one token each) every one has many pieces: their columns
+  // are spread over blocks, and few blocks look for them. With many there are
+  // some in every CTA. Measured (join alone, us): 2 x 131071 positions of 2 kv
+  // heads 18 this way and 20 the other, 64 x 8192 of 8 kv heads 18 and 9.
+  const bool few = (size_t)p.n_req * p.nkv * p.hgroups * 4 < (size_t)p.n_cta;
+  Kv4AttnParams j = p;
+  j.join_ctas = few ? kKvJoinCtas : 1;
+  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>,
+                         dim3((p.n_cta + j.join_ctas - 1) / j.join_ctas,
+                              few ? 8 : (p.tpt * p.gsz + 3) / 4),
+                         dim3(kKvJoinWarps * 32), 0, s, j));
   return MINQ_OK;
 }
 

@@ -271,7 +271,7 @@ minq_status launch_pages(const PagesParams& p, cudaStream_t s) {
   attr[1].val.clusterDim.x = ctas;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
   count_launch();
   MINQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, pages_kernel<EXTEND>, p));
   return MINQ_OK;
