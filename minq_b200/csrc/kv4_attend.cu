@@ -46,49 +46,19 @@
 // the pieces of the others go to the workspace, one per warp, or one per CTA
 // where an item fills it, and a second small launch joins them in a fixed
 // order, so results repeat bit for bit.
-#include <cuda_fp16.h>
+#include <limits.h>
 #include <math.h>
 
 #include <string>
 
 #include "common.cuh"
 #include "kernels.h"
+#include "kv4_attend.cuh"
 #include "pipeline.cuh"
 
 namespace minq {
 
 namespace {
-
-// The item that starts in a warp's piece of the line and goes on behind it.
-struct KvRec {
-  int parts, r, h, j;  // number of pieces (0: no item), request, head tile, column tile
-  int a, n_first, n_mid, z0;  // first piece and pieces in its CTA, CTAs between, first in the last
-};
-
-struct Kv4AttnParams {
-  const float* q;  // token t, head h at q + t * q_stride + h * hd
-  size_t q_stride;
-  const int* q_start;
-  int n_tokens;
-  const int* lens;
-  int n_req;
-  const int* table;
-  size_t table_stride;
-  const uint8_t* k_pages;
-  const uint8_t* v_pages;
-  int n_pages, page_shift;
-  int nh, nkv, hd;
-  float scale;
-  float* out;
-  size_t out_stride;
-  // tensor-core kernel
-  // columns of a tile (room for), heads per tile, head tiles per kv head, tokens per tile
-  int cols, gsz, hgroups, tpt;
-  int n_cta, join_ctas;  // CTAs of the first kernel, and those that a block of the second joins
-  float* part_o;   // [n_cta * warps][2][cols][hd] unnormalised partial outputs
-  float* part_ml;  // [n_cta * warps][2][cols][2] their maxima and sums
-  KvRec* rec;      // [n_cta * warps]
-};
 
 // Request of token t, or -1 where t lies behind the last sequence (or the
 // starts are not a valid partition there).
@@ -184,8 +154,12 @@ __device__ int g_kv4_status;
 
 constexpr int kKvWarps = 4;
 constexpr int kKvTile = 32;     // positions per tile
-constexpr int kKvItem = 64;     // an item's start and end, in positions
+constexpr int kKvExtra = 64;    // an item's start and end, in positions
 constexpr int kKvMinPiece = 96;  // smallest piece of the line per warp
+
+// Requests of so many (token, head) rows go to the tcgen05 kernel.
+constexpr size_t kKvUmmaMin = 32;
+constexpr int kKvUmmaSpread = 16;  // blocks that share the columns of its join's pieces
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -208,32 +182,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-
-// (x, y) as two f16 pairs, high and low parts.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = h2_bits(__floats2half2_rn(x, y));
-  float a, b;  // hi - x, exact; the mixed-precision form needs no conversion
-  asm("{\n\t.reg .f16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\t"
-      "sub.rn.f32.f16 %1, h, %4;\n\t}"
-      : "=f"(a), "=f"(b)
-      : "r"(hi), "f"(x), "f"(y));
-  lo = h2_bits(__floats2half2_rn(-a, -b));
-}
-
-// (x & m) | o as one instruction.
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(m), "r"(o));
-  return d;
-}
-
 // The part of (x, y) that a lane holds: round(x), or with neg = -1.0 (f16)
 // round(x - round(x)).
 __device__ __forceinline__ uint32_t part2(float x, float y, uint32_t neg) {
@@ -244,18 +192,6 @@ __device__ __forceinline__ uint32_t part2(float x, float y, uint32_t neg) {
       : "=f"(a), "=f"(b)
       : "r"(hi), "f"(x), "f"(y), "r"(neg));
   return h2_bits(__floats2half2_rn(a, b));
-}
-
-// The codes in nibbles 0..3 of both halves of x as exact signed integers:
-// 0x6400 | c is 1024 + c in f16, and 0x6400 | 16 c is 1024 + 16 c.
-__device__ __forceinline__ void codes4(uint32_t x, uint32_t* y) {
-  const __half2 m8 = __float2half2_rn(-1032.0f), m72 = __float2half2_rn(-72.0f),
-                r16 = __float2half2_rn(0.0625f);
-  const uint32_t z = x >> 8;
-  y[0] = h2_bits(__hadd2(bits_h2(and_or(x, 0x000f000fu, 0x64006400u)), m8));
-  y[1] = h2_bits(__hfma2(bits_h2(and_or(x, 0x00f000f0u, 0x64006400u)), r16, m72));
-  y[2] = h2_bits(__hadd2(bits_h2(and_or(z, 0x000f000fu, 0x64006400u)), m8));
-  y[3] = h2_bits(__hfma2(bits_h2(and_or(z, 0x00f000f0u, 0x64006400u)), r16, m72));
 }
 
 // o[0..1] += c[0..1], one packed addition.
@@ -281,30 +217,6 @@ __device__ __forceinline__ void load_trans(uint32_t* d, const uint8_t* row) {
 template <int HD>
 __device__ __forceinline__ int kv_dim(int b, int g) {
   return b * 32 + 4 * (HD == 128 ? (g - 2 * b - 2) & 7 : g);
-}
-
-// The line of items. Request r: n tokens in J column tiles per head tile.
-struct KvReq {
-  int r, t0, n, len;  // request, first token, tokens, positions
-  long long base;     // weight of column tile j: base + (j + 1) * tpt
-  long long J;
-};
-__device__ __forceinline__ KvReq kv_req(const Kv4AttnParams& p, int r) {
-  KvReq q;
-  q.r = r;
-  const int a = p.q_start[r], b = p.q_start[r + 1];
-  const bool ok = a >= 0 && b <= p.n_tokens && a < b;  // a valid run of tokens
-  q.t0 = ok ? a : 0;
-  q.n = ok ? b - a : 0;
-  q.len = p.lens[r];
-  const int prior = q.len - q.n;
-  q.base = (prior > 0 ? prior : 0) + kKvItem;
-  q.J = (q.n + p.tpt - 1) / p.tpt;
-  return q;
-}
-// Weight of column tiles 0 .. j - 1.
-__device__ __forceinline__ long long kv_cum(const KvReq& q, int tpt, long long j) {
-  return j * q.base + (long long)tpt * (j * (j + 1) / 2);
 }
 
 template <int HD, int NT>
@@ -583,69 +495,6 @@ __device__ __forceinline__ void kv_tile(KvState<HD, NT, SPLIT>& st, const uint8_
   }
 }
 
-// One item: tokens [tok0, tok0 + ntok) of a request for the heads [h0, h0 +
-// nhead), at [start, start + w) on the line.
-struct KvItem {
-  KvReq rq;
-  int h;        // head tile
-  long long j;  // column tile
-  long long start, w;
-  int kvh, h0, nhead, tok0, ntok, prior, lim_max;
-  long long cap;
-  long long x0, x1;  // the part of it that this warp (or CTA) takes
-};
-__device__ __forceinline__ void kv_item_set(const Kv4AttnParams& p, KvItem& it) {
-  const int G = p.nh / p.nkv, hg = it.h % p.hgroups;
-  it.w = it.rq.base + (it.j + 1) * p.tpt;
-  it.kvh = it.h / p.hgroups;
-  it.h0 = it.kvh * G + hg * p.gsz;
-  it.nhead = min(p.gsz, G - hg * p.gsz);
-  it.tok0 = (int)(it.j * p.tpt);
-  it.ntok = min(p.tpt, it.rq.n - it.tok0);
-  it.prior = it.rq.len - it.rq.n;
-  // positions of the table row (tile ends stay inside 31 bits)
-  it.cap = min((long long)p.table_stride << p.page_shift, 0x7fffff00ll);
-  // positions that the last token sees
-  const long long lim = min((long long)it.prior + it.tok0 + it.ntok, it.cap);
-  it.lim_max = lim > 0 ? (int)lim : 0;
-}
-// The item at u, in the request r that starts at `start` on the line.
-__device__ __forceinline__ void kv_item_at(const Kv4AttnParams& p, KvItem& it, int r,
-                                           long long start, long long u) {
-  it.rq = kv_req(p, r);
-  const long long W = kv_cum(it.rq, p.tpt, it.rq.J), off = u - start;
-  it.h = (int)(off / W);
-  const long long x = off - it.h * W;
-  long long lo = 0, hi = it.rq.J;
-  while (hi - lo > 1) {
-    const long long mid = (lo + hi) >> 1;
-    if (kv_cum(it.rq, p.tpt, mid) <= x)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  it.j = lo;
-  it.start = start + it.h * W + kv_cum(it.rq, p.tpt, lo);
-  kv_item_set(p, it);
-}
-// The next item on the line; false behind the last one.
-__device__ __forceinline__ bool kv_item_next(const Kv4AttnParams& p, KvItem& it) {
-  it.start += it.w;
-  if (++it.j == it.rq.J) {
-    it.j = 0;
-    if (++it.h == p.nkv * p.hgroups) {
-      it.h = 0;
-      int r = it.rq.r;
-      do {
-        if (++r >= p.n_req) return false;
-        it.rq = kv_req(p, r);
-      } while (it.rq.J == 0);
-    }
-  }
-  kv_item_set(p, it);
-  return true;
-}
-
 // The pieces of an item that starts in piece a: the warps' in the first and the
 // last CTA that it touches, and one per CTA that it fills.
 __device__ __forceinline__ KvRec kv_parts(const KvItem& it, int a, long long per, long long total) {
@@ -681,7 +530,7 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
   constexpr int NB = GM::NB;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n_tiles = (it.lim_max + kKvTile - 1) / kKvTile;
-  auto tile_at = [](long long x) { return x > kKvItem ? (x - kKvItem + kKvTile - 1) / kKvTile : 0; };
+  auto tile_at = [](long long x) { return x > kKvExtra ? (x - kKvExtra + kKvTile - 1) / kKvTile : 0; };
   const long long xa = tile_at(it.x0), xb = it.x1 == it.w ? n_tiles : tile_at(it.x1);
   const int ta = (int)min(xa, (long long)n_tiles) + lead, tb = (int)min(xb, (long long)n_tiles);
   const int my = tb > ta ? (tb - ta + step - 1) / step : 0;
@@ -736,7 +585,7 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
       bulk_g2s(ring.buf + sidx * 2 * GM::SIDE + (lane >> 1) * GM::SIDE + half * GM::HALF,
                side + (size_t)id * page_bytes + row * GM::ROW, GM::HALF, bar);
     }
-    ++ring.fill;
+    if (ring.alive) ++ring.fill;
   };
   const int first = min(my, GM::STAGES);
   for (int i = 0; i < first; ++i) issue(i, ids);
@@ -806,7 +655,7 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
     if (ring.alive)
       ring.alive = mbar_wait_timed(&ring.bar[sidx], (ring.used / GM::STAGES) & 1, &g_kv4_status);
     ring.alive = __all_sync(0xffffffffu, ring.alive);
-    ++ring.used;
+    if (ring.alive) ++ring.used;
     const int ok = (int)(__ballot_sync(0xffffffffu, ids >= 0) >> (2 * (i & 15))) & 3;
     if (ring.alive && ok) {
       const int pos0 = tile_pos(i);
@@ -823,6 +672,10 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
       ids = ids_next;
       ids_next = load_ids(i + 17);
     }
+  }
+  if (!ring.alive) {  // a wait gave up: let the copies in flight end before the CTA does
+    for (; ring.used < ring.fill; ++ring.used)
+      mbar_wait_timed(&ring.bar[ring.used % GM::STAGES], (ring.used / GM::STAGES) & 1, &g_kv4_status);
   }
   // sums over the positions' lanes
 #pragma unroll
@@ -874,8 +727,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
   total = 0;
 #pragma unroll
   for (int w = 0; w < kKvWarps; ++w) total += s_red[w];
-  const int n_piece = p.n_cta * kKvWarps;
-  long long per = (total + n_piece - 1) / n_piece;
+  long long per = (total + p.n_piece - 1) / p.n_piece;
   if (per < kKvMinPiece) per = kKvMinPiece;
   const long long c0 = per * kKvWarps * blockIdx.x, c1 = min(c0 + per * kKvWarps, total);
   KvRec* rec = p.rec + blockIdx.x * kKvWarps;
@@ -920,7 +772,10 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
     if (before > c1) break;  // uniform
   }
   __syncthreads();
-  if (s_req[0] < 0) return;  // cannot happen: the items cover the line
+  if (s_req[0] < 0) {  // cannot happen: the items cover the line
+    if (tid < kKvWarps) rec[tid].parts = 0;
+    return;
+  }
 
   KvState<HD, NT, SPLIT> st;
   KvItem& it = s_item[warp];
@@ -1047,15 +902,13 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
   }
 }
 
-// Joins the pieces of the items that start in the warps of join_ctas CTAs and
-// go on behind them, always in a fixed order. An item of few pieces is summed
+// Joins the pieces of the items that start in join_pieces pieces and go on behind them, always in a fixed order. An item of few pieces is summed
 // by a warp per column, the (item, column) pairs dealt out to the eight warps;
 // one of many by all eight warps, column by column. A long step of few items
 // has its columns spread over gridDim.y blocks.
 constexpr int kKvJoinWarps = 8;
 constexpr int kKvJoinAlone = 16;  // pieces
-constexpr int kKvJoinCtas = 4;    // most per block
-constexpr int kKvJoinRecs = kKvJoinCtas * kKvWarps;
+constexpr int kKvJoinRecs = 16;   // most pieces that a block looks through
 template <int HD>
 __global__ void __launch_bounds__(kKvJoinWarps * 32)
     kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
@@ -1069,9 +922,9 @@ __global__ void __launch_bounds__(kKvJoinWarps * 32)
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp == 0) {  // the items that there are, in order
-    const int per = p.join_ctas * kKvWarps, c = blockIdx.x * per + lane;
+    const int c = blockIdx.x * p.join_pieces + lane;
     KvRec rec{};
-    if (lane < per && c < p.n_cta * kKvWarps) rec = p.rec[c];
+    if (lane < p.join_pieces && c < p.n_piece) rec = p.rec[c];
     const uint32_t some = __ballot_sync(0xffffffffu, rec.parts > 0);
     const int at = __popc(some & ((1u << lane) - 1));
     if (rec.parts > 0) {
@@ -1163,8 +1016,10 @@ __global__ void __launch_bounds__(kKvJoinWarps * 32)
 // rows kernel serves it.
 struct KvPlan {
   int nt, n_cta;
-  bool split;  // columns hold the two parts of q: up to 4 columns a tile
-  size_t ws;
+  bool split;    // columns hold the two parts of q: up to 4 columns a tile
+  int umma_lo;   // requests of so many tokens go to the tcgen05 kernel (0: none)
+  size_t ws, umma_ws;
+  size_t bytes() const { return ws + umma_ws; }
 };
 KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_t hd) {
   KvPlan k{};
@@ -1174,37 +1029,49 @@ KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_
   k.split = k.nt == 1 && G <= 4;
   k.n_cta = sm_count() * (k.nt == 1 ? 4 : 2);
   k.ws = (size_t)k.n_cta * kKvWarps * (2 * 8 * k.nt * (hd + 2) * 4 + sizeof(KvRec));
+  const size_t gsz = G < (size_t)kKvUmmaRows ? G : kKvUmmaRows;
+  if (n_tokens > n_req && n_tokens * gsz >= kKvUmmaMin) {
+    k.umma_lo = (int)((kKvUmmaMin + gsz - 1) / gsz);
+    k.umma_ws = kv4_umma_workspace(hd);
+  }
   return k;
+}
+
+// join_pieces: pieces that a block looks through; spread: blocks that share their columns.
+template <int HD>
+minq_status launch_kv4_join(Kv4AttnParams p, int join_pieces, int spread, cudaStream_t s) {
+  p.join_pieces = join_pieces;
+  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3((p.n_piece + join_pieces - 1) / join_pieces, spread),
+                         dim3(kKvJoinWarps * 32), 0, s, p));
+  return MINQ_OK;
 }
 
 template <int HD, int NT, bool SPLIT>
 minq_status launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
   using GM = KvGeom<HD, NT>;
   MINQ_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kv4_attend_kernel<HD, NT, SPLIT>), GM::SMEM));
-  MINQ_CUDA_TRY(launch_k(kv4_attend_kernel<HD, NT, SPLIT>, dim3(p.n_cta), dim3(kKvWarps * 32), GM::SMEM, s,
-                         p));
+  MINQ_CUDA_TRY(launch_k(kv4_attend_kernel<HD, NT, SPLIT>, dim3(p.n_piece / kKvWarps), dim3(kKvWarps * 32),
+                         GM::SMEM, s, p));
   // With few items (of one token each) every one has many pieces: their columns
   // are spread over blocks, and few blocks look for them. With many there are
   // some in every CTA. Measured (join alone, us): 2 x 131071 positions of 2 kv
   // heads 18 this way and 20 the other, 64 x 8192 of 8 kv heads 18 and 9.
-  const bool few = (size_t)p.n_req * p.nkv * p.hgroups * 4 < (size_t)p.n_cta;
-  Kv4AttnParams j = p;
-  j.join_ctas = few ? kKvJoinCtas : 1;
-  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>,
-                         dim3((p.n_cta + j.join_ctas - 1) / j.join_ctas,
-                              few ? 8 : (p.tpt * p.gsz + 3) / 4),
-                         dim3(kKvJoinWarps * 32), 0, s, j));
-  return MINQ_OK;
+  const bool few = (size_t)p.n_req * p.nkv * p.hgroups * 4 < (size_t)p.n_piece / kKvWarps;
+  return launch_kv4_join<HD>(p, few ? kKvJoinRecs : kKvWarps, few ? 8 : (p.tpt * p.gsz + 3) / 4, s);
 }
 
 }  // namespace
 
 minq_status take_kv4_status() {
   int v = 0;
+  int u = 0;
+  MINQ_TRY(take_kv4_umma_status(&u));
   MINQ_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_kv4_status, sizeof(int)));
-  if (v == 0) return MINQ_OK;
-  const int zero = 0;
-  MINQ_CUDA_TRY(cudaMemcpyToSymbol(g_kv4_status, &zero, sizeof(int)));
+  if (v != 0) {
+    const int zero = 0;
+    MINQ_CUDA_TRY(cudaMemcpyToSymbol(g_kv4_status, &zero, sizeof(int)));
+  }
+  if ((u | v) == 0) return MINQ_OK;
   return fail(MINQ_ERR_TIMEOUT, "a bounded wait of kv4_attend timed out");
 }
 
@@ -1216,7 +1083,7 @@ extern "C" {
 
 size_t minq_kv4_attend_workspace_bytes(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv,
                                        size_t head_dim) {
-  return kv_plan(n_req, n_tokens, n_heads, n_kv, head_dim).ws;
+  return kv_plan(n_req, n_tokens, n_heads, n_kv, head_dim).bytes();
 }
 
 minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_start,
@@ -1246,7 +1113,7 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
   if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15)
     return fail(MINQ_ERR_ARG, "kv4_attend: pools must be 16-byte aligned");
   const KvPlan plan = kv_plan(n_req, n_tokens, n_heads, n_kv, head_dim);
-  if (plan.ws && (!workspace || workspace_bytes < plan.ws))
+  if (plan.ws && (!workspace || workspace_bytes < plan.bytes()))
     return fail(MINQ_ERR_ARG, "workspace smaller than minq_kv4_attend_workspace_bytes");
   if (plan.ws && (reinterpret_cast<uintptr_t>(workspace) & 15))
     return fail(MINQ_ERR_ARG, "kv4_attend: workspace must be 16-byte aligned");
@@ -1276,12 +1143,22 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
     p.gsz = G < most ? G : most;
     p.hgroups = (G + p.gsz - 1) / p.gsz;
     p.tpt = most / p.gsz;
-    p.n_cta = plan.n_cta;
-    const size_t pieces = (size_t)plan.n_cta * kKvWarps;
-    p.rec = static_cast<KvRec*>(workspace);
-    p.part_o = reinterpret_cast<float*>(p.rec + pieces);
-    p.part_ml = p.part_o + pieces * 2 * cols * head_dim;
     cudaStream_t s = (cudaStream_t)stream;
+    if (plan.umma_lo) {
+      Kv4AttnParams u = p;
+      u.n_lo = plan.umma_lo;
+      u.n_hi = INT_MAX;
+      MINQ_TRY(launch_kv4_umma(u, static_cast<uint8_t*>(workspace) + plan.ws, s));
+      MINQ_TRY(head_dim == 64 ? launch_kv4_join<64>(u, 1, kKvUmmaSpread, s)
+                              : launch_kv4_join<128>(u, 1, kKvUmmaSpread, s));
+    }
+    p.n_lo = 1;
+    p.n_hi = plan.umma_lo ? plan.umma_lo - 1 : INT_MAX;
+    p.extra = kKvExtra;
+    p.n_piece = plan.n_cta * kKvWarps;
+    p.rec = static_cast<KvRec*>(workspace);
+    p.part_o = reinterpret_cast<float*>(p.rec + p.n_piece);
+    p.part_ml = p.part_o + (size_t)p.n_piece * 2 * cols * head_dim;
     if (head_dim == 64)
       return plan.split     ? launch_kv4_attend<64, 1, true>(p, s)
              : plan.nt == 1 ? launch_kv4_attend<64, 1, false>(p, s)

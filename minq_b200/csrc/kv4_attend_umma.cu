@@ -1,0 +1,767 @@
+// Causal attention over the paged 4-bit cache for the prompt chunks of a step,
+// on the 5th-generation tensor cores: the requests with enough new tokens to
+// fill a good part of 128 (token, query head) rows. kv4_attend.cu has the
+// formulas, the line of items and the kernel for all other requests.
+//
+// A tile is 128 rows of one kv head x 64 positions. Its K and V rows come by
+// bulk copies of 16 rows of one page, are turned from codes into values once
+// for all 128 rows, and every product is made of f16 parts with f32
+// accumulation:
+//   q f = Qh + Ql,  k f_t = Kh + Kl,  p 2^10 = Ph + Pl,  v f' = Vh + Vl
+//   S = Ql Kh + Qh Kl + Qh Kh,      O = Pl Vh + Ph Vl + Ph Vh,
+// 22 bits of each factor; the dropped low x low term is below 2^-23 of the
+// product. f, f_t, f' are powers of two per query row, per position and per
+// tile that put the largest value (of K and V: the largest scale) into the
+// upper part of f16's range; they are taken out again in f32, so no size of
+// the inputs matters. A tile's O is summed by itself and added to the row's
+// sum in registers with f32's rounding: the tensor core truncates, always
+// towards zero, and over thousands of positions that would show.
+//
+// One CTA per SM, four roles that work on different tiles at the same time:
+//   warps 0-3    softmax: thread = row = TMEM lane. Reads S, moves the maximum
+//                only when a weight would exceed 2^4, writes P over S.
+//   warps 4-11   sums: thread = row x half of the dimensions. acc = acc * a + O.
+//   warps 12-19  values: raw tile -> Kh Kl, Vh Vl in 128-byte swizzled tiles;
+//                its first warp issues the bulk copies.
+//   warp 20      one thread issues the MMAs: S of the next tile, then P V.
+// S, O and the K and V tiles are double buffered; TMEM: Qh Ql, 2 S, 2 O.
+// The order of dimensions inside S's contraction and of positions inside
+// P V's is free, so both are chosen for the code layout and for stores without
+// bank conflicts (q_dim and the packing of P follow them).
+//
+// A value scale that is not finite would reach rows that do not see its
+// position (0 x inf): it is left out of the tile and makes the block of the
+// rows that see it NaN.
+#include <limits.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "kv4_attend.cuh"
+#include "pipeline.cuh"
+
+namespace minq {
+
+namespace {
+
+__device__ int g_kv4_umma_status;  // see g_kv4_status
+
+constexpr int kUTile = 64;       // positions per tile
+constexpr int kUSoft = 4, kUSum = 8, kUVal = 8;  // warps of the roles
+constexpr int kUThreads = 32 * (kUSoft + kUSum + kUVal + 1);
+constexpr int kUValThreads = 32 * kUVal;
+constexpr int kUExtra = 256;     // an item's start and end, in positions
+constexpr int kUMinPiece = 512;  // smallest piece of the line per CTA
+constexpr int kURaw = 4;         // raw tiles in flight
+
+template <int HD>
+struct UmGeom {
+  static constexpr int NB = HD / 32, ROW = NB * kQ4Bytes;
+  static constexpr int RUN = 16 * ROW;         // 16 positions of K or V
+  static constexpr int RAW = 2 * 4 * RUN;      // a raw tile: K, V
+  static constexpr int KT = kUTile * HD * 2;   // Kh, Kl, Vh or Vl
+  static constexpr int K = 0, V = 4 * KT, R = 8 * KT, CTL = R + kURaw * RAW;
+  // TMEM columns
+  static constexpr int QH = 0, QL = HD / 2, S = HD, O = HD + 2 * kUTile;
+};
+
+struct UmCtl {
+  float2 corr[4][kKvUmmaRows];  // per row: factor of its sum; bit b: block b becomes NaN
+  float2 ml[kKvUmmaRows];
+  float kinv[4][kUTile];        // 1 / f_t of K
+  float vscale[2][kUTile][4];   // finite value scales of the positions that exist, else 0
+  uint32_t vmax[2][kUVal];
+  float vinv[8];                // 2^-10 / f' of V
+  int ok[8];                    // runs of 16 positions that exist
+  uint32_t bad[8][kUVal];       // not finite value scales: bit (row of the warp) * NB + block
+  int raw_ok[kURaw];
+  uint64_t raw_full[kURaw], k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t q_full, drain;
+  uint32_t tmem;
+  int abort, more, req;
+  long long req_start, red[kUThreads / 32];
+  KvItem item;
+};
+
+__device__ __forceinline__ void fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// K-major tile in the 128-byte swizzle layout, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// 16-byte chunk c (0..7) of row r.
+__device__ __forceinline__ uint32_t sw_chunk(int r, int c) {
+  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
+}
+// D (+)= A (TMEM) x B, kind::f16: A and B f16, K-major, D f32, M = 128, N = n.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, int n, uint32_t acc) {
+  const uint32_t idesc = (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   smem_u32(bar))
+               : "memory");
+}
+// 32 lanes x 32 columns of 32-bit words (this warp's lane quarter).
+__device__ __forceinline__ void tm_ld32(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Wait for this thread's TMEM loads; the values pass through the asm so that no
+// use of them is scheduled before the wait.
+__device__ __forceinline__ void tm_wait_ld(float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+      "%29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void sts16(uint32_t a, const uint32_t* v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3])
+               : "memory");
+}
+
+// Bounded wait: false after 1 s (status word and the CTA's abort flag set) or
+// once another thread gave up.
+__device__ __forceinline__ bool um_wait1(uint64_t* bar, uint32_t parity, int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (;;) {
+    if (mbar_try_wait_sleep(bar, parity, 1000u)) return true;
+    if (*reinterpret_cast<volatile int*>(abort)) return false;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      *reinterpret_cast<volatile int*>(abort) = 1;
+      atomicOr(&g_kv4_umma_status, kDeviceTimeout);
+      return false;
+    }
+  }
+}
+// The same for a whole warp: its lanes go on or give up together.
+__device__ __forceinline__ bool um_wait(uint64_t* bar, uint32_t parity, int* abort) {
+  return __all_sync(0xffffffffu, um_wait1(bar, parity, abort));
+}
+
+// f (a power of two) that puts values of at most m, m normal, into [2^11, 2^12).
+__device__ __forceinline__ uint32_t up_exponent(float m) {
+  const int e = 265 - (int)(__float_as_uint(m) >> 23);
+  return (uint32_t)min(e, 253);
+}
+
+// Value of code pair y at scales d0, d1: high and low f16 parts.
+__device__ __forceinline__ void value2(uint32_t y, float d0, float d1, uint32_t& hi, uint32_t& lo) {
+  const float2 c = __half22float2(bits_h2(y));
+  split2(c.x * d0, c.y * d1, hi, lo);
+}
+
+// The tiles of an item that this CTA takes.
+struct UmTiles {
+  int first, n;
+};
+__device__ __forceinline__ UmTiles um_tiles(const KvItem& it) {
+  const int all = (it.lim_max + kUTile - 1) / kUTile;
+  auto tile_at = [](long long x) { return x > kUExtra ? (x - kUExtra + kUTile - 1) / kUTile : 0; };
+  const int a = (int)min((long long)tile_at(it.x0), (long long)all);
+  const int b = it.x1 == it.w ? all : (int)min((long long)tile_at(it.x1), (long long)all);
+  return {a, max(b - a, 0)};
+}
+
+// Values role: all tiles of the item. g0: number of tiles that the CTA has done.
+template <int HD>
+__device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, uint8_t* sm, uint32_t base,
+                                          UmTiles tl, uint32_t g0) {
+  using GM = UmGeom<HD>;
+  constexpr int NB = GM::NB, ROW = GM::ROW;
+  const int dt = threadIdx.x - 32 * (kUSoft + kUSum), lane = dt & 31, w = dt >> 5;
+  const int lim_max = c.item.lim_max;
+  // copies: lanes 0..7 of the first warp take a run of K or V each
+  const int run = lane & 3;
+  const uint8_t* side = (lane & 4 ? p.v_pages : p.k_pages) + ((size_t)c.item.kvh << p.page_shift) * ROW;
+  const size_t page_bytes = ((size_t)p.nkv << p.page_shift) * ROW;
+  const int* tab = p.table + (size_t)c.item.rq.r * p.table_stride;
+  auto load_id = [&](int i) {
+    const int pos = (tl.first + i) * kUTile + 16 * run;
+    int id = -1;
+    if (lane < 8 && i < tl.n && pos < lim_max) id = tab[pos >> p.page_shift];
+    return id < p.n_pages ? id : -1;
+  };
+  auto issue = [&](int i, int id) {
+    const uint32_t st = (g0 + i) % kURaw;
+    const uint32_t have = __ballot_sync(0xffffffffu, id >= 0) & 15u;
+    if (lane == 0) {
+      c.raw_ok[st] = (int)have;
+      if (have)
+        mbar_arrive_expect_tx(&c.raw_full[st], 2 * __popc(have) * GM::RUN);
+      else
+        mbar_arrive(&c.raw_full[st]);
+    }
+    __syncwarp();
+    if (id >= 0) {
+      const int row = ((tl.first + i) * kUTile + 16 * run) & ((1 << p.page_shift) - 1);
+      bulk_g2s(sm + GM::R + st * GM::RAW + (lane >> 2) * 4 * GM::RUN + run * GM::RUN,
+               side + (size_t)id * page_bytes + (size_t)row * ROW, GM::RUN, &c.raw_full[st]);
+    }
+  };
+  int id = -1, issued = 0, landed = 0;
+  if (w == 0) {
+    for (; issued < min(tl.n, kURaw - 1); ++issued) issue(issued, load_id(issued));
+    id = load_id(kURaw - 1);
+  }
+  bool alive = true;  // no wait gave up; else only the barrier of the role is kept up
+  // K: (position kr, block kb) of the thread; V: eight positions pg + 8 i and
+  // four dimensions of block vb
+  const bool k_on = HD == 128 || dt < 128;
+  const int kr = (HD == 128 ? dt : dt & 127) / NB, kb = dt % NB;
+  const int vt = HD == 128 ? dt : dt - 128, pg = vt & 7, dq = vt >> 3, vb = dq >> 3;
+  for (int i = 0; i < tl.n; ++i) {
+    const uint32_t g = g0 + i, par = g >> 1, st = g & 1;
+    alive = alive && um_wait(&c.raw_full[g % kURaw], (g / kURaw) & 1, &c.abort);
+    if (alive) landed = i + 1;
+    const int pos0 = (tl.first + i) * kUTile, ok = c.raw_ok[g % kURaw];
+    const uint8_t* rk = sm + GM::R + (g % kURaw) * GM::RAW;
+    const uint8_t* rv = rk + 4 * GM::RUN;
+    const uint8_t* blk = rk + kr * ROW + kb * kQ4Bytes;
+    const bool there = k_on && ((ok >> (kr >> 4)) & 1) && pos0 + kr < lim_max;
+    const float dk = there ? *reinterpret_cast<const float*>(blk) : 0.0f;
+    const float dv = there ? *reinterpret_cast<const float*>(rv + kr * ROW + kb * kQ4Bytes) : 0.0f;
+    const bool fin = fabsf(dv) < INFINITY;
+    uint32_t code[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) code[x] = *reinterpret_cast<const uint32_t*>(blk + 4 + 4 * x);
+    // what the other roles read of tile g - 2 (K) and of g - 4, g - 8 is done with
+    if (alive && g >= 2) alive = um_wait(&c.s_full[st], (par - 1) & 1, &c.abort);
+    if (!alive) {
+      asm volatile("bar.sync 2, %0;" ::"r"(kUValThreads) : "memory");
+      continue;
+    }
+    const uint32_t bad = __ballot_sync(0xffffffffu, there && !fin);
+    const uint32_t vm = __reduce_max_sync(0xffffffffu, fin ? __float_as_uint(fabsf(dv)) : 0u);
+    if (lane == 0) {
+      c.bad[g & 7][w] = bad;
+      c.vmax[st][w] = vm;
+    }
+    float m = fabsf(dk) < INFINITY ? fabsf(dk) : 0.0f;
+#pragma unroll
+    for (int o = 1; o < NB; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t fe = up_exponent(m);
+    if (k_on) {
+      c.vscale[st][kr][kb] = fin ? dv : 0.0f;
+      if (kb == 0) c.kinv[g & 3][kr] = __uint_as_float((254u - fe) << 23);
+      if (dt == 0) c.ok[g & 7] = ok;
+      const float d = dk * __uint_as_float(fe << 23);
+      const uint32_t tile = base + GM::K + st * 2 * GM::KT + (kb >> 1) * kUTile * 128;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        uint32_t y[4], hi[4], lo[4];
+        codes4(code[x], y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) value2(y[e], d, d, hi[e], lo[e]);
+        // blocks 2, 3: chunks in another order, against bank conflicts
+        const uint32_t at = tile + sw_chunk(kr, 4 * (kb & 1) + (x ^ (kb & 2)));
+        sts16(at, hi);
+        sts16(at + GM::KT, lo);
+      }
+    }
+    fence_async_smem();
+    mbar_arrive(&c.k_full[st]);
+    asm volatile("bar.sync 2, %0;" ::"r"(kUValThreads) : "memory");
+    if (w == 0) {  // everyone is done with raw tile g - 1
+      if (issued < tl.n) issue(issued++, id);
+      id = load_id(i + kURaw);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int x = 0; x < kUVal; ++x) top = max(top, c.vmax[st][x]);
+    const uint32_t ve = up_exponent(__uint_as_float(top));
+    const float vf = __uint_as_float(ve << 23);
+    if (dt == 0) c.vinv[g & 7] = __uint_as_float((254u - ve) << 23) * 0.0009765625f;
+    if (g >= 2) alive = um_wait(&c.pv_done[st], (par - 1) & 1, &c.abort);
+    if (!alive) continue;
+    if (HD == 128 || dt >= 128) {
+      uint32_t hi[4][4], lo[4][4];  // [dimension][pair of positions]
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r0 = pg + 16 * q;
+        const uint8_t* v0 = rv + r0 * ROW + vb * kQ4Bytes + 4 + 2 * (dq & 7);
+        const uint32_t x0 = *reinterpret_cast<const uint16_t*>(v0);
+        const uint32_t x1 = *reinterpret_cast<const uint16_t*>(v0 + 8 * ROW);
+        const float d0 = c.vscale[st][r0][vb] * vf, d1 = c.vscale[st][r0 + 8][vb] * vf;
+        uint32_t y[4];
+        codes4(__byte_perm(x0, x1, 0x5410), y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) value2(y[e], d0, d1, hi[e][q], lo[e][q]);
+      }
+      const uint32_t tile = base + GM::V + st * 2 * GM::KT;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t at = tile + sw_chunk(4 * dq + e, pg);
+        sts16(at, hi[e]);
+        sts16(at + GM::KT, lo[e]);
+      }
+    }
+    fence_async_smem();
+    mbar_arrive(&c.v_full[st]);
+  }
+  if (w == 0)  // after a wait that gave up: let the copies in flight end
+    for (; landed < issued; ++landed)
+      mbar_wait_timed(&c.raw_full[(g0 + landed) % kURaw], ((g0 + landed) / kURaw) & 1,
+                      &g_kv4_umma_status);
+}
+
+// First of the eight dimensions d of chunk x of S's contraction (4 columns of
+// Q, d + e and d + e + 4 in column e): see um_values.
+template <int HD>
+__device__ __forceinline__ constexpr int q_dim(int x) {
+  return (x >> 2) * 32 + 8 * ((x & 3) ^ ((x >> 2) & 2));
+}
+
+// Softmax role.
+template <int HD>
+__device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, uint32_t tmem, UmTiles tl,
+                                           uint32_t g0) {
+  using GM = UmGeom<HD>;
+  constexpr int NB = GM::NB;
+  const int row = threadIdx.x;
+  const uint32_t tlane = tmem + ((uint32_t)(row & ~31) << 16);
+  const int ct = row / p.gsz, ch = row - ct * p.gsz;
+  const bool on = ct < c.item.ntok && ch < c.item.nhead;
+  long long lim64 = on ? (long long)c.item.prior + c.item.tok0 + ct + 1 : 0;
+  lim64 = lim64 < 0 ? 0 : lim64 < c.item.cap ? lim64 : c.item.cap;
+  const int lim = (int)lim64;
+  float cn;
+  {
+    const float* q = p.q + (size_t)(c.item.rq.t0 + c.item.tok0 + (on ? ct : 0)) * p.q_stride +
+                     (size_t)(c.item.h0 + (on ? ch : 0)) * HD;
+    const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+    auto load8 = [&](int d, float* v) {
+      if (vec) {
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(q + d);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(q + d + 4);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = q[d + e];
+      }
+    };
+    float m = 0.0f;
+#pragma unroll 4
+    for (int d = 0; d < HD; d += 8) {
+      float v[8];
+      load8(d, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+    }
+    const int ex = min(max((int)(__float_as_uint(m) >> 23), 24), 254);
+    float f = __uint_as_float((uint32_t)(264 - ex) << 23);
+    cn = fabsf(p.scale) * 1.4426950408889634f * (1.0f / f);
+    if (cn == 0.0f) cn = 1.4e-45f;  // -inf stays masked
+    if (p.scale < 0.0f) f = -f;
+#pragma unroll
+    for (int x0 = 0; x0 < HD / 2; x0 += 32) {
+      uint32_t hi[32], lo[32];
+#pragma unroll
+      for (int x = 0; x < 32; x += 4) {
+        float v[8];
+        load8(q_dim<HD>((x0 + x) / 4), v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          split2(on ? v[e] * f : 0.0f, on ? v[e + 4] * f : 0.0f, hi[x + e], lo[x + e]);
+      }
+      tm_st32(tlane + GM::QH + x0, hi);
+      tm_st32(tlane + GM::QL + x0, lo);
+    }
+    tm_wait_st();
+    fence_before();
+    mbar_arrive(&c.q_full);
+  }
+  float m = -INFINITY, l = 0.0f;
+  for (int i = 0; i < tl.n; ++i) {
+    const uint32_t g = g0 + i, st = g & 1;
+    if (!um_wait(&c.s_full[st], (g >> 1) & 1, &c.abort)) return;
+    fence_after();
+    float s[kUTile];
+    tm_ld32(tlane + GM::S + st * kUTile, s);
+    tm_ld32(tlane + GM::S + st * kUTile + 32, s + 32);
+    tm_wait_ld(s);
+    tm_wait_ld(s + 32);
+    const int pos0 = (tl.first + i) * kUTile, ok = c.ok[g & 7];
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kUTile; j += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(&c.kinv[g & 3][j]);
+      s[j] *= k.x;
+      s[j + 1] *= k.y;
+      s[j + 2] *= k.z;
+      s[j + 3] *= k.w;
+    }
+    if (!__all_sync(0xffffffffu, ok == 15 && pos0 + kUTile <= lim)) {
+#pragma unroll
+      for (int j = 0; j < kUTile; ++j)
+        if (!((ok >> (j >> 4)) & 1) || pos0 + j >= lim) s[j] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < kUTile; ++j) top = fmaxf(top, s[j]);
+    top = top == -INFINITY ? top : top * cn;
+    float a = 1.0f;
+    if (top > m + 4.0f) {  // also the first that is seen
+      a = ex2(m - top);
+      m = top;
+      l *= a;
+    }
+    const float off = m == -INFINITY ? 0.0f : 10.0f - m;
+    float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kUTile; j += 2) {
+      s[j] = ex2(fmaf(s[j], cn, off));
+      s[j + 1] = ex2(fmaf(s[j + 1], cn, off));
+      sum0 += s[j];
+      sum1 += s[j + 1];
+    }
+    l += sum0 + sum1;
+    // P's column x holds positions (x / 4) + 16 (x mod 4) and 8 further on
+    uint32_t hi[32], lo[32];
+#pragma unroll
+    for (int x = 0; x < 32; ++x) {
+      const int j = (x >> 2) + 16 * (x & 3);
+      split2(s[j], s[j + 8], hi[x], lo[x]);
+    }
+    tm_st32(tlane + GM::S + st * kUTile, hi);
+    tm_st32(tlane + GM::S + st * kUTile + 32, lo);
+    uint32_t nan = 0, any = 0;
+#pragma unroll
+    for (int x = 0; x < kUVal; ++x) any |= c.bad[g & 7][x];
+    if (any) {
+      constexpr int PER = 32 / NB;  // positions of a word
+      for (int x = 0; x < kUTile / PER; ++x)
+        for (int b = 0; b < 32; ++b)
+          if (((c.bad[g & 7][x] >> b) & 1) && pos0 + x * PER + b / NB < lim) nan |= 1u << (b % NB);
+    }
+    c.corr[g & 3][row] = make_float2(a, __uint_as_float(nan));
+    tm_wait_st();
+    fence_before();
+    mbar_arrive(&c.p_full[st]);
+  }
+  c.ml[row] = make_float2(l == 0.0f ? -3.0e38f : m, l * 0.0009765625f);
+}
+
+// The thread that issues the MMAs.
+template <int HD>
+__device__ __forceinline__ void um_mma(UmCtl& c, uint32_t tmem, uint32_t base, UmTiles tl, uint32_t g0,
+                                       uint32_t items) {
+  using GM = UmGeom<HD>;
+  if (!um_wait1(&c.q_full, items & 1, &c.abort)) return;
+  auto scores = [&](int i) {
+    const uint32_t g = g0 + i, st = g & 1, d = tmem + GM::S + st * kUTile;
+    if (!um_wait1(&c.k_full[st], (g >> 1) & 1, &c.abort)) return false;
+    fence_after();
+    const uint32_t kt = base + GM::K + st * 2 * GM::KT;
+    // the small parts first: what the accumulation truncates next to them is nothing
+#pragma unroll
+    for (int part = 0; part < 3; ++part)
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j) {
+        const uint32_t a = tmem + (part == 0 ? GM::QL : GM::QH) + 8 * j;
+        const uint32_t b = kt + (part == 1 ? GM::KT : 0) + (j >> 2) * kUTile * 128 + (j & 3) * 32;
+        mma_ts(d, a, sw128(b), kUTile, part > 0 || j > 0);
+      }
+    mma_commit(&c.s_full[st]);
+    return true;
+  };
+  if (tl.n > 0 && !scores(0)) return;
+  for (int i = 0; i < tl.n; ++i) {
+    if (i + 1 < tl.n && !scores(i + 1)) return;
+    const uint32_t g = g0 + i, st = g & 1, par = (g >> 1) & 1;
+    if (!um_wait1(&c.p_full[st], par, &c.abort) || !um_wait1(&c.v_full[st], par, &c.abort)) return;
+    if (g >= 2 && !um_wait1(&c.o_free[st], par ^ 1, &c.abort)) return;
+    fence_after();
+    const uint32_t vt = base + GM::V + st * 2 * GM::KT, d = tmem + GM::O + st * HD;
+#pragma unroll
+    for (int part = 0; part < 3; ++part)
+#pragma unroll
+      for (int j = 0; j < kUTile / 16; ++j) {
+        const uint32_t a = tmem + GM::S + st * kUTile + (part == 0 ? 32 : 0) + 8 * j;
+        mma_ts(d, a, sw128(vt + (part == 1 ? GM::KT : 0) + j * 32), HD, part > 0 || j > 0);
+      }
+    mma_commit(&c.pv_done[st]);
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_constant__ Kv4AttnParams p) {
+  using GM = UmGeom<HD>;
+  extern __shared__ uint8_t um_smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t base = (smem_u32(um_smem) + 1023u) & ~1023u;
+  uint8_t* sm = um_smem + (base - smem_u32(um_smem));
+  UmCtl& c = *reinterpret_cast<UmCtl*>(sm + GM::CTL);
+  constexpr int kMmaWarp = kUSoft + kUSum + kUVal;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < kURaw; ++i) mbar_init(&c.raw_full[i], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&c.k_full[i], kUValThreads);
+        mbar_init(&c.v_full[i], kUValThreads);
+        mbar_init(&c.s_full[i], 1);
+        mbar_init(&c.p_full[i], 32 * kUSoft);
+        mbar_init(&c.pv_done[i], 1);
+        mbar_init(&c.o_free[i], 32 * kUSum);
+      }
+      mbar_init(&c.q_full, 32 * kUSoft);
+      mbar_init(&c.drain, 1);
+      c.abort = 0;
+      c.req = -1;
+      mbar_fence_init();
+    }
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_u32(&c.tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // the line: every warp weighs a run of the requests, and the warp in whose
+  // run the CTA's piece starts looks for the request
+  const int H = p.nkv * p.hgroups, seg = (p.n_req + kUThreads / 32 - 1) / (kUThreads / 32);
+  const int r_lo = min(warp * seg, p.n_req), r_hi = min(r_lo + seg, p.n_req);
+  auto weight = [&](int r) {
+    const KvReq q = kv_req(p, r);
+    return H * kv_cum(q, p.tpt, q.J);
+  };
+  long long mine = 0;
+  for (int r = r_lo + lane; r < r_hi; r += 32) mine += weight(r);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) c.red[warp] = mine;
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = c.tmem;
+  long long total = 0, before = 0;
+  for (int x = 0; x < kUThreads / 32; ++x) {
+    if (x < warp) before += c.red[x];
+    total += c.red[x];
+  }
+  long long per = (total + p.n_piece - 1) / p.n_piece;
+  if (per < kUMinPiece) per = kUMinPiece;
+  const long long c0 = per * blockIdx.x, c1 = min(c0 + per, total);
+  if (c0 < c1 && before <= c0 && c0 < before + mine) {
+    for (int r0 = r_lo; r0 < r_hi; r0 += 32) {
+      const long long w = r0 + lane < r_hi ? weight(r0 + lane) : 0;
+      long long incl = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+      }
+      const long long start = before + incl - w;
+      if (start <= c0 && c0 < start + w) {
+        c.req = r0 + lane;
+        c.req_start = start;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  if (tid == 0) p.rec[blockIdx.x].parts = 0;
+  __syncthreads();
+  if (tid == 0) {
+    c.more = c0 < c1 && c.req >= 0;
+    if (c.more) {
+      KvItem x;
+      kv_item_at(p, x, c.req, c.req_start, c0);
+      x.x0 = c0 - x.start;
+      x.x1 = min(c1 - x.start, x.w);
+      c.item = x;
+    }
+  }
+  __syncthreads();
+
+  uint32_t g0 = 0;
+  bool more = c.more;
+  for (uint32_t items = 0; more; ++items) {
+    const UmTiles tl = um_tiles(c.item);
+    if (warp < kUSoft) {
+      um_softmax<HD>(p, c, tmem, tl, g0);
+      __syncthreads();
+      if (tid == 0) {
+        const KvItem& it = c.item;
+        if (it.x1 < it.w && it.x0 == 0) {  // starts here and goes on
+          KvRec r{};
+          r.r = it.rq.r;
+          r.h = it.h;
+          r.j = (int)it.j;
+          r.a = blockIdx.x;
+          r.n_first = r.parts = (int)((it.start + it.w - 1) / per) - (int)blockIdx.x + 1;
+          p.rec[blockIdx.x] = r;
+        }
+      }
+    } else if (warp < kUSoft + kUSum) {
+      // sums: row x half of the dimensions
+      constexpr int N = HD / 2;
+      const int row = 32 * (warp & 3) + lane, half = (warp - kUSoft) >> 2;
+      const uint32_t col = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + GM::O + half * N;
+      float acc[N];
+#pragma unroll
+      for (int d = 0; d < N; ++d) acc[d] = 0.0f;
+      for (int i = 0; i < tl.n; ++i) {
+        const uint32_t g = g0 + i, st = g & 1, par = (g >> 1) & 1;
+        if (!um_wait(&c.pv_done[st], par, &c.abort)) break;
+        fence_after();
+        const float2 cr = c.corr[g & 3][row];
+        const float f = c.vinv[g & 7];
+        const uint32_t nan = __float_as_uint(cr.y);
+#pragma unroll
+        for (int d0 = 0; d0 < N; d0 += 32) {
+          float o[32];
+          tm_ld32(col + st * HD + d0, o);
+          tm_wait_ld(o);
+          const float bad = (nan >> ((half * N + d0) / 32)) & 1 ? NAN : 0.0f;
+          if (__any_sync(0xffffffffu, nan != 0))
+#pragma unroll
+            for (int d = 0; d < 32; ++d) o[d] += bad;
+#pragma unroll
+          for (int d = 0; d < 32; ++d) acc[d0 + d] = fmaf(acc[d0 + d], cr.x, o[d] * f);
+        }
+        fence_before();
+        mbar_arrive(&c.o_free[st]);
+      }
+      __syncthreads();
+      const KvItem& it = c.item;
+      const int ct = row / p.gsz, ch = row - ct * p.gsz;
+      if (ct < it.ntok && ch < it.nhead) {
+        const float2 ml = c.ml[row];
+        const bool whole = it.x0 == 0 && it.x1 == it.w;
+        const size_t at = ((size_t)blockIdx.x * 2 + (it.x0 > 0 ? 0 : 1)) * kKvUmmaRows + row;
+        const float r = !whole ? 1.0f : ml.y != 0.0f ? 1.0f / ml.y : 0.0f;
+        float* dst = whole ? p.out + (size_t)(it.rq.t0 + it.tok0 + ct) * p.out_stride +
+                                 (size_t)(it.h0 + ch) * HD
+                           : p.part_o + at * HD;
+        dst += half * N;
+        if (!whole && half == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = ml;
+        if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+#pragma unroll
+          for (int d = 0; d < N; d += 4)
+            *reinterpret_cast<float4*>(dst + d) =
+                make_float4(acc[d] * r, acc[d + 1] * r, acc[d + 2] * r, acc[d + 3] * r);
+        } else {
+#pragma unroll
+          for (int d = 0; d < N; ++d) dst[d] = acc[d] * r;
+        }
+      }
+    } else {
+      if (warp < kMmaWarp) {
+        um_values<HD>(p, c, sm, base, tl, g0);
+      } else {
+        if (lane == 0) um_mma<HD>(c, tmem, base, tl, g0, items);
+        __syncwarp();
+      }
+      __syncthreads();
+    }
+    g0 += tl.n;
+    __syncthreads();
+    if (c.abort) break;
+    if (tid == 0) {
+      KvItem x = c.item;
+      c.more = x.start + x.w < c1 && kv_item_next(p, x);
+      if (c.more) {
+        x.x0 = 0;
+        x.x1 = min(c1 - x.start, x.w);
+        c.item = x;
+      }
+    }
+    __syncthreads();
+    more = c.more;
+  }
+  if (c.abort && tid == 32 * kMmaWarp) {  // after a wait that gave up: let the MMAs end
+    mma_commit(&c.drain);
+    mbar_wait_timed(&c.drain, 0, &g_kv4_umma_status);
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+template <int HD>
+minq_status launch_umma(const Kv4AttnParams& p, cudaStream_t s) {
+  constexpr size_t smem = 1024 + UmGeom<HD>::CTL + sizeof(UmCtl);
+  static_assert(smem <= 227 * 1024, "shared memory of the tcgen05 kernel");
+  auto k = kv4_umma_kernel<HD>;
+  MINQ_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(k), smem));
+  MINQ_CUDA_TRY(launch_k(k, dim3(p.n_piece), dim3(kUThreads), smem, s, p));
+  return MINQ_OK;
+}
+
+}  // namespace
+
+size_t kv4_umma_workspace(size_t head_dim) {
+  return (size_t)sm_count() * (2 * kKvUmmaRows * (head_dim + 2) * 4 + sizeof(KvRec));
+}
+
+minq_status launch_kv4_umma(Kv4AttnParams& p, void* workspace, cudaStream_t s) {
+  const int G = p.nh / p.nkv;
+  p.cols = kKvUmmaRows;
+  p.gsz = G < kKvUmmaRows ? G : kKvUmmaRows;
+  p.hgroups = (G + p.gsz - 1) / p.gsz;
+  p.tpt = kKvUmmaRows / p.gsz;
+  p.extra = kUExtra;
+  p.n_piece = sm_count();
+  p.rec = static_cast<KvRec*>(workspace);
+  p.part_o = reinterpret_cast<float*>(p.rec + p.n_piece);
+  p.part_ml = p.part_o + (size_t)p.n_piece * 2 * kKvUmmaRows * p.hd;
+  return p.hd == 64 ? launch_umma<64>(p, s) : launch_umma<128>(p, s);
+}
+
+minq_status take_kv4_umma_status(int* v) {
+  MINQ_CUDA_TRY(cudaMemcpyFromSymbol(v, g_kv4_umma_status, sizeof(int)));
+  if (*v == 0) return MINQ_OK;
+  const int zero = 0;
+  MINQ_CUDA_TRY(cudaMemcpyToSymbol(g_kv4_umma_status, &zero, sizeof(int)));
+  return MINQ_OK;
+}
+
+}  // namespace minq
