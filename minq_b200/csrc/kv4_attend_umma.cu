@@ -20,10 +20,10 @@
 // One CTA per SM, four roles that work on different tiles at the same time:
 //   warps 0-3    softmax: thread = row = TMEM lane. Reads S, moves the maximum
 //                only when a weight would exceed 2^4, writes P over S.
-//   warps 4-11   sums: thread = row x half of the dimensions. acc = acc * a + O.
-//   warps 12-19  values: raw tile -> Kh Kl, Vh Vl in 128-byte swizzled tiles;
+//   warps 4-7    sums: thread = row. acc = acc * a + O.
+//   warps 8-15   values: raw tile -> Kh Kl, Vh Vl in 128-byte swizzled tiles;
 //                its first warp issues the bulk copies.
-//   warp 20      one thread issues the MMAs: S of the next tile, then P V.
+//   warp 16      one thread issues the MMAs: S of the next tile, then P V.
 // S, O and the K and V tiles are double buffered; TMEM: Qh Ql, 2 S, 2 O.
 // The order of dimensions inside S's contraction and of positions inside
 // P V's is free, so both are chosen for the code layout and for stores without
@@ -46,8 +46,12 @@ namespace {
 __device__ int g_kv4_umma_status;  // see g_kv4_status
 
 constexpr int kUTile = 64;       // positions per tile
-constexpr int kUSoft = 4, kUSum = 8, kUVal = 8;  // warps of the roles
-constexpr int kUThreads = 32 * (kUSoft + kUSum + kUVal + 1);
+constexpr int kUSoft = 4, kUSum = 4, kUVal = 8;  // warps of the roles
+constexpr int kUThreads = 32 * (kUSoft + kUSum + kUVal + 4);
+// Registers a thread: 96 at the launch (640 threads), then by role (each a
+// whole number of warpgroups): 120 + 176 + 2 x 72 + 40 <= 5 x 96.
+constexpr int kURegSoft = 120, kURegSum = 176, kURegVal = 72, kURegMma = 40;
+static_assert(kURegSoft + kURegSum + 2 * kURegVal + kURegMma <= 5 * 96, "registers");
 constexpr int kUValThreads = 32 * kUVal;
 constexpr int kUExtra = 256;     // an item's start and end, in positions
 constexpr int kUMinPiece = 512;  // smallest piece of the line per CTA
@@ -68,7 +72,8 @@ struct UmCtl {
   float2 corr[4][kKvUmmaRows];  // per row: factor of its sum; bit b: block b becomes NaN
   float2 ml[kKvUmmaRows];
   float kinv[4][kUTile];        // 1 / f_t of K
-  float vscale[2][kUTile][4];   // finite value scales of the positions that exist, else 0
+  // value scales of the positions that exist (0: not, or not finite) as two f16 parts
+  uint32_t vscale[2][kUTile][4];
   uint32_t vmax[2][kUVal];
   float vinv[8];                // 2^-10 / f' of V
   int ok[8];                    // runs of 16 positions that exist
@@ -79,7 +84,7 @@ struct UmCtl {
   uint32_t tmem;
   int abort, more, req;
   long long req_start, red[kUThreads / 32];
-  KvItem item;
+  KvItem item[2];  // this one and the next
 };
 
 __device__ __forceinline__ void fence_before() {
@@ -142,6 +147,18 @@ __device__ __forceinline__ void tm_wait_ld(float* v) {
                :
                : "memory");
 }
+// 16 columns, waited for.
+__device__ __forceinline__ void tm_ld16(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
@@ -165,8 +182,7 @@ __device__ __forceinline__ void sts16(uint32_t a, const uint32_t* v) {
 
 // Bounded wait: false after 1 s (status word and the CTA's abort flag set) or
 // once another thread gave up.
-__device__ __forceinline__ bool um_wait1(uint64_t* bar, uint32_t parity, int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
+__device__ __forceinline__ bool um_wait_long(uint64_t* bar, uint32_t parity, int* abort) {
   const uint64_t t0 = global_timer_ns();
   for (;;) {
     if (mbar_try_wait_sleep(bar, parity, 1000u)) return true;
@@ -177,6 +193,9 @@ __device__ __forceinline__ bool um_wait1(uint64_t* bar, uint32_t parity, int* ab
       return false;
     }
   }
+}
+__device__ __forceinline__ bool um_wait1(uint64_t* bar, uint32_t parity, int* abort) {
+  return mbar_try_wait_sleep(bar, parity, 20000u) || um_wait_long(bar, parity, abort);
 }
 // The same for a whole warp: its lanes go on or give up together.
 __device__ __forceinline__ bool um_wait(uint64_t* bar, uint32_t parity, int* abort) {
@@ -189,10 +208,34 @@ __device__ __forceinline__ uint32_t up_exponent(float m) {
   return (uint32_t)min(e, 253);
 }
 
-// Value of code pair y at scales d0, d1: high and low f16 parts.
-__device__ __forceinline__ void value2(uint32_t y, float d0, float d1, uint32_t& hi, uint32_t& lo) {
-  const float2 c = __half22float2(bits_h2(y));
-  split2(c.x * d0, c.y * d1, hi, lo);
+// A scale d as two f16 parts, high in the low half word. The high part has 8
+// bits, so a code (4 bits with its sign) times it is exact; the low part and
+// its product with a code are rounded, 2^-20 of the value each at most.
+__device__ __forceinline__ uint32_t scale_parts(float d) {
+  const __half h = __float2half_rn(__uint_as_float((__float_as_uint(d) + 0x8000u) & 0xffff0000u));
+  return h2_bits(__halves2half2(h, __float2half_rn(d - __half2float(h))));
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  return h2_bits(__hmul2(bits_h2(a), bits_h2(b)));
+}
+// x = x * y, x = x * y + z, x + y on two f32 at once.
+__device__ __forceinline__ void mul_f2(float* x, float y0, float y1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x[0]), "+f"(x[1])
+      : "f"(y0), "f"(y1));
+}
+__device__ __forceinline__ void fma_f2(float* x, float y, float z0, float z1) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\t"
+      "mov.b64 c, {%3, %4};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x[0]), "+f"(x[1])
+      : "f"(y), "f"(z0), "f"(z1));
+}
+__device__ __forceinline__ void add_f2(float* x, const float* y) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x[0]), "+f"(x[1])
+      : "f"(y[0]), "f"(y[1]));
 }
 
 // The tiles of an item that this CTA takes.
@@ -209,17 +252,17 @@ __device__ __forceinline__ UmTiles um_tiles(const KvItem& it) {
 
 // Values role: all tiles of the item. g0: number of tiles that the CTA has done.
 template <int HD>
-__device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, uint8_t* sm, uint32_t base,
-                                          UmTiles tl, uint32_t g0) {
+__device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, const KvItem& it, uint8_t* sm,
+                                          uint32_t base, UmTiles tl, uint32_t g0) {
   using GM = UmGeom<HD>;
   constexpr int NB = GM::NB, ROW = GM::ROW;
   const int dt = threadIdx.x - 32 * (kUSoft + kUSum), lane = dt & 31, w = dt >> 5;
-  const int lim_max = c.item.lim_max;
+  const int lim_max = it.lim_max;
   // copies: lanes 0..7 of the first warp take a run of K or V each
   const int run = lane & 3;
-  const uint8_t* side = (lane & 4 ? p.v_pages : p.k_pages) + ((size_t)c.item.kvh << p.page_shift) * ROW;
+  const uint8_t* side = (lane & 4 ? p.v_pages : p.k_pages) + ((size_t)it.kvh << p.page_shift) * ROW;
   const size_t page_bytes = ((size_t)p.nkv << p.page_shift) * ROW;
-  const int* tab = p.table + (size_t)c.item.rq.r * p.table_stride;
+  const int* tab = p.table + (size_t)it.rq.r * p.table_stride;
   auto load_id = [&](int i) {
     const int pos = (tl.first + i) * kUTile + 16 * run;
     int id = -1;
@@ -273,6 +316,7 @@ __device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, uint
     if (alive && g >= 2) alive = um_wait(&c.s_full[st], (par - 1) & 1, &c.abort);
     if (!alive) {
       asm volatile("bar.sync 2, %0;" ::"r"(kUValThreads) : "memory");
+      asm volatile("bar.sync 3, %0;" ::"r"(kUValThreads) : "memory");
       continue;
     }
     const uint32_t bad = __ballot_sync(0xffffffffu, there && !fin);
@@ -281,30 +325,6 @@ __device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, uint
       c.bad[g & 7][w] = bad;
       c.vmax[st][w] = vm;
     }
-    float m = fabsf(dk) < INFINITY ? fabsf(dk) : 0.0f;
-#pragma unroll
-    for (int o = 1; o < NB; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t fe = up_exponent(m);
-    if (k_on) {
-      c.vscale[st][kr][kb] = fin ? dv : 0.0f;
-      if (kb == 0) c.kinv[g & 3][kr] = __uint_as_float((254u - fe) << 23);
-      if (dt == 0) c.ok[g & 7] = ok;
-      const float d = dk * __uint_as_float(fe << 23);
-      const uint32_t tile = base + GM::K + st * 2 * GM::KT + (kb >> 1) * kUTile * 128;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint32_t y[4], hi[4], lo[4];
-        codes4(code[x], y);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) value2(y[e], d, d, hi[e], lo[e]);
-        // blocks 2, 3: chunks in another order, against bank conflicts
-        const uint32_t at = tile + sw_chunk(kr, 4 * (kb & 1) + (x ^ (kb & 2)));
-        sts16(at, hi);
-        sts16(at + GM::KT, lo);
-      }
-    }
-    fence_async_smem();
-    mbar_arrive(&c.k_full[st]);
     asm volatile("bar.sync 2, %0;" ::"r"(kUValThreads) : "memory");
     if (w == 0) {  // everyone is done with raw tile g - 1
       if (issued < tl.n) issue(issued++, id);
@@ -314,8 +334,37 @@ __device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, uint
 #pragma unroll
     for (int x = 0; x < kUVal; ++x) top = max(top, c.vmax[st][x]);
     const uint32_t ve = up_exponent(__uint_as_float(top));
-    const float vf = __uint_as_float(ve << 23);
-    if (dt == 0) c.vinv[g & 7] = __uint_as_float((254u - ve) << 23) * 0.0009765625f;
+    if (dt == 0) {
+      c.vinv[g & 7] = __uint_as_float((254u - ve) << 23) * 0.0009765625f;
+      c.ok[g & 7] = ok;
+    }
+    float m = fabsf(dk) < INFINITY ? fabsf(dk) : 0.0f;
+#pragma unroll
+    for (int o = 1; o < NB; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t fe = up_exponent(m);
+    if (k_on) {
+      c.vscale[st][kr][kb] = scale_parts((fin ? dv : 0.0f) * __uint_as_float(ve << 23));
+      if (kb == 0) c.kinv[g & 3][kr] = __uint_as_float((254u - fe) << 23);
+      const uint32_t d = scale_parts(dk * __uint_as_float(fe << 23));
+      const uint32_t dh = __byte_perm(d, d, 0x1010), dl = __byte_perm(d, d, 0x3232);
+      const uint32_t tile = base + GM::K + st * 2 * GM::KT + (kb >> 1) * kUTile * 128;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        uint32_t y[4], v[4];
+        codes4(code[x], y);
+        // blocks 2, 3: chunks in another order, against bank conflicts
+        const uint32_t at = tile + sw_chunk(kr, 4 * (kb & 1) + (x ^ (kb & 2)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = mul2(y[e], dh);
+        sts16(at, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = mul2(y[e], dl);
+        sts16(at + GM::KT, v);
+      }
+    }
+    fence_async_smem();
+    mbar_arrive(&c.k_full[st]);
+    asm volatile("bar.sync 3, %0;" ::"r"(kUValThreads) : "memory");
     if (g >= 2) alive = um_wait(&c.pv_done[st], (par - 1) & 1, &c.abort);
     if (!alive) continue;
     if (HD == 128 || dt >= 128) {
@@ -326,11 +375,15 @@ __device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, uint
         const uint8_t* v0 = rv + r0 * ROW + vb * kQ4Bytes + 4 + 2 * (dq & 7);
         const uint32_t x0 = *reinterpret_cast<const uint16_t*>(v0);
         const uint32_t x1 = *reinterpret_cast<const uint16_t*>(v0 + 8 * ROW);
-        const float d0 = c.vscale[st][r0][vb] * vf, d1 = c.vscale[st][r0 + 8][vb] * vf;
+        const uint32_t d0 = c.vscale[st][r0][vb], d1 = c.vscale[st][r0 + 8][vb];
+        const uint32_t dh = __byte_perm(d0, d1, 0x5410), dl = __byte_perm(d0, d1, 0x7632);
         uint32_t y[4];
         codes4(__byte_perm(x0, x1, 0x5410), y);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) value2(y[e], d0, d1, hi[e][q], lo[e][q]);
+        for (int e = 0; e < 4; ++e) {
+          hi[e][q] = mul2(y[e], dh);
+          lo[e][q] = mul2(y[e], dl);
+        }
       }
       const uint32_t tile = base + GM::V + st * 2 * GM::KT;
 #pragma unroll
@@ -358,21 +411,21 @@ __device__ __forceinline__ constexpr int q_dim(int x) {
 
 // Softmax role.
 template <int HD>
-__device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, uint32_t tmem, UmTiles tl,
-                                           uint32_t g0) {
+__device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, const KvItem& it,
+                                           uint32_t tmem, UmTiles tl, uint32_t g0) {
   using GM = UmGeom<HD>;
   constexpr int NB = GM::NB;
   const int row = threadIdx.x;
   const uint32_t tlane = tmem + ((uint32_t)(row & ~31) << 16);
   const int ct = row / p.gsz, ch = row - ct * p.gsz;
-  const bool on = ct < c.item.ntok && ch < c.item.nhead;
-  long long lim64 = on ? (long long)c.item.prior + c.item.tok0 + ct + 1 : 0;
-  lim64 = lim64 < 0 ? 0 : lim64 < c.item.cap ? lim64 : c.item.cap;
+  const bool on = ct < it.ntok && ch < it.nhead;
+  long long lim64 = on ? (long long)it.prior + it.tok0 + ct + 1 : 0;
+  lim64 = lim64 < 0 ? 0 : lim64 < it.cap ? lim64 : it.cap;
   const int lim = (int)lim64;
   float cn;
   {
-    const float* q = p.q + (size_t)(c.item.rq.t0 + c.item.tok0 + (on ? ct : 0)) * p.q_stride +
-                     (size_t)(c.item.h0 + (on ? ch : 0)) * HD;
+    const float* q = p.q + (size_t)(it.rq.t0 + it.tok0 + (on ? ct : 0)) * p.q_stride +
+                     (size_t)(it.h0 + (on ? ch : 0)) * HD;
     const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
     auto load8 = [&](int d, float* v) {
       if (vec) {
@@ -429,10 +482,8 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, uin
 #pragma unroll
     for (int j = 0; j < kUTile; j += 4) {
       const float4 k = *reinterpret_cast<const float4*>(&c.kinv[g & 3][j]);
-      s[j] *= k.x;
-      s[j + 1] *= k.y;
-      s[j + 2] *= k.z;
-      s[j + 3] *= k.w;
+      mul_f2(s + j, k.x, k.y);
+      mul_f2(s + j + 2, k.z, k.w);
     }
     if (!__all_sync(0xffffffffu, ok == 15 && pos0 + kUTile <= lim)) {
 #pragma unroll
@@ -449,15 +500,15 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, uin
       l *= a;
     }
     const float off = m == -INFINITY ? 0.0f : 10.0f - m;
-    float sum0 = 0.0f, sum1 = 0.0f;
+    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < kUTile; j += 2) {
-      s[j] = ex2(fmaf(s[j], cn, off));
-      s[j + 1] = ex2(fmaf(s[j + 1], cn, off));
-      sum0 += s[j];
-      sum1 += s[j + 1];
+      fma_f2(s + j, cn, off, off);
+      s[j] = ex2(s[j]);
+      s[j + 1] = ex2(s[j + 1]);
+      add_f2(sum, s + j);
     }
-    l += sum0 + sum1;
+    l += sum[0] + sum[1];
     // P's column x holds positions (x / 4) + 16 (x mod 4) and 8 further on
     uint32_t hi[32], lo[32];
 #pragma unroll
@@ -524,6 +575,72 @@ __device__ __forceinline__ void um_mma(UmCtl& c, uint32_t tmem, uint32_t base, U
       }
     mma_commit(&c.pv_done[st]);
   }
+}
+
+// Sums role, up to the item's outputs.
+template <int HD>
+__device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const KvItem& it, uint32_t tmem,
+                                        UmTiles tl, uint32_t g0) {
+  using GM = UmGeom<HD>;
+  const int row = threadIdx.x - 32 * kUSoft;
+  const uint32_t col = tmem + ((uint32_t)(row & ~31) << 16) + GM::O;
+  float acc[HD];
+#pragma unroll
+  for (int d = 0; d < HD; ++d) acc[d] = 0.0f;
+  for (int i = 0; i < tl.n; ++i) {
+    const uint32_t g = g0 + i, st = g & 1;
+    if (!um_wait(&c.pv_done[st], (g >> 1) & 1, &c.abort)) break;
+    fence_after();
+    const float2 cr = c.corr[g & 3][row];
+    const float f = c.vinv[g & 7];
+    const uint32_t nan = __float_as_uint(cr.y);
+#pragma unroll
+    for (int d0 = 0; d0 < HD; d0 += 16) {
+      float o[16];
+      tm_ld16(col + st * HD + d0, o);
+      const float fn = (nan >> (d0 / 32)) & 1 ? NAN : f;
+#pragma unroll
+      for (int d = 0; d < 16; d += 2) {
+        mul_f2(o + d, fn, fn);
+        fma_f2(acc + d0 + d, cr.x, o[d], o[d + 1]);
+      }
+    }
+    fence_before();
+    mbar_arrive(&c.o_free[st]);
+  }
+  __syncthreads();
+  const int ct = row / p.gsz, ch = row - ct * p.gsz;
+  if (ct < it.ntok && ch < it.nhead) {
+    const float2 ml = c.ml[row];
+    const bool whole = it.x0 == 0 && it.x1 == it.w;
+    const size_t at = ((size_t)blockIdx.x * 2 + (it.x0 > 0 ? 0 : 1)) * kKvUmmaRows + row;
+    const float r = !whole ? 1.0f : ml.y != 0.0f ? 1.0f / ml.y : 0.0f;
+    float* dst = whole ? p.out + (size_t)(it.rq.t0 + it.tok0 + ct) * p.out_stride +
+                             (size_t)(it.h0 + ch) * HD
+                       : p.part_o + at * HD;
+    if (!whole) *reinterpret_cast<float2*>(p.part_ml + at * 2) = ml;
+    if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+#pragma unroll
+      for (int d = 0; d < HD; d += 4)
+        *reinterpret_cast<float4*>(dst + d) =
+            make_float4(acc[d] * r, acc[d + 1] * r, acc[d + 2] * r, acc[d + 3] * r);
+    } else {
+#pragma unroll
+      for (int d = 0; d < HD; ++d) dst[d] = acc[d] * r;
+    }
+  }
+}
+
+// Thread 0, when the item's tiles are done: what the join has to know of it.
+__device__ __forceinline__ void um_record(const Kv4AttnParams& p, const KvItem& it, long long per) {
+  if (it.x0 != 0 || it.x1 == it.w) return;  // starts before, or is whole
+  KvRec r{};
+  r.r = it.rq.r;
+  r.h = it.h;
+  r.j = (int)it.j;
+  r.a = blockIdx.x;
+  r.n_first = r.parts = (int)((it.start + it.w - 1) / per) - (int)blockIdx.x + 1;
+  p.rec[blockIdx.x] = r;
 }
 
 template <int HD>
@@ -613,116 +730,76 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
       kv_item_at(p, x, c.req, c.req_start, c0);
       x.x0 = c0 - x.start;
       x.x1 = min(c1 - x.start, x.w);
-      c.item = x;
+      c.item[0] = x;
     }
   }
   __syncthreads();
 
+  // the roles; between two items all of them meet twice: when the item's tiles
+  // are done, and when the next item is known
   uint32_t g0 = 0;
   bool more = c.more;
-  for (uint32_t items = 0; more; ++items) {
-    const UmTiles tl = um_tiles(c.item);
-    if (warp < kUSoft) {
-      um_softmax<HD>(p, c, tmem, tl, g0);
-      __syncthreads();
-      if (tid == 0) {
-        const KvItem& it = c.item;
-        if (it.x1 < it.w && it.x0 == 0) {  // starts here and goes on
-          KvRec r{};
-          r.r = it.rq.r;
-          r.h = it.h;
-          r.j = (int)it.j;
-          r.a = blockIdx.x;
-          r.n_first = r.parts = (int)((it.start + it.w - 1) / per) - (int)blockIdx.x + 1;
-          p.rec[blockIdx.x] = r;
-        }
-      }
-    } else if (warp < kUSoft + kUSum) {
-      // sums: row x half of the dimensions
-      constexpr int N = HD / 2;
-      const int row = 32 * (warp & 3) + lane, half = (warp - kUSoft) >> 2;
-      const uint32_t col = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + GM::O + half * N;
-      float acc[N];
-#pragma unroll
-      for (int d = 0; d < N; ++d) acc[d] = 0.0f;
-      for (int i = 0; i < tl.n; ++i) {
-        const uint32_t g = g0 + i, st = g & 1, par = (g >> 1) & 1;
-        if (!um_wait(&c.pv_done[st], par, &c.abort)) break;
-        fence_after();
-        const float2 cr = c.corr[g & 3][row];
-        const float f = c.vinv[g & 7];
-        const uint32_t nan = __float_as_uint(cr.y);
-#pragma unroll
-        for (int d0 = 0; d0 < N; d0 += 32) {
-          float o[32];
-          tm_ld32(col + st * HD + d0, o);
-          tm_wait_ld(o);
-          const float bad = (nan >> ((half * N + d0) / 32)) & 1 ? NAN : 0.0f;
-          if (__any_sync(0xffffffffu, nan != 0))
-#pragma unroll
-            for (int d = 0; d < 32; ++d) o[d] += bad;
-#pragma unroll
-          for (int d = 0; d < 32; ++d) acc[d0 + d] = fmaf(acc[d0 + d], cr.x, o[d] * f);
-        }
-        fence_before();
-        mbar_arrive(&c.o_free[st]);
-      }
-      __syncthreads();
-      const KvItem& it = c.item;
-      const int ct = row / p.gsz, ch = row - ct * p.gsz;
-      if (ct < it.ntok && ch < it.nhead) {
-        const float2 ml = c.ml[row];
-        const bool whole = it.x0 == 0 && it.x1 == it.w;
-        const size_t at = ((size_t)blockIdx.x * 2 + (it.x0 > 0 ? 0 : 1)) * kKvUmmaRows + row;
-        const float r = !whole ? 1.0f : ml.y != 0.0f ? 1.0f / ml.y : 0.0f;
-        float* dst = whole ? p.out + (size_t)(it.rq.t0 + it.tok0 + ct) * p.out_stride +
-                                 (size_t)(it.h0 + ch) * HD
-                           : p.part_o + at * HD;
-        dst += half * N;
-        if (!whole && half == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = ml;
-        if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-#pragma unroll
-          for (int d = 0; d < N; d += 4)
-            *reinterpret_cast<float4*>(dst + d) =
-                make_float4(acc[d] * r, acc[d + 1] * r, acc[d + 2] * r, acc[d + 3] * r);
-        } else {
-#pragma unroll
-          for (int d = 0; d < N; ++d) dst[d] = acc[d] * r;
-        }
-      }
-    } else {
-      if (warp < kMmaWarp) {
-        um_values<HD>(p, c, sm, base, tl, g0);
-      } else {
-        if (lane == 0) um_mma<HD>(c, tmem, base, tl, g0, items);
-        __syncwarp();
-      }
-      __syncthreads();
-    }
+  UmTiles tl{};
+  int cur = 0;
+  auto next = [&]() {
     g0 += tl.n;
-    __syncthreads();
-    if (c.abort) break;
-    if (tid == 0) {
-      KvItem x = c.item;
-      c.more = x.start + x.w < c1 && kv_item_next(p, x);
-      if (c.more) {
-        x.x0 = 0;
-        x.x1 = min(c1 - x.start, x.w);
-        c.item = x;
-      }
-    }
+    cur ^= 1;
     __syncthreads();
     more = c.more;
-  }
-  if (c.abort && tid == 32 * kMmaWarp) {  // after a wait that gave up: let the MMAs end
-    mma_commit(&c.drain);
-    mbar_wait_timed(&c.drain, 0, &g_kv4_umma_status);
-  }
-  fence_before();
-  __syncthreads();
-  if (warp == 0) {
-    fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  };
+  if (warp < kUSoft) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kURegSoft));
+    while (more) {
+      tl = um_tiles(c.item[cur]);
+      um_softmax<HD>(p, c, c.item[cur], tmem, tl, g0);
+      __syncthreads();
+      if (tid == 0) {
+        KvItem x = c.item[cur];
+        um_record(p, x, per);
+        c.more = x.start + x.w < c1 && !c.abort && kv_item_next(p, x);
+        x.x0 = 0;
+        x.x1 = min(c1 - x.start, x.w);
+        c.item[cur ^ 1] = x;
+      }
+      next();
+    }
+    __syncthreads();
+    if (warp == 0) {
+      fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+  } else if (warp < kUSoft + kUSum) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kURegSum));
+    while (more) {
+      tl = um_tiles(c.item[cur]);
+      um_sums<HD>(p, c, c.item[cur], tmem, tl, g0);
+      next();
+    }
+    fence_before();
+    __syncthreads();
+  } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kURegVal));
+    while (more) {
+      tl = um_tiles(c.item[cur]);
+      um_values<HD>(p, c, c.item[cur], sm, base, tl, g0);
+      __syncthreads();
+      next();
+    }
+    __syncthreads();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kURegMma));
+    for (uint32_t items = 0; more; ++items) {
+      tl = um_tiles(c.item[cur]);
+      if (tid == 32 * kMmaWarp) um_mma<HD>(c, tmem, base, tl, g0, items);
+      __syncwarp();
+      __syncthreads();
+      next();
+    }
+    if (tid == 32 * kMmaWarp && c.abort) {  // after a wait that gave up: let the MMAs end
+      mma_commit(&c.drain);
+      mbar_wait_timed(&c.drain, 0, &g_kv4_umma_status);
+    }
+    __syncthreads();
   }
 }
 
