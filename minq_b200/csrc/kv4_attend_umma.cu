@@ -21,8 +21,8 @@
 //   warps 0-3    softmax: thread = row = TMEM lane. Reads S, moves the maximum
 //                only when a weight would exceed 2^4, writes P over S.
 //   warps 4-7    sums: thread = row. acc = acc * a + O.
-//   warps 8-15   values: raw tile -> Kh Kl, Vh Vl in 128-byte swizzled tiles;
-//                its first warp issues the bulk copies.
+//   warps 8-15   values: raw tile -> Kh Kl, Vh Vl in 128-byte swizzled tiles.
+//   warps 17-19  bulk copies, K's scales, V's scales.
 //   warp 16      one thread issues the MMAs: S of the next tile, then P V.
 // S, O and the K and V tiles are double buffered; TMEM: Qh Ql, 2 S, 2 O.
 // The order of dimensions inside S's contraction and of positions inside
@@ -49,8 +49,8 @@ constexpr int kUTile = 64;       // positions per tile
 constexpr int kUSoft = 4, kUSum = 4, kUVal = 8;  // warps of the roles
 constexpr int kUThreads = 32 * (kUSoft + kUSum + kUVal + 4);
 // Registers a thread: 96 at the launch (640 threads), then by role (each a
-// whole number of warpgroups): 120 + 176 + 2 x 72 + 40 <= 5 x 96.
-constexpr int kURegSoft = 120, kURegSum = 176, kURegVal = 72, kURegMma = 40;
+// whole number of warpgroups): 120 + 176 + 2 x 64 + 56 <= 5 x 96.
+constexpr int kURegSoft = 120, kURegSum = 176, kURegVal = 64, kURegMma = 56;
 static_assert(kURegSoft + kURegSum + 2 * kURegVal + kURegMma <= 5 * 96, "registers");
 constexpr int kUValThreads = 32 * kUVal;
 constexpr int kUExtra = 256;     // an item's start and end, in positions
@@ -71,15 +71,15 @@ struct UmGeom {
 struct UmCtl {
   float2 corr[4][kKvUmmaRows];  // per row: factor of its sum; bit b: block b becomes NaN
   float2 ml[kKvUmmaRows];
-  float kinv[4][kUTile];        // 1 / f_t of K
-  // value scales of the positions that exist (0: not, or not finite) as two f16 parts
-  uint32_t vscale[2][kUTile][4];
-  uint32_t vmax[2][kUVal];
-  float vinv[8];                // 2^-10 / f' of V
+  float kinv[8][kUTile];        // 1 / f_t of K
+  // scales of the positions that exist (0: not; V: or not finite) as two f16 parts
+  uint32_t kscale[kURaw][kUTile * 4], vscale[kURaw][kUTile * 4];
+  float vinv[16];               // 2^-10 / f' of V
   int ok[8];                    // runs of 16 positions that exist
-  uint32_t bad[8][kUVal];       // not finite value scales: bit (row of the warp) * NB + block
+  uint32_t bad[8][8];           // not finite value scales: word and bit of (position * NB + block)
   int raw_ok[kURaw];
-  uint64_t raw_full[kURaw], k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t raw_full[kURaw], raw_free[kURaw], scale_full[kURaw];
+  uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], o_free[2];
   uint64_t q_full, drain;
   uint32_t tmem;
   int abort, more, req;
@@ -96,58 +96,42 @@ __device__ __forceinline__ void fence_after() {
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-// K-major tile in the 128-byte swizzle layout, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128(uint32_t saddr) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Descriptor of a K-major tile in the 128-byte swizzle layout, 8-row groups
+// 1024 bytes apart: the low word (the address, which moves) and the high one.
+__device__ __forceinline__ uint32_t sw128_lo(uint32_t saddr) {
+  return ((saddr & 0x3FFFFu) >> 4) | (1u << 16);
 }
+constexpr uint32_t kSw128Hi = (1024u >> 4) | (1u << 14) | (2u << 29);
 // 16-byte chunk c (0..7) of row r.
 __device__ __forceinline__ uint32_t sw_chunk(int r, int c) {
   return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
 }
-// D (+)= A (TMEM) x B, kind::f16: A and B f16, K-major, D f32, M = 128, N = n.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, int n, uint32_t acc) {
+// D (+)= A (TMEM) x B, kind::f16: A and B f16, K-major, D f32, M = 128, N = n;
+// by the elected lane. The warp runs this together, so that addresses and
+// descriptors stay in uniform registers.
+__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d, uint32_t a, uint32_t b_lo, int n,
+                                       uint32_t acc) {
   const uint32_t idesc = (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "n"(kSw128Hi), "r"(idesc), "r"(acc), "r"(on)
       : "memory");
+}
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t on;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}"
+      : "=r"(on));
+  return on;
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    smem_u32(bar))
                : "memory");
 }
-// 32 lanes x 32 columns of 32-bit words (this warp's lane quarter).
-__device__ __forceinline__ void tm_ld32(uint32_t taddr, float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-// Wait for this thread's TMEM loads; the values pass through the asm so that no
-// use of them is scheduled before the wait.
-__device__ __forceinline__ void tm_wait_ld(float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
-                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
-                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
-}
-// 16 columns, waited for.
+// 32 lanes x 16 columns of 32-bit words (this warp's lane quarter), waited for.
 __device__ __forceinline__ void tm_ld16(uint32_t taddr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
@@ -159,16 +143,12 @@ __device__ __forceinline__ void tm_ld16(uint32_t taddr, float* v) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
-      "%29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() {
@@ -238,6 +218,10 @@ __device__ __forceinline__ void add_f2(float* x, const float* y) {
       : "f"(y[0]), "f"(y[1]));
 }
 
+// S's column (K's row in its tile) of position r of the tile: the place that
+// V's tile gives r in P V's contraction, so P can take S's place in TMEM.
+__device__ __forceinline__ int s_column(int r) { return (r & 7) * 8 + (r >> 3); }
+
 // The tiles of an item that this CTA takes.
 struct UmTiles {
   int first, n;
@@ -250,28 +234,29 @@ __device__ __forceinline__ UmTiles um_tiles(const KvItem& it) {
   return {a, max(b - a, 0)};
 }
 
-// Values role: all tiles of the item. g0: number of tiles that the CTA has done.
+// Copies: one warp, whose lanes 0..7 take a run of K or V each.
 template <int HD>
-__device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, const KvItem& it, uint8_t* sm,
-                                          uint32_t base, UmTiles tl, uint32_t g0) {
+__device__ __forceinline__ void um_copies(const Kv4AttnParams& p, UmCtl& c, const KvItem& it, uint8_t* sm,
+                                          UmTiles tl, uint32_t g0) {
   using GM = UmGeom<HD>;
-  constexpr int NB = GM::NB, ROW = GM::ROW;
-  const int dt = threadIdx.x - 32 * (kUSoft + kUSum), lane = dt & 31, w = dt >> 5;
-  const int lim_max = it.lim_max;
-  // copies: lanes 0..7 of the first warp take a run of K or V each
-  const int run = lane & 3;
-  const uint8_t* side = (lane & 4 ? p.v_pages : p.k_pages) + ((size_t)it.kvh << p.page_shift) * ROW;
-  const size_t page_bytes = ((size_t)p.nkv << p.page_shift) * ROW;
+  const int lane = threadIdx.x & 31, run = lane & 3, lim_max = it.lim_max;
+  const uint8_t* side =
+      (lane & 4 ? p.v_pages : p.k_pages) + ((size_t)it.kvh << p.page_shift) * GM::ROW;
+  const size_t page_bytes = ((size_t)p.nkv << p.page_shift) * GM::ROW;
   const int* tab = p.table + (size_t)it.rq.r * p.table_stride;
-  auto load_id = [&](int i) {
+  auto load_id = [&](int i) {  // checked where it is used, when it has come
     const int pos = (tl.first + i) * kUTile + 16 * run;
-    int id = -1;
-    if (lane < 8 && i < tl.n && pos < lim_max) id = tab[pos >> p.page_shift];
-    return id < p.n_pages ? id : -1;
+    return lane < 8 && i < tl.n && pos < lim_max ? tab[pos >> p.page_shift] : -1;
   };
-  auto issue = [&](int i, int id) {
-    const uint32_t st = (g0 + i) % kURaw;
-    const uint32_t have = __ballot_sync(0xffffffffu, id >= 0) & 15u;
+  int id = load_id(0), i = 0;
+  bool alive = true;
+  for (; i < tl.n; ++i) {
+    const int id_next = load_id(i + 1);
+    const uint32_t g = g0 + i, st = g % kURaw;
+    if (g >= kURaw) alive = um_wait(&c.raw_free[st], (g / kURaw - 1) & 1, &c.abort);
+    if (!alive) break;
+    const bool on = id >= 0 && id < p.n_pages;
+    const uint32_t have = __ballot_sync(0xffffffffu, on) & 15u;
     if (lane == 0) {
       c.raw_ok[st] = (int)have;
       if (have)
@@ -279,81 +264,105 @@ __device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, cons
       else
         mbar_arrive(&c.raw_full[st]);
     }
-    __syncwarp();
-    if (id >= 0) {
+    __syncwarp();  // the bytes are expected before they can come
+    if (on) {
       const int row = ((tl.first + i) * kUTile + 16 * run) & ((1 << p.page_shift) - 1);
       bulk_g2s(sm + GM::R + st * GM::RAW + (lane >> 2) * 4 * GM::RUN + run * GM::RUN,
-               side + (size_t)id * page_bytes + (size_t)row * ROW, GM::RUN, &c.raw_full[st]);
+               side + (size_t)id * page_bytes + (size_t)row * GM::ROW, GM::RUN, &c.raw_full[st]);
     }
-  };
-  int id = -1, issued = 0, landed = 0;
-  if (w == 0) {
-    for (; issued < min(tl.n, kURaw - 1); ++issued) issue(issued, load_id(issued));
-    id = load_id(kURaw - 1);
+    id = id_next;
   }
-  bool alive = true;  // no wait gave up; else only the barrier of the role is kept up
-  // K: (position kr, block kb) of the thread; V: eight positions pg + 8 i and
-  // four dimensions of block vb
-  const bool k_on = HD == 128 || dt < 128;
-  const int kr = (HD == 128 ? dt : dt & 127) / NB, kb = dt % NB;
-  const int vt = HD == 128 ? dt : dt - 128, pg = vt & 7, dq = vt >> 3, vb = dq >> 3;
+  if (!alive)  // let the copies in flight end
+    for (int k = i > kURaw ? i - kURaw : 0; k < i; ++k)
+      mbar_wait_timed(&c.raw_full[(g0 + k) % kURaw], ((g0 + k) / kURaw) & 1, &g_kv4_umma_status);
+}
+
+// Scales: one warp for K's, one for V's.
+template <int HD, bool V>
+__device__ __forceinline__ void um_scales(UmCtl& c, const KvItem& it, const uint8_t* sm, UmTiles tl,
+                                          uint32_t g0) {
+  using GM = UmGeom<HD>;
+  constexpr int NB = GM::NB, N = kUTile * NB / 32;
+  const int lane = threadIdx.x & 31, lim_max = it.lim_max;
   for (int i = 0; i < tl.n; ++i) {
-    const uint32_t g = g0 + i, par = g >> 1, st = g & 1;
-    alive = alive && um_wait(&c.raw_full[g % kURaw], (g / kURaw) & 1, &c.abort);
-    if (alive) landed = i + 1;
-    const int pos0 = (tl.first + i) * kUTile, ok = c.raw_ok[g % kURaw];
-    const uint8_t* rk = sm + GM::R + (g % kURaw) * GM::RAW;
+    const uint32_t g = g0 + i, st = g % kURaw;
+    if (!um_wait(&c.raw_full[st], (g / kURaw) & 1, &c.abort)) return;
+    const int pos0 = (tl.first + i) * kUTile, ok = c.raw_ok[st];
+    const uint8_t* raw = sm + GM::R + st * GM::RAW + (V ? 4 * GM::RUN : 0);
+    auto scale = [&](int j) {
+      const int x = lane + 32 * j, row = x / NB;
+      const bool there = ((ok >> (row >> 4)) & 1) && pos0 + row < lim_max;
+      return there ? *reinterpret_cast<const float*>(raw + x * kQ4Bytes) : 0.0f;
+    };
+    if (V) {
+      uint32_t top = 0;
+#pragma unroll 2
+      for (int j = 0; j < N; ++j) {
+        const float d = scale(j);
+        const bool fin = fabsf(d) < INFINITY;
+        const uint32_t bad = __ballot_sync(0xffffffffu, !fin);
+        if (lane == 0) c.bad[g & 7][j] = bad;
+        top = max(top, fin ? __float_as_uint(fabsf(d)) : 0u);
+      }
+      const uint32_t e = up_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, top)));
+      if (lane == 0) {
+        c.vinv[g & 15] = __uint_as_float((254u - e) << 23) * 0.0009765625f;
+        c.ok[g & 7] = ok;
+      }
+#pragma unroll 2
+      for (int j = 0; j < N; ++j) {
+        const float d = scale(j);
+        c.vscale[st][lane + 32 * j] =
+            scale_parts(fabsf(d) < INFINITY ? d * __uint_as_float(e << 23) : 0.0f);
+      }
+    } else {
+#pragma unroll 2
+      for (int j = 0; j < N; ++j) {
+        const float d = scale(j);
+        float m = fabsf(d) < INFINITY ? fabsf(d) : 0.0f;
+#pragma unroll
+        for (int o = 1; o < NB; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const uint32_t e = up_exponent(m);
+        const int x = lane + 32 * j;
+        c.kscale[st][x] = scale_parts(d * __uint_as_float(e << 23));
+        if (x % NB == 0) c.kinv[g & 7][s_column(x / NB)] = __uint_as_float((254u - e) << 23);
+      }
+    }
+    mbar_arrive(&c.scale_full[st]);
+  }
+}
+
+// Values role: the item's tiles, from codes and scales to f16 parts.
+template <int HD>
+__device__ __forceinline__ void um_values(UmCtl& c, const uint8_t* sm, uint32_t base, UmTiles tl,
+                                          uint32_t g0) {
+  using GM = UmGeom<HD>;
+  constexpr int NB = GM::NB, ROW = GM::ROW;
+  const int dt = threadIdx.x - 32 * (kUSoft + kUSum), lane = dt & 31;
+  // K: block kb of position kr; V: positions pg + 8 i, four dimensions of block
+  // vb. With head_dim 64 half of the threads have K, the other half V.
+  const bool k_on = HD == 128 || dt < 128, v_on = HD == 128 || dt >= 128;
+  const int kt = HD == 128 ? dt : dt & 127, kr = kt / NB, kb = kt % NB;
+  const int pg = kt & 7, dq = kt >> 3, vb = dq >> 3;
+  for (int i = 0; i < tl.n; ++i) {
+    const uint32_t g = g0 + i, par = g >> 1, st = g & 1, rs = g % kURaw;
+    if (!um_wait(&c.raw_full[rs], (g / kURaw) & 1, &c.abort) ||
+        !um_wait(&c.scale_full[rs], (g / kURaw) & 1, &c.abort))
+      return;
+    const uint8_t* rk = sm + GM::R + rs * GM::RAW;
     const uint8_t* rv = rk + 4 * GM::RUN;
-    const uint8_t* blk = rk + kr * ROW + kb * kQ4Bytes;
-    const bool there = k_on && ((ok >> (kr >> 4)) & 1) && pos0 + kr < lim_max;
-    const float dk = there ? *reinterpret_cast<const float*>(blk) : 0.0f;
-    const float dv = there ? *reinterpret_cast<const float*>(rv + kr * ROW + kb * kQ4Bytes) : 0.0f;
-    const bool fin = fabsf(dv) < INFINITY;
-    uint32_t code[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) code[x] = *reinterpret_cast<const uint32_t*>(blk + 4 + 4 * x);
-    // what the other roles read of tile g - 2 (K) and of g - 4, g - 8 is done with
-    if (alive && g >= 2) alive = um_wait(&c.s_full[st], (par - 1) & 1, &c.abort);
-    if (!alive) {
-      asm volatile("bar.sync 2, %0;" ::"r"(kUValThreads) : "memory");
-      asm volatile("bar.sync 3, %0;" ::"r"(kUValThreads) : "memory");
-      continue;
-    }
-    const uint32_t bad = __ballot_sync(0xffffffffu, there && !fin);
-    const uint32_t vm = __reduce_max_sync(0xffffffffu, fin ? __float_as_uint(fabsf(dv)) : 0u);
-    if (lane == 0) {
-      c.bad[g & 7][w] = bad;
-      c.vmax[st][w] = vm;
-    }
-    asm volatile("bar.sync 2, %0;" ::"r"(kUValThreads) : "memory");
-    if (w == 0) {  // everyone is done with raw tile g - 1
-      if (issued < tl.n) issue(issued++, id);
-      id = load_id(i + kURaw);
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int x = 0; x < kUVal; ++x) top = max(top, c.vmax[st][x]);
-    const uint32_t ve = up_exponent(__uint_as_float(top));
-    if (dt == 0) {
-      c.vinv[g & 7] = __uint_as_float((254u - ve) << 23) * 0.0009765625f;
-      c.ok[g & 7] = ok;
-    }
-    float m = fabsf(dk) < INFINITY ? fabsf(dk) : 0.0f;
-#pragma unroll
-    for (int o = 1; o < NB; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t fe = up_exponent(m);
+    const uint32_t d = c.kscale[rs][kt];
+    // S of tile g - 2 has read this buffer
+    if (g >= 2 && !um_wait(&c.s_full[st], (par - 1) & 1, &c.abort)) return;
     if (k_on) {
-      c.vscale[st][kr][kb] = scale_parts((fin ? dv : 0.0f) * __uint_as_float(ve << 23));
-      if (kb == 0) c.kinv[g & 3][kr] = __uint_as_float((254u - fe) << 23);
-      const uint32_t d = scale_parts(dk * __uint_as_float(fe << 23));
       const uint32_t dh = __byte_perm(d, d, 0x1010), dl = __byte_perm(d, d, 0x3232);
       const uint32_t tile = base + GM::K + st * 2 * GM::KT + (kb >> 1) * kUTile * 128;
-#pragma unroll
+#pragma unroll 1
       for (int x = 0; x < 4; ++x) {
         uint32_t y[4], v[4];
-        codes4(code[x], y);
+        codes4(*reinterpret_cast<const uint32_t*>(rk + kt * kQ4Bytes + 4 + 4 * x), y);
         // blocks 2, 3: chunks in another order, against bank conflicts
-        const uint32_t at = tile + sw_chunk(kr, 4 * (kb & 1) + (x ^ (kb & 2)));
+        const uint32_t at = tile + sw_chunk(s_column(kr), 4 * (kb & 1) + (x ^ (kb & 2)));
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = mul2(y[e], dh);
         sts16(at, v);
@@ -364,27 +373,28 @@ __device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, cons
     }
     fence_async_smem();
     mbar_arrive(&c.k_full[st]);
-    asm volatile("bar.sync 3, %0;" ::"r"(kUValThreads) : "memory");
-    if (g >= 2) alive = um_wait(&c.pv_done[st], (par - 1) & 1, &c.abort);
-    if (!alive) continue;
-    if (HD == 128 || dt >= 128) {
-      uint32_t hi[4][4], lo[4][4];  // [dimension][pair of positions]
+    uint32_t hi[4][4], lo[4][4];  // [dimension][pair of positions]
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r0 = pg + 16 * q;
-        const uint8_t* v0 = rv + r0 * ROW + vb * kQ4Bytes + 4 + 2 * (dq & 7);
-        const uint32_t x0 = *reinterpret_cast<const uint16_t*>(v0);
-        const uint32_t x1 = *reinterpret_cast<const uint16_t*>(v0 + 8 * ROW);
-        const uint32_t d0 = c.vscale[st][r0][vb], d1 = c.vscale[st][r0 + 8][vb];
-        const uint32_t dh = __byte_perm(d0, d1, 0x5410), dl = __byte_perm(d0, d1, 0x7632);
-        uint32_t y[4];
-        codes4(__byte_perm(x0, x1, 0x5410), y);
+    for (int q = 0; q < 4; ++q) {
+      const int r0 = pg + 16 * q;
+      const uint8_t* v0 = rv + r0 * ROW + vb * kQ4Bytes + 4 + 2 * (dq & 7);
+      const uint32_t x0 = *reinterpret_cast<const uint16_t*>(v0);
+      const uint32_t x1 = *reinterpret_cast<const uint16_t*>(v0 + 8 * ROW);
+      const uint32_t d0 = c.vscale[rs][r0 * NB + vb], d1 = c.vscale[rs][(r0 + 8) * NB + vb];
+      const uint32_t dh = __byte_perm(d0, d1, 0x5410), dl = __byte_perm(d0, d1, 0x7632);
+      uint32_t y[4];
+      codes4(__byte_perm(x0, x1, 0x5410), y);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          hi[e][q] = mul2(y[e], dh);
-          lo[e][q] = mul2(y[e], dl);
-        }
+      for (int e = 0; e < 4; ++e) {
+        hi[e][q] = mul2(y[e], dh);
+        lo[e][q] = mul2(y[e], dl);
       }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&c.raw_free[rs]);
+    // P V of tile g - 2 has read this buffer
+    if (g >= 2 && !um_wait(&c.pv_done[st], (par - 1) & 1, &c.abort)) return;
+    if (v_on) {
       const uint32_t tile = base + GM::V + st * 2 * GM::KT;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -396,10 +406,6 @@ __device__ __forceinline__ void um_values(const Kv4AttnParams& p, UmCtl& c, cons
     fence_async_smem();
     mbar_arrive(&c.v_full[st]);
   }
-  if (w == 0)  // after a wait that gave up: let the copies in flight end
-    for (; landed < issued; ++landed)
-      mbar_wait_timed(&c.raw_full[(g0 + landed) % kURaw], ((g0 + landed) / kURaw) & 1,
-                      &g_kv4_umma_status);
 }
 
 // First of the eight dimensions d of chunk x of S's contraction (4 columns of
@@ -449,19 +455,19 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
     cn = fabsf(p.scale) * 1.4426950408889634f * (1.0f / f);
     if (cn == 0.0f) cn = 1.4e-45f;  // -inf stays masked
     if (p.scale < 0.0f) f = -f;
+#pragma unroll 1
+    for (int x0 = 0; x0 < HD / 2; x0 += 16) {
+      uint32_t hi[16], lo[16];
 #pragma unroll
-    for (int x0 = 0; x0 < HD / 2; x0 += 32) {
-      uint32_t hi[32], lo[32];
-#pragma unroll
-      for (int x = 0; x < 32; x += 4) {
+      for (int x = 0; x < 16; x += 4) {
         float v[8];
         load8(q_dim<HD>((x0 + x) / 4), v);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           split2(on ? v[e] * f : 0.0f, on ? v[e + 4] * f : 0.0f, hi[x + e], lo[x + e]);
       }
-      tm_st32(tlane + GM::QH + x0, hi);
-      tm_st32(tlane + GM::QL + x0, lo);
+      tm_st16(tlane + GM::QH + x0, hi);
+      tm_st16(tlane + GM::QL + x0, lo);
     }
     tm_wait_st();
     fence_before();
@@ -472,26 +478,33 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
     const uint32_t g = g0 + i, st = g & 1;
     if (!um_wait(&c.s_full[st], (g >> 1) & 1, &c.abort)) return;
     fence_after();
-    float s[kUTile];
-    tm_ld32(tlane + GM::S + st * kUTile, s);
-    tm_ld32(tlane + GM::S + st * kUTile + 32, s + 32);
-    tm_wait_ld(s);
-    tm_wait_ld(s + 32);
     const int pos0 = (tl.first + i) * kUTile, ok = c.ok[g & 7];
+    const bool all = __all_sync(0xffffffffu, ok == 15 && pos0 + kUTile <= lim);
+    // 16 columns of S at a time, scaled and masked; column e of chunk x is
+    // position 2 x + e / 8 + 8 (e mod 8)
+    auto load = [&](int x, float* s) {
+      tm_ld16(tlane + GM::S + st * kUTile + 16 * x, s);
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(&c.kinv[g & 7][16 * x + j]);
+        mul_f2(s + j, k.x, k.y);
+        mul_f2(s + j + 2, k.z, k.w);
+      }
+      if (!all) {
+        const int left = lim - pos0 - 2 * x;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((ok >> ((e & 7) >> 1)) & 1) || (e >> 3) + 8 * (e & 7) >= left) s[e] = -INFINITY;
+      }
+    };
     float top = -INFINITY;
+#pragma unroll 1
+    for (int x = 0; x < kUTile / 16; ++x) {
+      float s[16];
+      load(x, s);
 #pragma unroll
-    for (int j = 0; j < kUTile; j += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(&c.kinv[g & 3][j]);
-      mul_f2(s + j, k.x, k.y);
-      mul_f2(s + j + 2, k.z, k.w);
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
     }
-    if (!__all_sync(0xffffffffu, ok == 15 && pos0 + kUTile <= lim)) {
-#pragma unroll
-      for (int j = 0; j < kUTile; ++j)
-        if (!((ok >> (j >> 4)) & 1) || pos0 + j >= lim) s[j] = -INFINITY;
-    }
-#pragma unroll
-    for (int j = 0; j < kUTile; ++j) top = fmaxf(top, s[j]);
     top = top == -INFINITY ? top : top * cn;
     float a = 1.0f;
     if (top > m + 4.0f) {  // also the first that is seen
@@ -501,26 +514,25 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
     }
     const float off = m == -INFINITY ? 0.0f : 10.0f - m;
     float sum[2] = {0.0f, 0.0f};
+#pragma unroll 1
+    for (int x = 0; x < kUTile / 16; ++x) {
+      float s[16];
+      load(x, s);
+      uint32_t part[16];  // eight columns of high, eight of low parts in S's place
 #pragma unroll
-    for (int j = 0; j < kUTile; j += 2) {
-      fma_f2(s + j, cn, off, off);
-      s[j] = ex2(s[j]);
-      s[j + 1] = ex2(s[j + 1]);
-      add_f2(sum, s + j);
+      for (int e = 0; e < 16; e += 2) {
+        fma_f2(s + e, cn, off, off);
+        s[e] = ex2(s[e]);
+        s[e + 1] = ex2(s[e + 1]);
+        add_f2(sum, s + e);
+        split2(s[e], s[e + 1], part[e / 2], part[e / 2 + 8]);
+      }
+      tm_st16(tlane + GM::S + st * kUTile + 16 * x, part);
     }
     l += sum[0] + sum[1];
-    // P's column x holds positions (x / 4) + 16 (x mod 4) and 8 further on
-    uint32_t hi[32], lo[32];
-#pragma unroll
-    for (int x = 0; x < 32; ++x) {
-      const int j = (x >> 2) + 16 * (x & 3);
-      split2(s[j], s[j + 8], hi[x], lo[x]);
-    }
-    tm_st32(tlane + GM::S + st * kUTile, hi);
-    tm_st32(tlane + GM::S + st * kUTile + 32, lo);
     uint32_t nan = 0, any = 0;
 #pragma unroll
-    for (int x = 0; x < kUVal; ++x) any |= c.bad[g & 7][x];
+    for (int x = 0; x < 2 * NB; ++x) any |= c.bad[g & 7][x];
     if (any) {
       constexpr int PER = 32 / NB;  // positions of a word
       for (int x = 0; x < kUTile / PER; ++x)
@@ -535,45 +547,51 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
   c.ml[row] = make_float2(l == 0.0f ? -3.0e38f : m, l * 0.0009765625f);
 }
 
-// The thread that issues the MMAs.
+// The warp that issues the MMAs (one lane of it does).
 template <int HD>
 __device__ __forceinline__ void um_mma(UmCtl& c, uint32_t tmem, uint32_t base, UmTiles tl, uint32_t g0,
                                        uint32_t items) {
   using GM = UmGeom<HD>;
-  if (!um_wait1(&c.q_full, items & 1, &c.abort)) return;
+  const uint32_t on = elect_lane();
+  tmem = __shfl_sync(0xffffffffu, tmem, 0);
+  g0 = __shfl_sync(0xffffffffu, g0, 0);
+  const int n = __shfl_sync(0xffffffffu, tl.n, 0);
+  if (!um_wait(&c.q_full, items & 1, &c.abort)) return;
   auto scores = [&](int i) {
     const uint32_t g = g0 + i, st = g & 1, d = tmem + GM::S + st * kUTile;
-    if (!um_wait1(&c.k_full[st], (g >> 1) & 1, &c.abort)) return false;
+    const uint32_t kt = sw128_lo(base + GM::K + st * 2 * GM::KT);
+    if (!um_wait(&c.k_full[st], (g >> 1) & 1, &c.abort)) return false;
     fence_after();
-    const uint32_t kt = base + GM::K + st * 2 * GM::KT;
     // the small parts first: what the accumulation truncates next to them is nothing
 #pragma unroll
     for (int part = 0; part < 3; ++part)
 #pragma unroll
-      for (int j = 0; j < HD / 16; ++j) {
-        const uint32_t a = tmem + (part == 0 ? GM::QL : GM::QH) + 8 * j;
-        const uint32_t b = kt + (part == 1 ? GM::KT : 0) + (j >> 2) * kUTile * 128 + (j & 3) * 32;
-        mma_ts(d, a, sw128(b), kUTile, part > 0 || j > 0);
-      }
-    mma_commit(&c.s_full[st]);
+      for (int j = 0; j < HD / 16; ++j)
+        mma_ts(on, d, tmem + (part == 0 ? GM::QL : GM::QH) + 8 * j,
+               kt + (((part == 1 ? GM::KT : 0) + (j >> 2) * kUTile * 128 + (j & 3) * 32) >> 4), kUTile,
+               part | j);
+    if (on) mma_commit(&c.s_full[st]);
+    __syncwarp();
     return true;
   };
-  if (tl.n > 0 && !scores(0)) return;
-  for (int i = 0; i < tl.n; ++i) {
-    if (i + 1 < tl.n && !scores(i + 1)) return;
+  if (n > 0 && !scores(0)) return;
+  for (int i = 0; i < n; ++i) {
+    if (i + 1 < n && !scores(i + 1)) return;
     const uint32_t g = g0 + i, st = g & 1, par = (g >> 1) & 1;
-    if (!um_wait1(&c.p_full[st], par, &c.abort) || !um_wait1(&c.v_full[st], par, &c.abort)) return;
-    if (g >= 2 && !um_wait1(&c.o_free[st], par ^ 1, &c.abort)) return;
+    const uint32_t a = tmem + GM::S + st * kUTile, d = tmem + GM::O + st * HD;
+    const uint32_t vt = sw128_lo(base + GM::V + st * 2 * GM::KT);
+    if (!um_wait(&c.v_full[st], par, &c.abort)) return;
+    if (g >= 2 && !um_wait(&c.o_free[st], par ^ 1, &c.abort)) return;
+    if (!um_wait(&c.p_full[st], par, &c.abort)) return;
     fence_after();
-    const uint32_t vt = base + GM::V + st * 2 * GM::KT, d = tmem + GM::O + st * HD;
 #pragma unroll
     for (int part = 0; part < 3; ++part)
 #pragma unroll
-      for (int j = 0; j < kUTile / 16; ++j) {
-        const uint32_t a = tmem + GM::S + st * kUTile + (part == 0 ? 32 : 0) + 8 * j;
-        mma_ts(d, a, sw128(vt + (part == 1 ? GM::KT : 0) + j * 32), HD, part > 0 || j > 0);
-      }
-    mma_commit(&c.pv_done[st]);
+      for (int j = 0; j < kUTile / 16; ++j)
+        mma_ts(on, d, a + (part == 0 ? 8 : 0) + 16 * j, vt + (((part == 1 ? GM::KT : 0) + j * 32) >> 4), HD,
+               part | j);
+    if (on) mma_commit(&c.pv_done[st]);
+    __syncwarp();
   }
 }
 
@@ -592,7 +610,7 @@ __device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const 
     if (!um_wait(&c.pv_done[st], (g >> 1) & 1, &c.abort)) break;
     fence_after();
     const float2 cr = c.corr[g & 3][row];
-    const float f = c.vinv[g & 7];
+    const float f = c.vinv[g & 15];
     const uint32_t nan = __float_as_uint(cr.y);
 #pragma unroll
     for (int d0 = 0; d0 < HD; d0 += 16) {
@@ -655,7 +673,11 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
 
   if (warp == 0) {
     if (lane == 0) {
-      for (int i = 0; i < kURaw; ++i) mbar_init(&c.raw_full[i], 1);
+      for (int i = 0; i < kURaw; ++i) {
+        mbar_init(&c.raw_full[i], 1);
+        mbar_init(&c.raw_free[i], kUVal);
+        mbar_init(&c.scale_full[i], 64);
+      }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&c.k_full[i], kUValThreads);
         mbar_init(&c.v_full[i], kUValThreads);
@@ -781,7 +803,7 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kURegVal));
     while (more) {
       tl = um_tiles(c.item[cur]);
-      um_values<HD>(p, c, c.item[cur], sm, base, tl, g0);
+      um_values<HD>(c, sm, base, tl, g0);
       __syncthreads();
       next();
     }
@@ -790,7 +812,10 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kURegMma));
     for (uint32_t items = 0; more; ++items) {
       tl = um_tiles(c.item[cur]);
-      if (tid == 32 * kMmaWarp) um_mma<HD>(c, tmem, base, tl, g0, items);
+      if (warp == kMmaWarp) um_mma<HD>(c, tmem, base, tl, g0, items);
+      if (warp == kMmaWarp + 1) um_copies<HD>(p, c, c.item[cur], sm, tl, g0);
+      if (warp == kMmaWarp + 2) um_scales<HD, false>(c, c.item[cur], sm, tl, g0);
+      if (warp == kMmaWarp + 3) um_scales<HD, true>(c, c.item[cur], sm, tl, g0);
       __syncwarp();
       __syncthreads();
       next();
