@@ -911,7 +911,11 @@ constexpr int kKvJoinAlone = 16;  // pieces
 constexpr int kKvJoinRecs = 16;   // most pieces that a block looks through
 template <int HD>
 __global__ void __launch_bounds__(kKvJoinWarps * 32)
-    kv4_join_kernel(const __grid_constant__ Kv4AttnParams p) {
+    kv4_join_kernel(const __grid_constant__ Kv4AttnParams p0, const __grid_constant__ Kv4AttnParams p1) {
+  // the first p0.join_blocks blocks have p0's pieces, the others p1's
+  const bool second = (int)blockIdx.x >= p0.join_blocks;
+  const Kv4AttnParams& p = second ? p1 : p0;
+  const int block = second ? blockIdx.x - p0.join_blocks : blockIdx.x;
   constexpr int PER = HD / 32;  // values per lane
   __shared__ float s_o[kKvJoinWarps][HD];
   __shared__ float s_l[kKvJoinWarps];
@@ -922,7 +926,7 @@ __global__ void __launch_bounds__(kKvJoinWarps * 32)
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp == 0) {  // the items that there are, in order
-    const int c = blockIdx.x * p.join_pieces + lane;
+    const int c = block * p.join_pieces + lane;
     KvRec rec{};
     if (lane < p.join_pieces && c < p.n_piece) rec = p.rec[c];
     const uint32_t some = __ballot_sync(0xffffffffu, rec.parts > 0);
@@ -1025,25 +1029,20 @@ KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_
   KvPlan k{};
   if ((hd != 64 && hd != 128) || n_kv == 0 || n_req == 0) return k;
   const size_t G = n_heads / n_kv;
-  k.nt = G > 8 || n_tokens > n_req ? 2 : 1;
+  // With kKvUmmaMin rows a request and more, the chunks are the tcgen05 kernel's and what
+  // is left for the other one are mostly single tokens.
+  const size_t gsz = G < (size_t)kKvUmmaRows ? G : kKvUmmaRows;
+  const bool chunks = n_tokens > n_req && n_tokens * gsz >= kKvUmmaMin;
+  const bool single = n_tokens <= n_req || n_tokens * gsz >= kKvUmmaMin * n_req;
+  k.nt = G > 8 || !single ? 2 : 1;
   k.split = k.nt == 1 && G <= 4;
   k.n_cta = sm_count() * (k.nt == 1 ? 4 : 2);
   k.ws = (size_t)k.n_cta * kKvWarps * (2 * 8 * k.nt * (hd + 2) * 4 + sizeof(KvRec));
-  const size_t gsz = G < (size_t)kKvUmmaRows ? G : kKvUmmaRows;
-  if (n_tokens > n_req && n_tokens * gsz >= kKvUmmaMin) {
+  if (chunks) {
     k.umma_lo = (int)((kKvUmmaMin + gsz - 1) / gsz);
     k.umma_ws = kv4_umma_workspace(hd);
   }
   return k;
-}
-
-// join_pieces: pieces that a block looks through; spread: blocks that share their columns.
-template <int HD>
-minq_status launch_kv4_join(Kv4AttnParams p, int join_pieces, int spread, cudaStream_t s) {
-  p.join_pieces = join_pieces;
-  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3((p.n_piece + join_pieces - 1) / join_pieces, spread),
-                         dim3(kKvJoinWarps * 32), 0, s, p));
-  return MINQ_OK;
 }
 
 template <int HD, int NT, bool SPLIT>
@@ -1052,12 +1051,28 @@ minq_status launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
   MINQ_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(kv4_attend_kernel<HD, NT, SPLIT>), GM::SMEM));
   MINQ_CUDA_TRY(launch_k(kv4_attend_kernel<HD, NT, SPLIT>, dim3(p.n_piece / kKvWarps), dim3(kKvWarps * 32),
                          GM::SMEM, s, p));
+  return MINQ_OK;
+}
+
+// One launch joins the pieces of both kernels (u: null where the tcgen05 kernel did not run).
+template <int HD>
+minq_status launch_kv4_join(Kv4AttnParams p, const Kv4AttnParams* u, cudaStream_t s) {
   // With few items (of one token each) every one has many pieces: their columns
   // are spread over blocks, and few blocks look for them. With many there are
   // some in every CTA. Measured (join alone, us): 2 x 131071 positions of 2 kv
   // heads 18 this way and 20 the other, 64 x 8192 of 8 kv heads 18 and 9.
   const bool few = (size_t)p.n_req * p.nkv * p.hgroups * 4 < (size_t)p.n_piece / kKvWarps;
-  return launch_kv4_join<HD>(p, few ? kKvJoinRecs : kKvWarps, few ? 8 : (p.tpt * p.gsz + 3) / 4, s);
+  p.join_pieces = few ? kKvJoinRecs : kKvWarps;
+  p.join_blocks = (p.n_piece + p.join_pieces - 1) / p.join_pieces;
+  int blocks = p.join_blocks, spread = few ? 8 : (p.tpt * p.gsz + 3) / 4;
+  Kv4AttnParams v = u ? *u : p;
+  if (u) {
+    v.join_pieces = 1;
+    blocks += v.n_piece;
+    spread = kKvUmmaSpread;
+  }
+  MINQ_CUDA_TRY(launch_k(kv4_join_kernel<HD>, dim3(blocks, spread), dim3(kKvJoinWarps * 32), 0, s, p, v));
+  return MINQ_OK;
 }
 
 }  // namespace
@@ -1144,13 +1159,11 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
     p.hgroups = (G + p.gsz - 1) / p.gsz;
     p.tpt = most / p.gsz;
     cudaStream_t s = (cudaStream_t)stream;
+    Kv4AttnParams u = p;
     if (plan.umma_lo) {
-      Kv4AttnParams u = p;
       u.n_lo = plan.umma_lo;
       u.n_hi = INT_MAX;
       MINQ_TRY(launch_kv4_umma(u, static_cast<uint8_t*>(workspace) + plan.ws, s));
-      MINQ_TRY(head_dim == 64 ? launch_kv4_join<64>(u, 1, kKvUmmaSpread, s)
-                              : launch_kv4_join<128>(u, 1, kKvUmmaSpread, s));
     }
     p.n_lo = 1;
     p.n_hi = plan.umma_lo ? plan.umma_lo - 1 : INT_MAX;
@@ -1159,13 +1172,16 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
     p.rec = static_cast<KvRec*>(workspace);
     p.part_o = reinterpret_cast<float*>(p.rec + p.n_piece);
     p.part_ml = p.part_o + (size_t)p.n_piece * 2 * cols * head_dim;
-    if (head_dim == 64)
-      return plan.split     ? launch_kv4_attend<64, 1, true>(p, s)
-             : plan.nt == 1 ? launch_kv4_attend<64, 1, false>(p, s)
-                            : launch_kv4_attend<64, 2, false>(p, s);
-    return plan.split     ? launch_kv4_attend<128, 1, true>(p, s)
-           : plan.nt == 1 ? launch_kv4_attend<128, 1, false>(p, s)
-                          : launch_kv4_attend<128, 2, false>(p, s);
+    if (head_dim == 64) {
+      MINQ_TRY((plan.split     ? launch_kv4_attend<64, 1, true>(p, s)
+               : plan.nt == 1 ? launch_kv4_attend<64, 1, false>(p, s)
+                              : launch_kv4_attend<64, 2, false>(p, s)));
+      return launch_kv4_join<64>(p, plan.umma_lo ? &u : nullptr, s);
+    }
+    MINQ_TRY((plan.split     ? launch_kv4_attend<128, 1, true>(p, s)
+             : plan.nt == 1 ? launch_kv4_attend<128, 1, false>(p, s)
+                            : launch_kv4_attend<128, 2, false>(p, s)));
+    return launch_kv4_join<128>(p, plan.umma_lo ? &u : nullptr, s);
   }
   const size_t rows = n_tokens * n_heads;
   MINQ_CUDA_TRY(launch_k(kv4_attend_rows_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0,

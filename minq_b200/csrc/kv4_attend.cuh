@@ -36,7 +36,7 @@ struct Kv4AttnParams {
   // columns of a tile (room for), heads per tile, head tiles per kv head, tokens per tile
   int cols, gsz, hgroups, tpt;
   int n_piece;       // pieces of the line
-  int join_pieces;   // those that a block of the join looks through
+  int join_pieces, join_blocks;  // those that a block of the join looks through, its blocks
   float* part_o;     // [n_piece][2][cols][hd] unnormalised partial outputs
   float* part_ml;    // [n_piece][2][cols][2] their maxima and sums
   KvRec* rec;        // [n_piece]

@@ -18,8 +18,9 @@
 // towards zero, and over thousands of positions that would show.
 //
 // One CTA per SM, four roles that work on different tiles at the same time:
-//   warps 0-3    softmax: thread = row = TMEM lane. Reads S, moves the maximum
-//                only when a weight would exceed 2^4, writes P over S.
+//   warps 0-3    softmax: thread = row = TMEM lane. One pass over S in steps of
+//                16 columns: moves the maximum only when a weight would exceed
+//                2^4 (and then scales what it has written), writes P over S.
 //   warps 4-7    sums: thread = row. acc = acc * a + O.
 //   warps 8-15   values: raw tile -> Kh Kl, Vh Vl in 128-byte swizzled tiles.
 //   warps 17-19  bulk copies, K's scales, V's scales.
@@ -131,17 +132,28 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
                    smem_u32(bar))
                : "memory");
 }
-// 32 lanes x 16 columns of 32-bit words (this warp's lane quarter), waited for.
+// 32 lanes x 16 columns of 32-bit words (this warp's lane quarter).
 __device__ __forceinline__ void tm_ld16(uint32_t taddr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      "%12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
+}
+// Wait for this thread's TMEM loads; the values pass through the asm so that no
+// use of them is scheduled before the wait.
+__device__ __forceinline__ void tm_wait_ld16(float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 __device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -480,10 +492,9 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
     fence_after();
     const int pos0 = (tl.first + i) * kUTile, ok = c.ok[g & 7];
     const bool all = __all_sync(0xffffffffu, ok == 15 && pos0 + kUTile <= lim);
-    // 16 columns of S at a time, scaled and masked; column e of chunk x is
-    // position 2 x + e / 8 + 8 (e mod 8)
-    auto load = [&](int x, float* s) {
-      tm_ld16(tlane + GM::S + st * kUTile + 16 * x, s);
+    float a = 1.0f, sum[2] = {0.0f, 0.0f};
+    // 16 columns of S; column e of part x is position 2 x + e / 8 + 8 (e mod 8)
+    auto process = [&](int x, float* s) {
 #pragma unroll
       for (int j = 0; j < 16; j += 4) {
         const float4 k = *reinterpret_cast<const float4*>(&c.kinv[g & 7][16 * x + j]);
@@ -496,28 +507,35 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
         for (int e = 0; e < 16; ++e)
           if (!((ok >> ((e & 7) >> 1)) & 1) || (e >> 3) + 8 * (e & 7) >= left) s[e] = -INFINITY;
       }
-    };
-    float top = -INFINITY;
-#pragma unroll 1
-    for (int x = 0; x < kUTile / 16; ++x) {
-      float s[16];
-      load(x, s);
+      float top = s[0];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
-    }
-    top = top == -INFINITY ? top : top * cn;
-    float a = 1.0f;
-    if (top > m + 4.0f) {  // also the first that is seen
-      a = ex2(m - top);
-      m = top;
-      l *= a;
-    }
-    const float off = m == -INFINITY ? 0.0f : 10.0f - m;
-    float sum[2] = {0.0f, 0.0f};
-#pragma unroll 1
-    for (int x = 0; x < kUTile / 16; ++x) {
-      float s[16];
-      load(x, s);
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+      top = top == -INFINITY ? top : top * cn;
+      const bool more = top > m + 4.0f;  // also the first that is seen
+      if (__any_sync(0xffffffffu, more)) {
+        // the maximum moves by whole numbers, so the parts before are scaled exactly
+        const int k = !more ? 0 : m == -INFINITY ? 127 : (int)fminf(ceilf(top - m), 127.0f);
+        const float b = k == 127 ? 0.0f : __uint_as_float((uint32_t)(127 - k) << 23);
+        if (more) m = m == -INFINITY ? ceilf(top) : m + ceilf(top - m);
+        a *= b;
+        l *= b;
+        sum[0] *= b;
+        sum[1] *= b;
+        const int k1 = min(k, 14), k2 = min(k - k1, 24);
+        const __half2 f1 = __float2half2_rn(__uint_as_float((uint32_t)(127 - k1) << 23)),
+                      f2 = __float2half2_rn(__uint_as_float((uint32_t)(127 - k2) << 23));
+        for (int y = 0; y < x; ++y) {
+          float v[16];
+          uint32_t part[16];
+          tm_ld16(tlane + GM::S + st * kUTile + 16 * y, v);
+          tm_wait_ld16(v);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            part[e] = h2_bits(__hmul2(__hmul2(bits_h2(__float_as_uint(v[e])), f1), f2));
+          tm_st16(tlane + GM::S + st * kUTile + 16 * y, part);
+        }
+      }
+      const float off = m == -INFINITY ? 0.0f : 10.0f - m;
       uint32_t part[16];  // eight columns of high, eight of low parts in S's place
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
@@ -528,6 +546,13 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
         split2(s[e], s[e + 1], part[e / 2], part[e / 2 + 8]);
       }
       tm_st16(tlane + GM::S + st * kUTile + 16 * x, part);
+    };
+#pragma unroll 1
+    for (int x = 0; x < kUTile / 16; ++x) {
+      float s[16];
+      tm_ld16(tlane + GM::S + st * kUTile + 16 * x, s);
+      tm_wait_ld16(s);
+      process(x, s);
     }
     l += sum[0] + sum[1];
     uint32_t nan = 0, any = 0;
@@ -616,6 +641,7 @@ __device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const 
     for (int d0 = 0; d0 < HD; d0 += 16) {
       float o[16];
       tm_ld16(col + st * HD + d0, o);
+      tm_wait_ld16(o);
       const float fn = (nan >> (d0 / 32)) & 1 ? NAN : f;
 #pragma unroll
       for (int d = 0; d < 16; d += 2) {
