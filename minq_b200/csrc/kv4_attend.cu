@@ -159,7 +159,7 @@ constexpr int kKvMinPiece = 96;  // smallest piece of the line per warp
 
 // Requests of so many (token, head) rows go to the tcgen05 kernel.
 constexpr size_t kKvUmmaMin = 32;
-constexpr int kKvUmmaSpread = 16;  // blocks that share the columns of its join's pieces
+constexpr int kKvUmmaSpread = 4;  // blocks that share the columns of its join's pieces
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -200,15 +200,21 @@ __device__ __forceinline__ uint32_t up_exponent(float m) {
   return (uint32_t)min(e, 253);
 }
 
-// A scale d as two f16 parts, high in the low half word. The high part has 8
-// bits, so a code (4 bits with its sign) times it is exact; the low part and
-// its product with a code are rounded, 2^-20 of the value each at most.
+// A scale d as two f16 parts, high in the low half word.
 __device__ __forceinline__ uint32_t scale_parts(float d) {
-  const __half h = __float2half_rn(__uint_as_float((__float_as_uint(d) + 0x8000u) & 0xffff0000u));
+  const __half h = __float2half_rn(d);
   return h2_bits(__halves2half2(h, __float2half_rn(d - __half2float(h))));
 }
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  return h2_bits(__hmul2(bits_h2(a), bits_h2(b)));
+// Two values, code y times scale dh + dl, as two f16 parts: the high one
+// rounded, what that leaves out (exact) plus y dl the low one. Within 2^-23.
+// (Scales whose high part has 8 bits need no remainder, one instruction less
+// of three, but leave 2^-20.)
+__device__ __forceinline__ void value_parts(uint32_t y, uint32_t dh, uint32_t dl, uint32_t& hi,
+                                            uint32_t& lo) {
+  const __half2 h = __hmul2_rn(bits_h2(y), bits_h2(dh));
+  const __half2 rest = __hfma2(bits_h2(y), bits_h2(dh), __hneg2(h));
+  hi = h2_bits(h);
+  lo = h2_bits(__hfma2(bits_h2(y), bits_h2(dl), rest));
 }
 // x = x * y, x = x * y + z, x + y on two f32 at once.
 __device__ __forceinline__ void mul_f2(float* x, float y0, float y1) {
@@ -371,16 +377,14 @@ __device__ __forceinline__ void um_values(UmCtl& c, const uint8_t* sm, uint32_t 
       const uint32_t tile = base + GM::K + st * 2 * GM::KT + (kb >> 1) * kUTile * 128;
 #pragma unroll 1
       for (int x = 0; x < 4; ++x) {
-        uint32_t y[4], v[4];
+        uint32_t y[4], hi[4], lo[4];
         codes4(*reinterpret_cast<const uint32_t*>(rk + kt * kQ4Bytes + 4 + 4 * x), y);
         // blocks 2, 3: chunks in another order, against bank conflicts
         const uint32_t at = tile + sw_chunk(s_column(kr), 4 * (kb & 1) + (x ^ (kb & 2)));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = mul2(y[e], dh);
-        sts16(at, v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = mul2(y[e], dl);
-        sts16(at + GM::KT, v);
+        for (int e = 0; e < 4; ++e) value_parts(y[e], dh, dl, hi[e], lo[e]);
+        sts16(at, hi);
+        sts16(at + GM::KT, lo);
       }
     }
     fence_async_smem();
@@ -397,10 +401,7 @@ __device__ __forceinline__ void um_values(UmCtl& c, const uint8_t* sm, uint32_t 
       uint32_t y[4];
       codes4(__byte_perm(x0, x1, 0x5410), y);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        hi[e][q] = mul2(y[e], dh);
-        lo[e][q] = mul2(y[e], dl);
-      }
+      for (int e = 0; e < 4; ++e) value_parts(y[e], dh, dl, hi[e][q], lo[e][q]);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&c.raw_free[rs]);
