@@ -70,7 +70,7 @@ struct UmGeom {
 };
 
 struct UmCtl {
-  float2 corr[4][kKvUmmaRows];  // per row: factor of its sum; bit b: block b becomes NaN
+  float2 corr[4][kKvUmmaRows];  // per row: the maximum used; bit b: block b becomes NaN
   float2 ml[kKvUmmaRows];
   float kinv[8][kUTile];        // 1 / f_t of K
   // scales of the positions that exist (0: not; V: or not finite) as two f16 parts
@@ -228,6 +228,12 @@ __device__ __forceinline__ void fma_f2(float* x, float y, float z0, float z1) {
       "mov.b64 c, {%3, %4};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
       : "+f"(x[0]), "+f"(x[1])
       : "f"(y), "f"(z0), "f"(z1));
+}
+__device__ __forceinline__ void fma_acc2(float* x, const float* y, float z) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "mov.b64 c, {%4, %4};\n\tfma.rn.f32x2 a, b, c, a;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x[0]), "+f"(x[1])
+      : "f"(y[0]), "f"(y[1]), "f"(z));
 }
 __device__ __forceinline__ void add_f2(float* x, const float* y) {
   asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
@@ -493,7 +499,7 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
     fence_after();
     const int pos0 = (tl.first + i) * kUTile, ok = c.ok[g & 7];
     const bool all = __all_sync(0xffffffffu, ok == 15 && pos0 + kUTile <= lim);
-    float a = 1.0f, sum[2] = {0.0f, 0.0f};
+    float sum[2] = {0.0f, 0.0f};
     // 16 columns of S; column e of part x is position 2 x + e / 8 + 8 (e mod 8)
     auto process = [&](int x, float* s) {
 #pragma unroll
@@ -518,7 +524,6 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
         const int k = !more ? 0 : m == -INFINITY ? 127 : (int)fminf(ceilf(top - m), 127.0f);
         const float b = k == 127 ? 0.0f : __uint_as_float((uint32_t)(127 - k) << 23);
         if (more) m = m == -INFINITY ? ceilf(top) : m + ceilf(top - m);
-        a *= b;
         l *= b;
         sum[0] *= b;
         sum[1] *= b;
@@ -565,7 +570,7 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
         for (int b = 0; b < 32; ++b)
           if (((c.bad[g & 7][x] >> b) & 1) && pos0 + x * PER + b / NB < lim) nan |= 1u << (b % NB);
     }
-    c.corr[g & 3][row] = make_float2(a, __uint_as_float(nan));
+    c.corr[g & 3][row] = make_float2(m, __uint_as_float(nan));
     tm_wait_st();
     fence_before();
     mbar_arrive(&c.p_full[st]);
@@ -628,7 +633,7 @@ __device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const 
   using GM = UmGeom<HD>;
   const int row = threadIdx.x - 32 * kUSoft;
   const uint32_t col = tmem + ((uint32_t)(row & ~31) << 16) + GM::O;
-  float acc[HD];
+  float acc[HD], M = -3.0e38f;  // the sum, relative to the maximum of the last tile
 #pragma unroll
   for (int d = 0; d < HD; ++d) acc[d] = 0.0f;
   for (int i = 0; i < tl.n; ++i) {
@@ -637,6 +642,13 @@ __device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const 
     fence_after();
     const float2 cr = c.corr[g & 3][row];
     const float f = c.vinv[g & 15];
+    const bool more = cr.x > M;
+    if (__any_sync(0xffffffffu, more)) {
+      const float a = more ? ex2(M - cr.x) : 1.0f;
+      if (more) M = cr.x;
+#pragma unroll
+      for (int d = 0; d < HD; d += 2) mul_f2(acc + d, a, a);
+    }
     const uint32_t nan = __float_as_uint(cr.y);
 #pragma unroll
     for (int d0 = 0; d0 < HD; d0 += 16) {
@@ -645,10 +657,7 @@ __device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const 
       tm_wait_ld16(o);
       const float fn = (nan >> (d0 / 32)) & 1 ? NAN : f;
 #pragma unroll
-      for (int d = 0; d < 16; d += 2) {
-        mul_f2(o + d, fn, fn);
-        fma_f2(acc + d0 + d, cr.x, o[d], o[d + 1]);
-      }
+      for (int d = 0; d < 16; d += 2) fma_acc2(acc + d0 + d, o + d, fn);
     }
     fence_before();
     mbar_arrive(&c.o_free[st]);
