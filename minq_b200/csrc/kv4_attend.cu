@@ -157,9 +157,13 @@ constexpr int kKvTile = 32;     // positions per tile
 constexpr int kKvExtra = 64;    // an item's start and end, in positions
 constexpr int kKvMinPiece = 96;  // smallest piece of the line per warp
 
-// Requests of so many (token, head) rows go to the tcgen05 kernel.
-constexpr size_t kKvUmmaMin = 32;
-constexpr int kKvUmmaSpread = 4;  // blocks that share the columns of its join's pieces
+// Requests of so many (token, head) rows of a kv head go to the tcgen05 kernel,
+// whose tile has 128 rows whether they are filled or not. Measured (call, us,
+// it / this one) at 32, 48, 64 and 128 rows a request: 32 requests of 2048
+// positions, 8 kv heads, 163 / 124, 167 / 175, 169 / 220, 173 / 407; one of 8192
+// positions 52 / 42, 54 / 52, 56 / 54, 69 / 77.
+constexpr size_t kKvUmmaMin = 64;
+constexpr int kKvUmmaSpread = 8;  // blocks that share the columns of its join's pieces
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -907,7 +911,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
 // one of many by all eight warps, column by column. A long step of few items
 // has its columns spread over gridDim.y blocks.
 constexpr int kKvJoinWarps = 8;
-constexpr int kKvJoinAlone = 16;  // pieces
+constexpr int kKvJoinAlone = 32;  // pieces
 constexpr int kKvJoinRecs = 16;   // most pieces that a block looks through
 template <int HD>
 __global__ void __launch_bounds__(kKvJoinWarps * 32)
