@@ -517,8 +517,8 @@ minq_status minq_kv4_read(const void* k_pages, const void* v_pages, size_t n_pag
  * scaled by `scale` (1 / sqrt(head_dim) in the reference). A row that sees
  * nothing is zero; positions in a page whose id is outside the pool, or past
  * the table row, are not seen; rows behind q_start[n_req] are left as they
- * were. Any n_req <= 8192, n_tokens <= 2^24, n_heads a multiple of n_kv,
- * head_dim a multiple of 32 up to 256. `workspace` (16-byte aligned) holds
+ * were. Any n_req <= 8192, n_tokens <= 2^24, n_tokens * n_heads < 2^31, n_heads
+ * a multiple of n_kv, head_dim a multiple of 32 up to 256. `workspace` (16-byte aligned) holds
  * minq_kv4_attend_workspace_bytes(...) bytes, needs no initial value, and
  * must not be shared by calls that may overlap. */
 size_t minq_kv4_attend_workspace_bytes(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv,
@@ -542,8 +542,10 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
  * is the first kept one whose running sum reaches u * (kept sum), in that
  * order when a filter is on and by index otherwise; logits of -infinity or
  * NaN are never drawn, and a row of nothing else gives token 0. Greedy rows
- * (also top_k = 1) take minq_argmax's token. Sums are f64. n <= 4194304,
- * n_rows <= 2^20. */
+ * (also top_k = 1) take minq_argmax's token. Weights are fixed-point integers
+ * to 2^-28 of themselves and their sums exact, so a result depends on no order;
+ * temperatures below 1e-12 of the largest |logit| are treated alike.
+ * n <= 4194304, n_rows <= 2^20. */
 minq_status minq_sample_rows(const float* logits, size_t row_stride, size_t n_rows, size_t n,
                              const float* temperature, const int32_t* top_k, const float* top_p,
                              const float* min_p, const float* uniforms, uint32_t* tokens,

@@ -17,7 +17,9 @@
 // A value costs seven instructions (with roundf and an integer conversion each
 // it is twenty, and the write then waits for the arithmetic): the rounding half
 // away from zero is two additions rounded towards zero, and four codes are
-// added up in one float before a single conversion.
+// added up in one float before a single conversion. Measured at 8191 tokens of 8
+// heads of 128 (77 MB each): write 19.7 us, 3.9 TB/s (24.4 us before), read 16.6 us,
+// 4.7 TB/s; a copy of as many bytes at the measured rate takes 12 us.
 #include <string>
 
 #include "common.cuh"

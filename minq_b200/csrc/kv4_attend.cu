@@ -8,7 +8,10 @@
 // id is outside the pool, or before the start (pos < 0) do not exist; a row
 // that sees nothing is zero.
 //
-// The tensor-core kernel (head_dim 64, 128). With k_t = d_tb (c_tb - 8) for
+// Three kernels. Prompt chunks of head_dim 64 and 128 have tcgen05's
+// (kv4_attend_umma.cu); other head dims than those two have a plain one (below).
+// The kernel for single tokens and short runs of them, mma.sync: 4 to 16 columns
+// are too few to fill tcgen05's 128 rows. With k_t = d_tb (c_tb - 8) for
 // block b of 32 dimensions, scale s and codes c in 0..15,
 //   score  z_t  = sum_b d_tb sum_i s q_i (c_ti - 8)
 //   output o_i  = sum_t (p_t e_tb) (c_ti - 8)      (e: the scales of V)
@@ -46,6 +49,13 @@
 // the pieces of the others go to the workspace, one per warp, or one per CTA
 // where an item fills it, and a second small launch joins them in a fixed
 // order, so results repeat bit for bit.
+//
+// What bounds it: 64 requests of 1 to 8192 positions (8 kv heads of 128, 306 MB,
+// 47 us at the measured copy rate) take 89 us, 3.4 TB/s: the two f16 parts and the
+// scales cost about 400 warp instructions per 16 positions of a kv head, and a
+// scheduler issues one in 0.67 of its cycles. 2 x 131071 positions of 2 kv heads
+// of 64 take 36 us (41 MB), half of it the join; 1 x 1000 positions 19 us, the
+// launches and the dependent loads.
 #include <limits.h>
 #include <math.h>
 
@@ -74,26 +84,31 @@ __device__ __forceinline__ int kv4_request_of(const Kv4AttnParams& p, int t) {
   return p.q_start[lo] <= t && t < p.q_start[lo + 1] ? lo : -1;
 }
 
-// One warp per (token, query head); any head_dim that is a multiple of 32.
-// Scores: a lane per position; values: a lane per dimension of each block.
-__global__ void __launch_bounds__(128) kv4_attend_rows_kernel(Kv4AttnParams p) {
-  __shared__ float s_q[4][256];
+// One CTA per (token, query head), any head_dim that is a multiple of 32: the
+// kernel for the head dims that no model of this library has (64 and 128 have
+// the tensor-core kernels). Its warps take turns at 32 positions. Scores: a lane
+// per position; values: a lane per dimension of each block. Measured: 8 requests
+// of 2048 positions, 16 heads of 96, 207 us (128 dims on tensor cores 24).
+constexpr int kKvRowsWarps = 8;
+__global__ void __launch_bounds__(kKvRowsWarps * 32) kv4_attend_rows_kernel(Kv4AttnParams p) {
+  __shared__ float s_q[256];
+  __shared__ float s_o[kKvRowsWarps][256];
+  __shared__ float s_m[kKvRowsWarps], s_l[kKvRowsWarps];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const size_t row = (size_t)blockIdx.x * 4 + warp;
-  if (row >= (size_t)p.n_tokens * p.nh) return;
-  const int t = (int)(row / p.nh), h = (int)(row % p.nh);
+  const int t = blockIdx.x / p.nh, h = blockIdx.x % p.nh;
   const int r = kv4_request_of(p, t);
   if (r < 0) return;
   const int nb = p.hd / kBlock, kvh = h / (p.nh / p.nkv);
-  float* q = s_q[warp];
-  for (int d = lane; d < p.hd; d += 32) q[d] = p.q[t * p.q_stride + (size_t)h * p.hd + d] * p.scale;
-  __syncwarp();
+  const float* q = s_q;
+  for (int d = threadIdx.x; d < p.hd; d += kKvRowsWarps * 32)
+    s_q[d] = p.q[t * p.q_stride + (size_t)h * p.hd + d] * p.scale;
+  __syncthreads();
   const long long pos = (long long)p.lens[r] - (p.q_start[r + 1] - t);
   const long long cap = (long long)p.table_stride << p.page_shift;
   const long long n = pos + 1 < cap ? pos + 1 : cap;  // positions seen (< 1: none)
   float m = -INFINITY, l = 0.0f, o[8] = {};
-  for (long long p0 = 0; p0 < n; p0 += 32) {
+  for (long long p0 = 32 * warp; p0 < n; p0 += 32 * kKvRowsWarps) {
     // P >= 16: the 32 positions lie in one or two pages; a lane has its own row
     const long long i = p0 + lane;
     const int id = i < n ? p.table[(size_t)r * p.table_stride + (size_t)(i >> p.page_shift)] : -1;
@@ -123,6 +138,7 @@ __global__ void __launch_bounds__(128) kv4_attend_rows_kernel(Kv4AttnParams p) {
     l = l * a + w;
 #pragma unroll
     for (int b = 0; b < 8; ++b) o[b] *= a;
+#pragma unroll 4
     for (int j = 0; j < 32; ++j) {
       const float wj = __shfl_sync(0xffffffffu, w, j);
       const bool onj = __shfl_sync(0xffffffffu, (int)on, j) != 0;
@@ -139,12 +155,29 @@ __global__ void __launch_bounds__(128) kv4_attend_rows_kernel(Kv4AttnParams p) {
     }
   }
   l = warp_sum(l);
-  float* out = p.out + (size_t)t * p.out_stride + (size_t)h * p.hd;
 #pragma unroll
   for (int b = 0; b < 8; ++b)
-    if (b < nb) out[b * 32 + lane] = l != 0.0f ? o[b] / l : 0.0f;
+    if (b < nb) s_o[warp][b * 32 + lane] = o[b];
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kKvRowsWarps; ++w) M = fmaxf(M, s_m[w]);
+  float* out = p.out + (size_t)t * p.out_stride + (size_t)h * p.hd;
+  for (int d = threadIdx.x; d < p.hd; d += kKvRowsWarps * 32) {
+    float sum = 0.0f, L = 0.0f;
+    for (int w = 0; w < kKvRowsWarps; ++w)
+      if (s_m[w] != -INFINITY) {  // a warp that saw something
+        const float a = expf(s_m[w] - M);
+        sum += s_o[w][d] * a;
+        L += s_l[w] * a;
+      }
+    out[d] = L != 0.0f ? sum / L : 0.0f;
+  }
 }
-
 
 // ---- tensor cores ------------------------------------------------------------
 
@@ -906,10 +939,10 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
   }
 }
 
-// Joins the pieces of the items that start in join_pieces pieces and go on behind them, always in a fixed order. An item of few pieces is summed
-// by a warp per column, the (item, column) pairs dealt out to the eight warps;
-// one of many by all eight warps, column by column. A long step of few items
-// has its columns spread over gridDim.y blocks.
+// Joins the pieces of the items that start in join_pieces pieces and go on
+// behind them, always in a fixed order. An item of few pieces is summed by a warp
+// per column, the (item, column) pairs dealt out to the eight warps; one of many
+// by all eight warps, column by column. Columns are spread over gridDim.y blocks.
 constexpr int kKvJoinWarps = 8;
 constexpr int kKvJoinAlone = 32;  // pieces
 constexpr int kKvJoinRecs = 16;   // most pieces that a block looks through
@@ -1033,6 +1066,11 @@ KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_
   KvPlan k{};
   if ((hd != 64 && hd != 128) || n_kv == 0 || n_req == 0) return k;
   const size_t G = n_heads / n_kv;
+  // Columns of a tile and what is in them. Measured (call with 64 x 8192 cold, us):
+  // G = 4, one token each: both parts of q in one tile of 8 columns 171, a tile a
+  // part 256, two tiles a part 329. Two tiles a part or one: 12 to 16 heads to a
+  // kv head, 32 x 4096, 52 / 60; 2, 3, 4, 8 tokens each of G = 4, 32 x 2048,
+  // 91 / 83, 97 / 105, 99 / 124, 144 / 200.
   // With kKvUmmaMin rows a request and more, the chunks are the tcgen05 kernel's and what
   // is left for the other one are mostly single tokens.
   const size_t gsz = G < (size_t)kKvUmmaRows ? G : kKvUmmaRows;
@@ -1124,6 +1162,8 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
       table_stride == 0 || table_stride > (1u << 30))
     return fail(MINQ_ERR_SHAPE, "kv4_attend: heads, requests, tokens, pages or table width out of "
                                 "range");
+  if (n_tokens * n_heads > 0x7fffffffu)
+    return fail(MINQ_ERR_SHAPE, "kv4_attend: n_tokens * n_heads must be below 2^31");
   if (n_tokens > 1 && (q_stride < n_heads * head_dim || out_stride < n_heads * head_dim))
     return fail(MINQ_ERR_ARG, "kv4_attend: token strides must be at least n_heads * head_dim");
   if (n_tokens == 0 || n_req == 0 || n_heads == 0) return MINQ_OK;
@@ -1187,9 +1227,8 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
                             : launch_kv4_attend<128, 2, false>(p, s)));
     return launch_kv4_join<128>(p, plan.umma_lo ? &u : nullptr, s);
   }
-  const size_t rows = n_tokens * n_heads;
-  MINQ_CUDA_TRY(launch_k(kv4_attend_rows_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0,
-                         (cudaStream_t)stream, p));
+  MINQ_CUDA_TRY(launch_k(kv4_attend_rows_kernel, dim3((unsigned)(n_tokens * n_heads)),
+                         dim3(kKvRowsWarps * 32), 0, (cudaStream_t)stream, p));
   return MINQ_OK;
 }
 

@@ -30,6 +30,16 @@
 // P V's is free, so both are chosen for the code layout and for stores without
 // bank conflicts (q_dim and the packing of P follow them).
 //
+// Measured: 4 requests, two of them with 512 new tokens behind up to 3584, 32 query
+// and 8 kv heads of 128 (61 GFLOP of useful products): 220 us, 0.28 PFLOP/s, three
+// f16 products each, so 0.83 PFLOP/s of the tensor cores' work; the mma.sync kernel
+// takes 670 us. A tile costs an SM 3,300 cycles, of which the tensor cores need
+// 1,400; softmax (2,700 of its warps' time) and values (2,200) run beside them but
+// share the issue slots, which are used in 0.55 of the cycles. The roles' loops are
+// kept short (one step of 16 columns, not four unrolled): together they have to fit
+// the instruction cache, and unrolled they took 352 us. Eight softmax warps that
+// took turns at the tiles, with fewer registers each, took 234 us.
+//
 // A value scale that is not finite would reach rows that do not see its
 // position (0 x inf): it is left out of the tile and makes the block of the
 // rows that see it NaN.

@@ -78,7 +78,7 @@ def _shape(msg: str) -> MinqError:
     return MinqError(_lib.ERR_SHAPE, msg)
 
 
-def _refuse(name, t, dtype, dev, shape, contiguous):
+def _refuse(name, t, dtype, dev, shape):
     """Why a tensor argument is not taken."""
     if not getattr(t, "is_cuda", False):
         raise MinqError(_lib.ERR_CUDA, f"{name} must be a CUDA tensor (there is no CPU path)")
@@ -95,7 +95,7 @@ def _take(name, t, dtype, dev, shape=None):
     """Address of a contiguous tensor argument on CUDA device `dev`, checked."""
     if (t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous()
             or (shape is not None and t.shape != shape)):
-        _refuse(name, t, dtype, dev, shape, True)
+        _refuse(name, t, dtype, dev, shape)
     return t.data_ptr()
 
 
@@ -211,7 +211,7 @@ def _rows(name, x, n_heads, hd, dev):
     """Address and token stride of [tokens, heads, head_dim] rows (the tokens
     may be strided, as slices of a projection are)."""
     if x.dtype is not _b.f32 or x.get_device() != dev:
-        _refuse(name, x, _b.f32, dev, None, False)
+        _refuse(name, x, _b.f32, dev, None)
     shape, st = x.shape, x.stride()
     if len(shape) != 3 or shape[1] != n_heads or shape[2] != hd:
         raise _shape(f"{name} must have shape [tokens, {n_heads}, {hd}], got {list(shape)}")
@@ -300,7 +300,7 @@ def sample_rows(logits, uniforms, temperature=None, top_k=None, top_p=None, min_
     f32, i32, one = _b.f32, _b.i32, (rows,)
     stride, step = logits.stride()
     if logits.dtype is not f32:
-        _refuse("logits", logits, f32, dev, None, False)
+        _refuse("logits", logits, f32, dev, None)
     if step != 1 and n > 1:
         raise _arg("logits: a row must be contiguous")
     if out is None:

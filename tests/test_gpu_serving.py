@@ -496,6 +496,196 @@ def test_attend_repeats_bit_for_bit_and_in_a_graph(mq, torch):
     assert torch.equal(out, a)
 
 
+# Prompt chunks (64 and more rows of a kv head) have a kernel of their own, whose
+# arithmetic keeps the bound above: K and V as two f16 parts are off by 2^-23 of
+# each value; a score's 3 head_dim / 16 tensor-core steps truncate at 2 e each,
+# 48 e at head_dim 128, inside (head_dim + 8) e; a tile's 12 steps of P V 24 e,
+# inside 80 e, and the tiles' sums are n / 64 f32 additions. The smallest steps
+# of the parts of P and V are 2^-34 and 2^-36 of the largest weight and value.
+
+CHUNK_HEADS = [(32, 8, 128), (14, 2, 64), (4, 4, 128), (16, 1, 128), (160, 1, 64), (129, 1, 128)]
+
+
+@pytest.mark.parametrize("nh,nkv,hd", CHUNK_HEADS)
+@pytest.mark.parametrize("page,lens,new", [
+    (16, [64], [64]),                             # no history
+    (16, [130, 700, 5, 0, 64], [129, 64, 1, 0, 63]),  # ends inside a tile, with single tokens
+    (1024, [1100, 321], [70, 200]),               # one page holds whole tiles
+])
+def test_attend_chunks_match_the_formula(mq, torch, nh, nkv, hd, page, lens, new):
+    kp, vp, table, kv, vv = _fill(mq, torch, nh + hd, lens, nkv, hd, page)
+    start = [0] + np.cumsum(new).tolist()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.randn(start[-1], nh, hd, generator=g, device="cuda") * 2
+    got = mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp)
+    want, tol = _reference(torch, q, start, lens, table, page, kv, vv, hd ** -0.5)
+    _check(torch, got, want, tol)
+    assert torch.equal(got, mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.09, 0.4])
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (14, 2, 64)])
+def test_attend_chunks_any_scale_and_large_values(mq, torch, nh, nkv, hd, scale):
+    """Even weights, the reverse order, scores in the hundreds; value rows whose
+    scales differ by orders of magnitude."""
+    lens, page, new = [900, 77], 32, [65, 70]
+    kp, vp, table, kv, vv = _fill(mq, torch, 3, lens, nkv, hd, page, gain=6.0)
+    rows = vv * torch.exp(3 * torch.randn(vv.shape[0], 1, 1, device="cuda")).double()
+    slots = torch.arange(vv.shape[0], device="cuda")
+    mq.kv4_write(rows.float(), rows.float(), slots, vp, mq.kv4_pool(*vp.shape[:3], hd))
+    vv = mq.kv4_read(slots, kp, vp)[1].double()
+    start = [0, 65, 135]
+    q = torch.randn(135, nh, hd, device="cuda") * 8
+    got = mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp, scale=scale)
+    want, tol = _reference(torch, q, start, lens, table, page, kv, vv, scale)
+    _check(torch, got, want, tol)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (14, 2, 64)])
+def test_attend_chunks_ignore_what_a_token_may_not_see(mq, torch, nh, nkv, hd):
+    """Bad pages at the start, in the middle and throughout; NaN and infinite
+    scales in all that no token sees; a value scale that is not finite reaches
+    the tokens behind it, in its block, and no other."""
+    page, lens, new = 16, [200, 100, 150], [70, 65, 66]
+    kp, vp, table, kv, vv = _fill(mq, torch, 9, lens, nkv, hd, page, width=14, extra=3)
+    n_pages, nb = kp.shape[0], hd // 32
+    table[0, 0], table[0, 6], table[0, 9] = -1, n_pages, -2**31
+    table[1] = -1
+    seen = torch.zeros(n_pages, page, dtype=torch.bool, device="cuda")
+    for r, n in enumerate(lens):
+        for i in range(n):
+            pg = int(table[r, i // page])
+            if 0 <= pg < n_pages:
+                seen[pg, i % page] = True
+    blocks = [p.view(n_pages, nkv, page, nb, 20) for p in (kp, vp)]
+    for b, bad in zip(blocks, (float("nan"), float("inf"))):
+        mark = torch.tensor([bad], device="cuda").view(torch.uint8)
+        hide = ~seen[:, None, :, None].expand(n_pages, nkv, page, nb)
+        b[..., :4] = torch.where(hide[..., None], mark, b[..., :4])
+    start = [0] + np.cumsum(new).tolist()
+    T = start[-1] + 3
+    q = torch.randn(T, nh, hd, device="cuda")
+    q[start[-1]:] = float("nan")
+    out = torch.full((T, nh, hd), 5.0, device="cuda")
+    args = (q, dev(torch, start), dev(torch, lens), table, kp, vp)
+    mq.kv4_attend(*args, out=out)
+    want, tol = _reference(torch, q[:start[-1]], start, lens, table, page, kv, vv, hd ** -0.5)
+    assert not out[start[1]:start[2]].any()
+    assert (out[start[-1]:] == 5.0).all()
+    _check(torch, out[:start[-1]], want, tol)
+    # position 120 of request 2 (its tokens are 84 .. 149), kv head 1, block 1 of V
+    pg = int(table[2, 120 // page])
+    for bad in (float("inf"), float("nan")):
+        blocks[1][pg, 1, 120 % page, 1, :4] = torch.tensor([bad], device="cuda").view(torch.uint8)
+        got = mq.kv4_attend(*args)[:start[-1]]
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        G = nh // nkv
+        hit[start[2] + 36:start[3], G:2 * G, 32:64] = True
+        assert not torch.isfinite(got[hit]).any()
+        assert torch.equal(got[~hit], out[:start[-1]][~hit])
+    # a key scale that is not finite: the tokens before it do not notice
+    blocks[1][pg, 1, 120 % page, 1, :4] = torch.tensor([0.0], device="cuda").view(torch.uint8)
+    blocks[0][pg, 1, 120 % page, 0, :4] = torch.tensor([float("nan")], device="cuda").view(torch.uint8)
+    got = mq.kv4_attend(*args)[:start[-1]]
+    assert not torch.isfinite(got[start[2] + 36:start[3], G:2 * G]).any()
+    assert torch.equal(got[:start[2] + 36], out[:start[2] + 36])
+
+
+def test_attend_many_requests(mq, torch):
+    """More requests than a CTA has threads, decoding ones between chunks."""
+    rng = random.Random(4)
+    nh, nkv, hd, page = 8, 2, 64, 16
+    lens = [rng.choice([0, 1, 16, rng.randint(1, 90)]) for _ in range(900)]
+    new = [min(n, rng.choice([0, 1, 1, 1, 1, 1, 3])) for n in lens]
+    for r in (0, 333, 700, 899):
+        lens[r], new[r] = 150, 40
+    kp, vp, table, kv, vv = _fill(mq, torch, 1, lens, nkv, hd, page)
+    start = [0] + np.cumsum(new).tolist()
+    q = torch.randn(start[-1], nh, hd, device="cuda")
+    got = mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp)
+    want, tol = _reference(torch, q, start, lens, table, page, kv, vv, hd ** -0.5)
+    _check(torch, got, want, tol)
+    # the same requests with one token each (many more of them than a CTA's threads)
+    one = [min(n, 1) for n in lens]
+    start = [0] + np.cumsum(one).tolist()
+    q = torch.randn(start[-1], nh, hd, device="cuda")
+    got = mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp)
+    want, tol = _reference(torch, q, start, lens, table, page, kv, vv, hd ** -0.5)
+    _check(torch, got, want, tol)
+
+
+def test_attend_two_streams_and_a_chunk_in_a_graph(mq, torch):
+    """Calls that overlap on two streams, and a captured mixed step replayed over
+    other lengths (chunks that become single tokens and the other way round)."""
+    nh, nkv, hd, page = 32, 8, 128, 32
+    lens, new = [900, 400, 33], [64, 1, 30]
+    kp, vp, table, kv, vv = _fill(mq, torch, 5, lens, nkv, hd, page)
+    start = [0] + np.cumsum(new).tolist()
+    sd, ld = dev(torch, start), dev(torch, lens)
+    qs = [torch.randn(start[-1], nh, hd, device="cuda") for _ in range(2)]
+    alone = [mq.kv4_attend(q, sd, ld, table, kp, vp) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(mq.kv4_attend(qs[i], sd, ld, table, kp, vp))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, alone[i]) for g in got[i])
+    out = torch.empty_like(qs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mq.kv4_attend(qs[0], sd, ld, table, kp, vp, out=out)
+    graph.replay()
+    assert torch.equal(out, alone[0])
+    for lens2, new2 in (([700, 399, 31], [1, 80, 14]), ([20, 1, 33], [0, 1, 33]), (lens, new)):
+        start2 = [0] + np.cumsum(new2).tolist()
+        sd.copy_(dev(torch, start2))
+        ld.copy_(dev(torch, lens2))
+        out.fill_(7.0)
+        graph.replay()
+        want, tol = _reference(torch, qs[0], start2, lens2, table, page, kv, vv, hd ** -0.5)
+        _check(torch, out[:start2[-1]], want[:start2[-1]], tol[:start2[-1]])
+        assert (out[start2[-1]:] == 7.0).all()
+    assert torch.equal(out, alone[0])
+
+
+FIRST_CALL = """
+import torch, minq_b200 as mq
+kp, vp = (mq.kv4_pool(4, 8, 16, 128) for _ in range(2))
+i32 = dict(dtype=torch.int32, device="cuda")
+lens, table = torch.tensor([20], **i32), torch.tensor([[1, 3]], **i32)
+start, q = torch.tensor([0, 20], **i32), torch.randn(20, 32, 128, device="cuda")
+slots = torch.tensor([16 + i if i < 16 else 48 + i - 16 for i in range(20)], device="cuda")
+k, v = (torch.randn(20, 8, 128, device="cuda") for _ in range(2))
+logits, u = torch.randn(3, 5000, device="cuda"), torch.rand(3, device="cuda")
+new, free, n_free = torch.tensor([5], **i32), torch.tensor([0, 2], **i32), torch.tensor([2], **i32)
+torch.cuda.synchronize()
+def step():
+    mq.kv4_write(k, v, slots, kp, vp)
+    return (*mq.kv4_read(slots, kp, vp), mq.kv4_attend(q, start, lens, table, kp, vp),
+            mq.sample_rows(logits, u), mq.pages_extend(lens, new, table.clone(), free, n_free, 16, 8).slots)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):  # the first call of everything
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+want = step()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+mq._lib.check(mq._lib.lib().minq_device_status())
+print("same")
+"""
+
+
+def test_first_call_inside_a_capture(mq, torch):
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stderr[-2000:]
+
+
 def test_attend_pages_past_four_gigabytes(mq, torch):
     """Byte offsets beyond 32 bits: the pages lie at the end of a 5 GB pool."""
     nh, nkv, hd, page = 8, 8, 128, 64
@@ -636,6 +826,24 @@ def test_sample_rows_large_vocabulary(mq, torch, n):
                   np.float64(np.float32(s[r][2])), np.float64(np.float32(s[r][3])))
             for r in range(rows)]
     assert got == want, [(r, a, b, s[r]) for r, (a, b) in enumerate(zip(got, want)) if a != b]
+
+
+@pytest.mark.parametrize("n", [1500001, 4194304])
+def test_sample_rows_longer_than_shared_memory(mq, torch, n):
+    g = np.random.default_rng(n)
+    x = g.standard_normal((5, n)).astype(np.float32) * 3
+    x[1] = -1.5  # every token ties
+    x[2, ::2] = -np.inf
+    x[3] *= 1e-2
+    s = [(1.0, 0, 0.9, 0.0), (1.0, 0, 0.6, 0.0), (0.7, 0, 1.0, 0.0), (1.0, n // 2, 0.999, 0.0),
+         (1.0, 50, 0.95, 0.01)]
+    u = g.random(5).astype(np.float32)
+    f = lambda i, t=torch.float32: torch.tensor([v[i] for v in s], dtype=t, device="cuda")  # noqa: E731
+    got = mq.sample_rows(torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda(), temperature=f(0),
+                         top_k=f(1, torch.int32), top_p=f(2), min_p=f(3)).tolist()
+    want = [_draw(x[r], np.float64(u[r]), np.float64(np.float32(s[r][0])), s[r][1],
+                  np.float64(np.float32(s[r][2])), np.float64(np.float32(s[r][3]))) for r in range(5)]
+    assert got == want
 
 
 def test_sample_rows_edges(mq, torch):

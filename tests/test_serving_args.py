@@ -79,6 +79,7 @@ def test_kv4_attend_refusals(L):
     assert attend(R=8193) == _lib.ERR_SHAPE
     assert attend(T=(1 << 24) + 1) == _lib.ERR_SHAPE
     assert attend(w=0) == _lib.ERR_SHAPE
+    assert attend(T=1 << 20, nh=2048, nkv=8, hd=128, qs=1 << 20, os_=1 << 20) == _lib.ERR_SHAPE
     assert attend(qs=4095) == _lib.ERR_ARG
     assert attend(os_=100) == _lib.ERR_ARG
     for null in ("q", "st", "lens", "table", "kp", "vp", "out"):
