@@ -21,7 +21,7 @@
 //   warps 0-3    softmax: thread = row = TMEM lane. One pass over S in steps of
 //                16 columns: moves the maximum only when a weight would exceed
 //                2^4 (and then scales what it has written), writes P over S.
-//   warps 4-7    sums: thread = row. acc = acc * a + O.
+//   warps 4-7    sums: thread = row. Writes Qh and Ql, then acc = acc * a + O.
 //   warps 8-15   values: raw tile -> Kh Kl, Vh Vl in 128-byte swizzled tiles.
 //   warps 17-19  bulk copies, K's scales, V's scales.
 //   warp 16      one thread issues the MMAs: S of the next tile, then P V.
@@ -82,6 +82,7 @@ struct UmGeom {
 struct UmCtl {
   float2 corr[4][kKvUmmaRows];  // per row: the maximum used; bit b: block b becomes NaN
   float2 ml[kKvUmmaRows];
+  float cn[kKvUmmaRows];        // scores to log2 units
   float kinv[8][kUTile];        // 1 / f_t of K
   // scales of the positions that exist (0: not; V: or not finite) as two f16 parts
   uint32_t kscale[kURaw][kUTile * 4], vscale[kURaw][kUTile * 4];
@@ -457,57 +458,13 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
   long long lim64 = on ? (long long)it.prior + it.tok0 + ct + 1 : 0;
   lim64 = lim64 < 0 ? 0 : lim64 < it.cap ? lim64 : it.cap;
   const int lim = (int)lim64;
-  float cn;
-  {
-    const float* q = p.q + (size_t)(it.rq.t0 + it.tok0 + (on ? ct : 0)) * p.q_stride +
-                     (size_t)(it.h0 + (on ? ch : 0)) * HD;
-    const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-    auto load8 = [&](int d, float* v) {
-      if (vec) {
-        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(q + d);
-        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(q + d + 4);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = q[d + e];
-      }
-    };
-    float m = 0.0f;
-#pragma unroll 4
-    for (int d = 0; d < HD; d += 8) {
-      float v[8];
-      load8(d, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
-    }
-    const int ex = min(max((int)(__float_as_uint(m) >> 23), 24), 254);
-    float f = __uint_as_float((uint32_t)(264 - ex) << 23);
-    cn = fabsf(p.scale) * 1.4426950408889634f * (1.0f / f);
-    if (cn == 0.0f) cn = 1.4e-45f;  // -inf stays masked
-    if (p.scale < 0.0f) f = -f;
-#pragma unroll 1
-    for (int x0 = 0; x0 < HD / 2; x0 += 16) {
-      uint32_t hi[16], lo[16];
-#pragma unroll
-      for (int x = 0; x < 16; x += 4) {
-        float v[8];
-        load8(q_dim<HD>((x0 + x) / 4), v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          split2(on ? v[e] * f : 0.0f, on ? v[e + 4] * f : 0.0f, hi[x + e], lo[x + e]);
-      }
-      tm_st16(tlane + GM::QH + x0, hi);
-      tm_st16(tlane + GM::QL + x0, lo);
-    }
-    tm_wait_st();
-    fence_before();
-    mbar_arrive(&c.q_full);
-  }
   float m = -INFINITY, l = 0.0f;
   for (int i = 0; i < tl.n; ++i) {
     const uint32_t g = g0 + i, st = g & 1;
     if (!um_wait(&c.s_full[st], (g >> 1) & 1, &c.abort)) return;
     fence_after();
     const int pos0 = (tl.first + i) * kUTile, ok = c.ok[g & 7];
+    const float cn = c.cn[row];
     const bool all = __all_sync(0xffffffffu, ok == 15 && pos0 + kUTile <= lim);
     float sum[2] = {0.0f, 0.0f};
     // 16 columns of S; column e of part x is position 2 x + e / 8 + 8 (e mod 8)
@@ -643,7 +600,49 @@ __device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const 
   using GM = UmGeom<HD>;
   const int row = threadIdx.x - 32 * kUSoft;
   const uint32_t col = tmem + ((uint32_t)(row & ~31) << 16) + GM::O;
-  float acc[HD], M = -3.0e38f;  // the sum, relative to the maximum of the last tile
+  const int ct = row / p.gsz, ch = row - ct * p.gsz;
+  const bool on = ct < it.ntok && ch < it.nhead;
+  float acc[HD];
+  // the row of q, all of it in flight at once, as f16 parts into TMEM
+  {
+    const float* q = p.q + (size_t)(it.rq.t0 + it.tok0 + (on ? ct : 0)) * p.q_stride +
+                     (size_t)(it.h0 + (on ? ch : 0)) * HD;
+    if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+#pragma unroll
+      for (int d = 0; d < HD; d += 4)
+        *reinterpret_cast<float4*>(acc + d) = *reinterpret_cast<const float4*>(q + d);
+    } else {
+#pragma unroll
+      for (int d = 0; d < HD; ++d) acc[d] = q[d];
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int d = 0; d < HD; ++d) {
+      if (!on) acc[d] = 0.0f;
+      m = fmaxf(m, fabsf(acc[d]));
+    }
+    const int ex = min(max((int)(__float_as_uint(m) >> 23), 24), 254);
+    float f = __uint_as_float((uint32_t)(264 - ex) << 23);
+    const float cn = fabsf(p.scale) * 1.4426950408889634f * (1.0f / f);
+    c.cn[row] = cn == 0.0f ? 1.4e-45f : cn;  // -inf stays masked
+    if (p.scale < 0.0f) f = -f;
+    const uint32_t tq = tmem + ((uint32_t)(row & ~31) << 16);
+#pragma unroll
+    for (int x0 = 0; x0 < HD / 2; x0 += 16) {
+      uint32_t hi[16], lo[16];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int d = q_dim<HD>((x0 + x) / 4) + (x & 3);
+        split2(acc[d] * f, acc[d + 4] * f, hi[x], lo[x]);
+      }
+      tm_st16(tq + GM::QH + x0, hi);
+      tm_st16(tq + GM::QL + x0, lo);
+    }
+    tm_wait_st();
+    fence_before();
+    mbar_arrive(&c.q_full);
+  }
+  float M = -3.0e38f;  // acc is relative to the maximum of the last tile
 #pragma unroll
   for (int d = 0; d < HD; ++d) acc[d] = 0.0f;
   for (int i = 0; i < tl.n; ++i) {
@@ -673,8 +672,7 @@ __device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const 
     mbar_arrive(&c.o_free[st]);
   }
   __syncthreads();
-  const int ct = row / p.gsz, ch = row - ct * p.gsz;
-  if (ct < it.ntok && ch < it.nhead) {
+  if (on) {
     const float2 ml = c.ml[row];
     const bool whole = it.x0 == 0 && it.x1 == it.w;
     const size_t at = ((size_t)blockIdx.x * 2 + (it.x0 > 0 ? 0 : 1)) * kKvUmmaRows + row;
@@ -717,6 +715,9 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
   UmCtl& c = *reinterpret_cast<UmCtl*>(sm + GM::CTL);
   constexpr int kMmaWarp = kUSoft + kUSum + kUVal;
 
+  // before the TMEM: a kernel before this one that still has to allocate its own
+  // must not meet a CTA that holds all of it and waits
+  pdl_wait();
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < kURaw; ++i) {
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
         mbar_init(&c.pv_done[i], 1);
         mbar_init(&c.o_free[i], 32 * kUSum);
       }
-      mbar_init(&c.q_full, 32 * kUSoft);
+      mbar_init(&c.q_full, 32 * kUSum);
       mbar_init(&c.drain, 1);
       c.abort = 0;
       c.req = -1;
@@ -744,9 +745,6 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_wait();
-  pdl_launch_dependents();
-
   // the line: every warp weighs a run of the requests, and the warp in whose
   // run the CTA's piece starts looks for the request
   const int H = p.nkv * p.hgroups, seg = (p.n_req + kUThreads / 32 - 1) / (kUThreads / 32);
@@ -763,6 +761,7 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
   fence_before();
   __syncthreads();
   fence_after();
+  pdl_launch_dependents();
   const uint32_t tmem = c.tmem;
   long long total = 0, before = 0;
   for (int x = 0; x < kUThreads / 32; ++x) {
