@@ -60,6 +60,7 @@
 #include <math.h>
 
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -947,7 +948,7 @@ constexpr int kKvJoinWarps = 8;
 constexpr int kKvJoinAlone = 32;  // pieces
 constexpr int kKvJoinRecs = 16;   // most pieces that a block looks through
 template <int HD>
-__global__ void __launch_bounds__(kKvJoinWarps * 32)
+__global__ void __launch_bounds__(kKvJoinWarps * 32, 4)
     kv4_join_kernel(const __grid_constant__ Kv4AttnParams p0, const __grid_constant__ Kv4AttnParams p1) {
   // the first p0.join_blocks blocks have p0's pieces, the others p1's
   const bool second = (int)blockIdx.x >= p0.join_blocks;
@@ -988,7 +989,9 @@ __global__ void __launch_bounds__(kKvJoinWarps * 32)
     return p.out + (size_t)(s_tok[k].x + tok) * p.out_stride + (size_t)(kvh * G + head) * HD;
   };
   // pieces w, w + step, .. of an item: their sum relative to the maximum M of all
-  auto sum = [&](const KvRec& rec, int col, int w, int step, float& L, float* acc) {
+  // (B: loads in flight)
+  auto sum = [&](auto batch, const KvRec& rec, int col, int w, int step, float& L, float* acc) {
+    constexpr int B = decltype(batch)::value;
     auto at = [&](int i) {
       const int piece = i < rec.n_first ? rec.a + i
                         : i < rec.n_first + rec.n_mid
@@ -997,26 +1000,48 @@ __global__ void __launch_bounds__(kKvJoinWarps * 32)
       return ((size_t)piece * 2 + (i == 0 ? 1 : 0)) * p.cols + col;
     };
     float M = -3.0e38f;
-    for (int i = lane; i < rec.parts; i += 32) M = fmaxf(M, p.part_ml[at(i) * 2]);
+    for (int i0 = 0; i0 < rec.parts; i0 += 32 * B) {
+      float m[B];
+#pragma unroll
+      for (int e = 0; e < B; ++e) {
+        const int i = i0 + 32 * e + lane;
+        m[e] = i < rec.parts ? p.part_ml[at(i) * 2] : M;
+      }
+#pragma unroll
+      for (int e = 0; e < B; ++e) M = fmaxf(M, m[e]);
+    }
     M = warp_max(M);
     L = 0.0f;
 #pragma unroll
     for (int d = 0; d < PER; ++d) acc[d] = 0.0f;
-#pragma unroll 8
-    for (int i = w; i < rec.parts; i += step) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(i) * 2);
-      const float f = ex2(ml.x - M);
-      L += ml.y * f;
-      const float* o = p.part_o + at(i) * HD + PER * lane;
-      float v[PER];
+    for (int i0 = w; i0 < rec.parts; i0 += B * step) {
+      float2 ml[B];
+      float v[B][PER];
 #pragma unroll
-      for (int d = 0; d < PER; d += 2) {
-        const float2 x = *reinterpret_cast<const float2*>(o + d);
-        v[d] = x.x;
-        v[d + 1] = x.y;
+      for (int e = 0; e < B; ++e) {
+        const int i = i0 + e * step;
+        if (i >= rec.parts) {
+          ml[e] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+          for (int d = 0; d < PER; ++d) v[e][d] = 0.0f;
+          continue;
+        }
+        ml[e] = *reinterpret_cast<const float2*>(p.part_ml + at(i) * 2);
+        const float* o = p.part_o + at(i) * HD + PER * lane;
+#pragma unroll
+        for (int d = 0; d < PER; d += 2) {
+          const float2 x = *reinterpret_cast<const float2*>(o + d);
+          v[e][d] = x.x;
+          v[e][d + 1] = x.y;
+        }
       }
 #pragma unroll
-      for (int d = 0; d < PER; ++d) acc[d] += v[d] * f;
+      for (int e = 0; e < B; ++e) {
+        const float f = ex2(ml[e].x - M);
+        L += ml[e].y * f;
+#pragma unroll
+        for (int d = 0; d < PER; ++d) acc[d] += v[e][d] * f;
+      }
     }
   };
   float L, acc[PER];
@@ -1025,7 +1050,7 @@ __global__ void __launch_bounds__(kKvJoinWarps * 32)
     if (s_rec[k].parts > kKvJoinAlone) continue;
     float* out = row(k, col);
     if (!out) continue;
-    sum(s_rec[k], col, 0, 1, L, acc);
+    sum(std::integral_constant<int, 2>(), s_rec[k], col, 0, 1, L, acc);
 #pragma unroll
     for (int d = 0; d < PER; ++d) out[PER * lane + d] = L != 0.0f ? acc[d] / L : 0.0f;
   }
@@ -1034,7 +1059,7 @@ __global__ void __launch_bounds__(kKvJoinWarps * 32)
     for (int col = blockIdx.y; col < used; col += gridDim.y) {
       float* out = row(k, col);
       if (!out) continue;
-      sum(s_rec[k], col, warp, kKvJoinWarps, L, acc);
+      sum(std::integral_constant<int, 8>(), s_rec[k], col, warp, kKvJoinWarps, L, acc);
       __syncthreads();  // the sums before have been read
 #pragma unroll
       for (int d = 0; d < PER; ++d) s_o[warp][PER * lane + d] = acc[d];
