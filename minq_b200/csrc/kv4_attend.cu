@@ -54,7 +54,7 @@
 // 47 us at the measured copy rate) take 89 us, 3.4 TB/s: the two f16 parts and the
 // scales cost about 400 warp instructions per 16 positions of a kv head, and a
 // scheduler issues one in 0.67 of its cycles. 2 x 131071 positions of 2 kv heads
-// of 64 take 36 us (41 MB), half of it the join; 1 x 1000 positions 19 us, the
+// of 64 take 31 us (41 MB), a third of it the join; 1 x 1000 positions 18 us, the
 // launches and the dependent loads.
 #include <limits.h>
 #include <math.h>
@@ -1127,7 +1127,7 @@ minq_status launch_kv4_join(Kv4AttnParams p, const Kv4AttnParams* u, cudaStream_
   // With few items (of one token each) every one has many pieces: their columns
   // are spread over blocks, and few blocks look for them. With many there are
   // some in every CTA. Measured (join alone, us): 2 x 131071 positions of 2 kv
-  // heads 18 this way and 20 the other, 64 x 8192 of 8 kv heads 18 and 9.
+  // heads 13 this way and 24 the other, 64 x 8192 of 8 kv heads 11 and 8.
   const bool few = (size_t)p.n_req * p.nkv * p.hgroups * 4 < (size_t)p.n_piece / kKvWarps;
   p.join_pieces = few ? kKvJoinRecs : kKvWarps;
   p.join_blocks = (p.n_piece + p.join_pieces - 1) / p.join_pieces;
