@@ -450,8 +450,9 @@ minq_status minq_generate_sampled(minq_model* m, minq_sampler* s, const uint32_t
 /* (quantize.rs:120-143, 20 bytes per 32 values: 6.4 times smaller than f32); */
 /* page_size is a power of two in 16..1024. Slot s is position s % page_size  */
 /* of page s / page_size. Request r's position i lies in page                 */
-/* table[r * table_stride + i / page_size]. One step of a batch: extend the   */
-/* tables, write each layer's new keys and values, attend, and draw a token   */
+/* table[r * table_stride + i / page_size]; a page belongs to one request.    */
+/* One step of a batch: extend the tables, write each layer's new keys and    */
+/* values, attend, and draw a token                                           */
 /* per row. All calls are asynchronous on `stream`, keep no state, and may be  */
 /* captured into a CUDA graph. All pointers are device memory.                */
 

@@ -131,6 +131,30 @@ def test_extend_and_trim_follow_the_list(mq, torch, n_req, page, width, steps):
         gpu.same(book)
 
 
+def test_steps_of_nothing(mq, torch):
+    """No requests, no tokens, no room for tokens, no free pages."""
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    free, n_free = dev(torch, [2, 0, 1]), dev(torch, [3])
+    s = mq.pages_extend(none, none, none.reshape(0, 4), free, n_free, 16, 3)
+    assert s.slots.tolist() == [-1] * 3 and s.positions.tolist() == [0] * 3
+    assert s.q_start.tolist() == [0] and s.n_free.tolist() == [3] and s.info.tolist() == [0, 0]
+    t = mq.pages_trim(none, none, none.reshape(0, 4), free, n_free, 16)
+    assert t.n_free.tolist() == [3] and t.info.tolist() == [0, 0] and free.tolist() == [2, 0, 1]
+    lens, table = dev(torch, [5, 0]), dev(torch, [[2, -1], [-1, -1]])
+    s = mq.pages_extend(lens, dev(torch, [0, 0]), table, free, n_free, 16, 0)
+    assert s.lens.tolist() == [5, 0] and s.q_start.tolist() == [0, 0, 0] and s.info.tolist() == [0, 0]
+    s = mq.pages_extend(lens, dev(torch, [11, 0]), table, free, dev(torch, [0]), 16, 11)
+    assert s.info.tolist() == [0, 0] and s.slots.tolist() == [2 * 16 + 5 + i for i in range(11)]
+    kp, vp = (mq.kv4_pool(3, 2, 16, 64) for _ in range(2))
+    rows = torch.empty(0, 2, 64, device="cuda")
+    empty = torch.empty(0, dtype=torch.int64, device="cuda")
+    mq.kv4_write(rows, rows, empty, kp, vp)
+    assert mq.kv4_read(empty, kp, vp)[0].shape == (0, 2, 64)
+    out = mq.kv4_attend(rows, dev(torch, [0]), none, none.reshape(0, 1), kp, vp)
+    assert out.shape == (0, 2, 64)
+    assert mq.sample_rows(torch.empty(0, 7, device="cuda"), torch.empty(0, device="cuda")).shape == (0,)
+
+
 def test_trim_undoes_extend(mq, torch):
     book = Book(7, 16, 9, 70, 3)
     gpu = Pages(torch, book)
@@ -980,3 +1004,8 @@ def test_serving_steps_end_to_end(mq, torch):
     book.trim([99, 0, 99])
     gpu.lens, gpu.n_free = cut.lens, cut.n_free
     gpu.same(book)
+
+
+def test_no_bounded_wait_gave_up(mq):
+    """After all of the above: no kernel left a mark in the status words."""
+    mq._lib.check(mq._lib.lib().minq_device_status())
