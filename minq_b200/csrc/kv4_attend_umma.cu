@@ -63,6 +63,8 @@ constexpr int kUThreads = 32 * (kUSoft + kUSum + kUVal + 4);
 // whole number of warpgroups): 120 + 176 + 2 x 64 + 56 <= 5 x 96.
 constexpr int kURegSoft = 120, kURegSum = 176, kURegVal = 64, kURegMma = 56;
 static_assert(kURegSoft + kURegSum + 2 * kURegVal + kURegMma <= 5 * 96, "registers");
+static_assert(kURegSoft >= 96 && kURegSum >= 96 && kURegVal <= 96 && kURegMma <= 96,
+              "setmaxnreg.inc may not lower the count, .dec not raise it");
 constexpr int kUValThreads = 32 * kUVal;
 constexpr int kUExtra = 256;     // an item's start and end, in positions
 constexpr int kUMinPiece = 512;  // smallest piece of the line per CTA
