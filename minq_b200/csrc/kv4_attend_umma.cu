@@ -35,7 +35,7 @@
 // f16 products each, so 0.83 PFLOP/s of the tensor cores' work; the mma.sync kernel
 // takes 670 us. A tile costs an SM 3,300 cycles, of which the tensor cores need
 // 1,400; softmax (2,700 of its warps' time) and values (2,200) run beside them but
-// share the issue slots, which are used in 0.55 of the cycles. The roles' loops are
+// share the issue slots, which are used in half of the cycles. The roles' loops are
 // kept short (one step of 16 columns, not four unrolled): together they have to fit
 // the instruction cache, and unrolled they took 352 us. Eight softmax warps that
 // took turns at the tiles, with fewer registers each, took 234 us.
