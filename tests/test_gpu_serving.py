@@ -735,6 +735,40 @@ def test_attend_pages_past_four_gigabytes(mq, torch):
     _check(torch, got, want, tol)
 
 
+@pytest.mark.parametrize("tokens,hd", [(100, 128), (100, 64), (3, 96)])
+def test_attend_kernels_past_four_gigabytes(mq, torch, tokens, hd):
+    """The same for a chunk's kernel and for the plain one."""
+    nh, nkv, page, n = 4, 4, 32, 150
+    n_pages = 2**32 // (nkv * page * (hd // 32 * 20)) + 100
+    kp = torch.empty(n_pages, nkv, page, hd // 32 * 20, dtype=torch.uint8, device="cuda")
+    vp = torch.empty_like(kp)
+    ids = [n_pages - 1, 5, n_pages - 2, n_pages // 2, n_pages - 9]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(2, n, nkv, hd, generator=g, device="cuda")
+    slots = torch.tensor([ids[i // page] * page + i % page for i in range(n)], device="cuda")
+    mq.kv4_write(x[0], x[1], slots, kp, vp)
+    k, v = mq.kv4_read(slots, kp, vp)
+    q = torch.randn(tokens, nh, hd, generator=g, device="cuda")
+    got = mq.kv4_attend(q, dev(torch, [0, tokens]), dev(torch, [n]), dev(torch, [ids]), kp, vp)
+    full = torch.zeros(5 * page, nkv, hd, dtype=torch.float64, device="cuda")
+    kv, vv = full.clone(), full.clone()
+    kv[:n], vv[:n] = k.double(), v.double()
+    want, tol = _reference(torch, q, [0, tokens], [n], dev(torch, [[0, 1, 2, 3, 4]]), page, kv, vv,
+                           hd ** -0.5)
+    _check(torch, got, want, tol)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,new", [(4, 1, 64, 20), (4, 1, 64, 3), (2, 1, 128, 64)])
+def test_attend_few_rows_of_a_long_history(mq, torch, nh, nkv, hd, new):
+    """More pieces of an item than one warp joins."""
+    lens, page = [70001], 64
+    kp, vp, table, kv, vv = _fill(mq, torch, 12, lens, nkv, hd, page)
+    q = torch.randn(new, nh, hd, device="cuda")
+    got = mq.kv4_attend(q, dev(torch, [0, new]), dev(torch, lens), table, kp, vp)
+    want, tol = _reference(torch, q, [0, new], lens, table, page, kv, vv, hd ** -0.5)
+    _check(torch, got, want, tol)
+
+
 def test_attend_equals_the_f32_cache_attention(mq, torch):
     """Next to minq_attend over the values that the cache stands for."""
     from minq_b200 import _lib
