@@ -45,7 +45,7 @@
 // choices, us at 64 x 151936 / 256 x 128257: 8 CTAs a row holding it in shared memory
 // 62 / 205, 4 holding it 70 / 234, 8 reading it again from L2 96 / 314, 4 so
 // 107 / 273; 384 threads a CTA 68 / 225, 512 79 / 258. A row that shared memory
-// cannot hold (more than 8 x 48 K tokens) is read again.
+// cannot hold (more than 8 x kRowsCached = 390784 tokens) is read again.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -67,8 +67,8 @@ constexpr int kRowsBuckets = 512;           // two per thread
 constexpr float kRowsPerNat = 32.0f;        // buckets per unit of (max - x) / T
 constexpr int kRowsList = 4 * kRowsThreads; // tokens a list holds: four per thread
 constexpr int kRowsMaxCtas = 8;             // the portable cluster size
-constexpr uint32_t kRowsCached = 48 * 1024; // floats of a row that a CTA can hold
 constexpr int kRowsTable = 256;
+constexpr size_t kRowsSmem = 227 * 1024;    // shared memory of a CTA
 
 struct RowsParams {
   const float* logits;
@@ -128,6 +128,14 @@ struct RowsShared {
   unsigned long long pickm;
   uint64_t bar;
 };
+
+// Floats of a row that a CTA can hold beside its static shared memory (eight
+// more: up to three of padding at either end, for the row's alignment).
+constexpr size_t rows_cached_smem(uint32_t chunk) { return ((size_t)chunk + 8) * sizeof(float); }
+constexpr uint32_t kRowsCached = (uint32_t)((kRowsSmem - sizeof(RowsShared)) / sizeof(float)) - 8;
+static_assert(sizeof(RowsShared) % 16 == 0, "the row is 16-byte aligned behind it");
+static_assert(sizeof(RowsShared) + rows_cached_smem(kRowsCached) <= kRowsSmem,
+              "static and dynamic shared memory of the longest row that is held");
 
 __device__ __forceinline__ RowsShared& rows_shared() {
   __shared__ RowsShared s;
@@ -1052,7 +1060,7 @@ minq_status minq_sample_rows(const float* logits, size_t row_stride, size_t n_ro
          (n > 19456u * ctas || (n_rows * ctas < (size_t)sm_count() && n > 4096u * ctas)))
     ctas *= 2;
   p.chunk = (uint32_t)((n + ctas - 1) / ctas);
-  p.cached = p.chunk <= kRowsCached - 4;
+  p.cached = p.chunk <= kRowsCached;
   int chunk_bits = 0, n_bits = 0;
   while ((1u << chunk_bits) < p.chunk) ++chunk_bits;
   while ((1u << n_bits) < p.n) ++n_bits;
@@ -1060,7 +1068,7 @@ minq_status minq_sample_rows(const float* logits, size_t row_stride, size_t n_ro
   p.part_bits = 32 - chunk_bits < 15 ? 32 - chunk_bits : 15;
   p.drop = 30 - 2 * p.part_bits;
   p.mass_bits = 62 - n_bits < 47 ? 62 - n_bits : 47;
-  const size_t smem = p.cached ? ((size_t)p.chunk + 8) * sizeof(float) : 0;
+  const size_t smem = p.cached ? rows_cached_smem(p.chunk) : 0;
   auto kernel = p.cached ? sample_rows_kernel<true> : sample_rows_kernel<false>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   MINQ_TRY(ensure_dynamic_smem(fn, smem));

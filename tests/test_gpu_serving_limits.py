@@ -1,0 +1,31 @@
+"""Serving-step operators where they had failed: ranges of sizes, borders and
+inputs on which a call was refused, answered wrongly or read too early."""
+import numpy as np
+import pytest
+
+from test_gpu_serving import _check, _draw, _fill, _reference, dev, torch  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- sampling -------------------------------------------------------------------
+
+def _rows(mq, torch, x, u, s):
+    f = lambda i, t=torch.float32: torch.tensor([v[i] for v in s], dtype=t, device="cuda")  # noqa: E731
+    got = mq.sample_rows(torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda(), temperature=f(0),
+                         top_k=f(1, torch.int32), top_p=f(2), min_p=f(3)).tolist()
+    want = [_draw(x[r], np.float64(u[r]), np.float64(np.float32(s[r][0])), s[r][1],
+                  np.float64(np.float32(s[r][2])), np.float64(np.float32(s[r][3])))
+            for r in range(len(s))]
+    assert got == want, [(r, a, b, s[r]) for r, (a, b) in enumerate(zip(got, want)) if a != b]
+
+
+@pytest.mark.parametrize("n", [390784, 390785, 393184, 393185])
+def test_sample_rows_around_what_shared_memory_holds(mq, torch, n):
+    """The longest rows that eight CTAs hold in shared memory, and the next ones."""
+    g = np.random.default_rng(n)
+    s = [(1.0, 0, 1.0, 0.0), (0.8, 50, 0.95, 0.0), (1.2, 0, 0.9, 0.0), (0.0, 0, 1.0, 0.0),
+         (1.0, 3000, 1.0, 0.01)]
+    x = g.standard_normal((len(s), n)).astype(np.float32) * 2.5
+    x[3, -1] = 40.0  # the greedy row's token is its last
+    _rows(mq, torch, x, g.random(len(s)).astype(np.float32), s)
