@@ -542,7 +542,8 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
  * sum top_p * sum(w); those with w >= min_p (never fewer than one). The token
  * is the first kept one whose running sum reaches u * (kept sum), in that
  * order when a filter is on and by index otherwise; logits of -infinity or
- * NaN are never drawn, and a row of nothing else gives token 0. Greedy rows
+ * NaN are never drawn, nor is one more than 745 T below the maximum (its w is 0
+ * in f64), and a row of nothing but -infinity and NaN gives token 0. Greedy rows
  * (also top_k = 1) take minq_argmax's token. Weights are fixed-point integers
  * to 2^-28 of themselves and their sums exact, so a result depends on no order;
  * temperatures below 1e-12 of the largest |logit| are treated alike.

@@ -11,7 +11,8 @@
 // and never less than the first token. The draw takes the first kept token
 // whose running sum reaches u * (kept sum): in rank order when a filter is
 // on, in index order otherwise. Tokens at -infinity (or NaN) have w = 0 and
-// are never drawn; a row without any other token gives token 0.
+// are never drawn, nor are others whose w is 0 in f64 (745 T below the maximum);
+// a row without any other token gives token 0.
 //
 // Next to a border a draw is decided by digits that an f32 sum over a
 // vocabulary does not hold (with 100,000 even tokens, borders moved by 1e-7 of
@@ -87,6 +88,14 @@ struct RowsParams {
 
 // Whether a token can be drawn (a number above -infinity).
 __device__ __forceinline__ bool rows_real(float v) { return v > -INFINITY; }
+
+// The least logit that weighs anything: below it exp((x - max) / T) is 0 even in
+// f64 (2^-1075 = e^-745.13). Only a uniform of 0 asks: any other target is reached
+// by a weight that the sums hold, 0 by whatever comes first, a mask of -1e9 too.
+// Rounded up, so that values next to a large maximum stay out.
+__device__ __forceinline__ float rows_floor(float max, float t) {
+  return fmaxf(__double2float_ru((double)max - 745.13 * (double)t), -3.402823466e+38f);
+}
 
 // Set when a bounded wait gave up (read and cleared by take_sample_rows_status).
 __device__ int g_rows_status;
@@ -183,6 +192,7 @@ struct Row {
   uint32_t base, count;  // its tokens
   uint32_t top;          // key of the maximum
   float fmax, per, low;  // buckets: (fmax - x) * per; what is below low weighs nothing
+  float drawn;           // the least logit of an unfiltered draw, see rows_floor
   double scale, shift;   // 256 log2(w) = x * scale + shift, plus kMagic
   int bits, drop;        // see RowsParams
   static constexpr double kMagic = 402653184.0;  // 1.5 * 2^28: 24 fractional bits
@@ -822,7 +832,7 @@ struct Search {
     uint32_t last = 0xffffffffu;
     for (uint32_t i = lo; i < hi; ++i) {
       const float v = row.at(i);
-      if (!rows_real(v)) continue;
+      if (!(v >= row.drawn)) continue;
       mine += row.value_weight(v);
       last = i;
     }
@@ -859,7 +869,7 @@ struct Search {
       uint32_t hit = last;
       for (uint32_t i = lo; i < hi; ++i) {
         const float v = row.at(i);
-        if (!rows_real(v)) continue;
+        if (!(v >= row.drawn)) continue;
         r += row.value_weight(v);
         if ((double)r >= target) {
           hit = i;
@@ -975,6 +985,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     const float tt = fmaxf(t, fmaxf(1e-30f, fabsf(row.fmax) * 1e-12f));
     row.per = kRowsPerNat / tt;
     row.low = row.fmax - 64.0f * tt;
+    row.drawn = rows_floor(row.fmax, tt);
     row.bits = p.mass_bits;
     row.drop = p.drop;
     row.scale = (kRowsTable * 1.4426950408889634074) / (double)tt;

@@ -29,3 +29,22 @@ def test_sample_rows_around_what_shared_memory_holds(mq, torch, n):
     x = g.standard_normal((len(s), n)).astype(np.float32) * 2.5
     x[3, -1] = 40.0  # the greedy row's token is its last
     _rows(mq, torch, x, g.random(len(s)).astype(np.float32), s)
+
+
+@pytest.mark.parametrize("n", [2, 100, 5000, 151936, 400001])
+@pytest.mark.parametrize("low", [-1e9, float(np.finfo(np.float32).min)])
+def test_sample_rows_never_draws_a_masked_token(mq, torch, n, low):
+    """A uniform of 0 takes the first token that weighs anything: masks of a very
+    low value count like -infinity, small weights do not."""
+    g = np.random.default_rng(n)
+    x = np.clip(g.standard_normal((4, n)), -4, 4).astype(np.float32)
+    x[0, :n // 2] = low
+    x[1] = low           # masks alone: they all weigh the same
+    x[2, :-1] = low
+    x[3, 0] = -200.0     # exp(-200) is a weight
+    u = np.zeros(4, np.float32)
+    _rows(mq, torch, x, u, [(1.0, 0, 1.0, 0.0)] * 4)
+    # at the lowest temperature: what a double still holds, and what it does not
+    y = np.full((2, n), 3.0, np.float32)
+    y[0, 0], y[1, 0] = 3.0 - 0.3 * 740, 3.0 - 0.3 * 750
+    _rows(mq, torch, y, u[:2], [(0.3, 0, 1.0, 0.0)] * 2)
