@@ -464,7 +464,9 @@ enum {
   MINQ_PAGES_ROW_FULL = 2,        /* a request does not fit its table row */
   MINQ_PAGES_TOO_MANY_TOKENS = 4, /* more new tokens than max_tokens */
   MINQ_PAGES_BAD_LENGTH = 8,      /* a negative length */
-  MINQ_PAGES_BAD_PAGE = 16        /* a page id or free count outside the pool */
+  MINQ_PAGES_BAD_PAGE = 16        /* a page id that the call uses, or the free count, outside the
+                                     pool (extend: new pages, and the partly filled ones that new
+                                     tokens go on in; trim: the pages given back) */
 };
 
 /* Grow request r (n_req <= 8192) from lens[r] to lens[r] + new_tokens[r]

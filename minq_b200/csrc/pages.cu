@@ -142,7 +142,8 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(PagesParams p) {
   for (int base = 0; base < p.n_req; base += nthreads) {
     const int r = base + tid;
     long long t = 0, g = 0;
-    int len = 0, from = 0;
+    int len = 0, from = 0, last = 0;
+    bool goes_on = false;
     if (r < p.n_req) {
       len = p.lens[r];
       const int arg = p.arg[r];
@@ -155,6 +156,10 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(PagesParams p) {
         } else {
           from = pages_of(len, shift);
           g = pages_of((int)after, shift) - from;
+          // the partly filled page that new tokens go on in (a column of the row,
+          // as len < after <= cap); looked at behind the scan, when it has come
+          goes_on = arg > 0 && (len & mask);
+          if (goes_on) last = p.table[(size_t)r * p.table_stride + (len >> shift)];
         }
         t = arg;
       } else {
@@ -165,6 +170,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(PagesParams p) {
     }
     long long tt, tg;
     scan2(t, g, tt, tg, sh);
+    if (goes_on && (last < 0 || last >= p.n_pages)) flags |= MINQ_PAGES_BAD_PAGE;
     // offsets past 2^31 only occur in a step that is refused below
     if (r < p.n_req) {
       s_page[r] = (int)(pages + g);
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(PagesParams p) {
         const int col = pos >> shift;
         const int id = col < s_base[r] ? p.table[(size_t)r * p.table_stride + col]
                                        : p.free_pages[n_free - 1 - (s_page[r] + (col - s_base[r]))];
-        slot = id < 0 || id >= p.n_pages ? -1 : ((long long)id << shift) + (pos & mask);
+        slot = ((long long)id << shift) + (pos & mask);
       }
       p.slots[t] = slot;
       if (p.positions) p.positions[t] = pos;

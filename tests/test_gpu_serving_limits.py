@@ -8,6 +8,37 @@ from test_gpu_serving import _check, _draw, _fill, _reference, dev, torch  # noq
 pytestmark = pytest.mark.gpu
 
 
+# ---- page tables ----------------------------------------------------------------
+
+@pytest.mark.parametrize("bad", [-1, 24, 2**31 - 1, -2**31])
+def test_extend_into_a_page_outside_the_pool_changes_nothing(mq, torch, bad):
+    """New tokens that go on in a partly filled page whose id is bad: the step is
+    refused (their keys and values would be lost). A bad id that no new token
+    reaches is none of the step's."""
+    def state():
+        return (dev(torch, [20, 32, 5, 0]),
+                dev(torch, [[3, 4, -1, -1], [bad, 6, -1, -1], [8, -1, -1, -1], [-1] * 4]),
+                dev(torch, [0, 1, 2, 10, 11, 12] + [-1] * 18), dev(torch, [6]))
+    for n, r in ((1, 0), (12, 0), (13, 2), (1, 2)):
+        lens, table, free, n_free = state()
+        table[r, int(lens[r]) // 16] = bad
+        new = [1, 1, 0, 3]
+        new[r] = n
+        before = [t.clone() for t in (lens, table, free, n_free)]
+        s = mq.pages_extend(lens, dev(torch, new), table, free, n_free, 16, 30)
+        assert s.info.tolist() == [mq.PAGES_BAD_PAGE, 0]
+        assert all(torch.equal(a, b) for a, b in zip(before, (lens, table, free, n_free)))
+        assert torch.equal(s.lens, lens) and torch.equal(s.n_free, n_free)
+        assert (s.slots == -1).all() and s.q_start.tolist() == [0] * 5
+        new[r] = 0  # the others' tokens alone
+        s = mq.pages_extend(lens, dev(torch, new), table, free, n_free, 16, 30)
+        assert s.info.tolist() == [0, 0] and (s.slots[:sum(new)] >= 0).all()
+    # full pages before the new tokens are not looked at
+    lens, table, free, n_free = state()
+    s = mq.pages_extend(lens, dev(torch, [0, 2, 0, 0]), table, free, n_free, 16, 2)
+    assert s.info.tolist() == [0, 0] and s.slots.tolist() == [12 * 16, 12 * 16 + 1]
+
+
 # ---- sampling -------------------------------------------------------------------
 
 def _rows(mq, torch, x, u, s):
