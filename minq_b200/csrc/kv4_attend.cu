@@ -72,7 +72,7 @@ namespace minq {
 namespace {
 
 // Request of token t, or -1 where t lies behind the last sequence (or the
-// starts are not a valid partition there).
+// starts are not a valid run of tokens there, see kv_req).
 __device__ __forceinline__ int kv4_request_of(const Kv4AttnParams& p, int t) {
   int lo = 0, hi = p.n_req;
   while (hi - lo > 1) {
@@ -82,7 +82,8 @@ __device__ __forceinline__ int kv4_request_of(const Kv4AttnParams& p, int t) {
     else
       hi = mid;
   }
-  return p.q_start[lo] <= t && t < p.q_start[lo + 1] ? lo : -1;
+  const int a = p.q_start[lo], b = p.q_start[lo + 1];
+  return a >= 0 && a <= t && t < b && b <= p.n_tokens ? lo : -1;
 }
 
 // One CTA per (token, query head), any head_dim that is a multiple of 32: the

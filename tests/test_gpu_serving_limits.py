@@ -39,6 +39,32 @@ def test_extend_into_a_page_outside_the_pool_changes_nothing(mq, torch, bad):
     assert s.info.tolist() == [0, 0] and s.slots.tolist() == [12 * 16, 12 * 16 + 1]
 
 
+# ---- attention ------------------------------------------------------------------
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (4, 2, 96), (4, 1, 32)])
+@pytest.mark.parametrize("T,starts,rows", [
+    (6, [-2, 1, 99], []), (6, [-1, 6, 7], []), (6, [0, 3, 99], [0, 1, 2]), (6, [5, 2, 4], [2, 3]),
+    (200, [-2, 100, 999], []), (200, [0, 100, 201], range(100)), (200, [-90, 100, 200], range(100, 200)),
+])
+def test_attend_requests_outside_the_tokens_have_none(mq, torch, nh, nkv, hd, T, starts, rows):
+    """A request whose run of tokens is not inside them is left out as a whole,
+    by every kernel alike; its rows stay as they were."""
+    lens, page = [120, 130], 16
+    kp, vp, table, kv, vv = _fill(mq, torch, 2, lens, nkv, hd, page)
+    q = torch.randn(T, nh, hd, device="cuda")
+    out = torch.full((T, nh, hd), 3.0, device="cuda")
+    mq.kv4_attend(q, dev(torch, starts), dev(torch, lens), table, kp, vp, out=out)
+    on = torch.zeros(T, dtype=torch.bool, device="cuda")
+    on[list(rows)] = True
+    assert (out[~on] == 3.0).all()
+    valid = [r for r in range(2) if 0 <= starts[r] < starts[r + 1] <= T]
+    for r in valid:
+        want, tol = _reference(torch, q, [starts[r], starts[r + 1]], [lens[r]], table[r:r + 1], page,
+                               kv, vv, hd ** -0.5)
+        _check(torch, out[starts[r]:starts[r + 1]], want[starts[r]:starts[r + 1]],
+               tol[starts[r]:starts[r + 1]])
+
+
 # ---- sampling -------------------------------------------------------------------
 
 def _rows(mq, torch, x, u, s):
