@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(kKvRowsWarps * 32) kv4_attend_rows_kernel(Kv4A
   const long long cap = (long long)p.table_stride << p.page_shift;
   const long long n = pos + 1 < cap ? pos + 1 : cap;  // positions seen (< 1: none)
   float m = -INFINITY, l = 0.0f, o[8] = {};
+  bool seen = false;
   for (long long p0 = 32 * warp; p0 < n; p0 += 32 * kKvRowsWarps) {
     // P >= 16: the 32 positions lie in one or two pages; a lane has its own row
     const long long i = p0 + lane;
@@ -133,9 +134,11 @@ __global__ void __launch_bounds__(kKvRowsWarps * 32) kv4_attend_rows_kernel(Kv4A
         s += acc * __uint_as_float(blk[0]);
       }
     }
-    const float mn = fmaxf(m, warp_max(s));
-    if (mn == -INFINITY) continue;  // nothing seen yet
-    const float a = expf(m - mn), w = on ? expf(s - mn) : 0.0f;
+    if (!__any_sync(0xffffffffu, on)) continue;
+    seen = true;
+    // (a maximum over NaN alone is -inf: the weights are NaN relative to anything)
+    const float mn = fmaxf(m, warp_max(s)), ref = mn == -INFINITY ? 0.0f : mn;
+    const float a = expf(m - ref), w = on ? expf(s - ref) : 0.0f;
     m = mn;
     l = l * a + w;
 #pragma unroll
@@ -164,20 +167,21 @@ __global__ void __launch_bounds__(kKvRowsWarps * 32) kv4_attend_rows_kernel(Kv4A
     s_m[warp] = m;
     s_l[warp] = l;
   }
-  __syncthreads();
+  const bool any = __syncthreads_or(seen) != 0;
   float M = -INFINITY;
 #pragma unroll
   for (int w = 0; w < kKvRowsWarps; ++w) M = fmaxf(M, s_m[w]);
+  const float ref = M == -INFINITY ? 0.0f : M;
   float* out = p.out + (size_t)t * p.out_stride + (size_t)h * p.hd;
   for (int d = threadIdx.x; d < p.hd; d += kKvRowsWarps * 32) {
     float sum = 0.0f, L = 0.0f;
-    for (int w = 0; w < kKvRowsWarps; ++w)
-      if (s_m[w] != -INFINITY) {  // a warp that saw something
-        const float a = expf(s_m[w] - M);
-        sum += s_o[w][d] * a;
-        L += s_l[w] * a;
-      }
-    out[d] = L != 0.0f ? sum / L : 0.0f;
+    for (int w = 0; w < kKvRowsWarps; ++w) {
+      const float a = expf(s_m[w] - ref);  // 0 for a warp that saw nothing, NaN stays NaN
+      sum += s_o[w][d] * a;
+      L += s_l[w] * a;
+    }
+    // what is seen but weighs nothing (every score -inf) is not a number
+    out[d] = any ? sum / L : 0.0f;
   }
 }
 

@@ -65,6 +65,37 @@ def test_attend_requests_outside_the_tokens_have_none(mq, torch, nh, nkv, hd, T,
                tol[starts[r]:starts[r + 1]])
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 2, 128), (4, 2, 96), (4, 1, 32), (2, 1, 256)])
+@pytest.mark.parametrize("lens,new", [([1, 40], [1, 1]), ([70, 300], [2, 1]), ([130, 90], [100, 70])])
+def test_attend_keeps_what_is_not_a_number(mq, torch, nh, nkv, hd, lens, new):
+    """A query row that holds NaN gives NaN, not the zeros of a row that sees
+    nothing; so do keys whose scales are NaN. Other rows do not notice."""
+    page = 16
+    kp, vp, table, kv, vv = _fill(mq, torch, 7, lens, nkv, hd, page)
+    start = [0, new[0], sum(new)]
+    q = torch.randn(start[-1], nh, hd, device="cuda")
+    args = (dev(torch, start), dev(torch, lens), table, kp, vp)
+    clean = mq.kv4_attend(q, *args)
+    assert torch.isfinite(clean).all()
+    bad = q.clone()
+    bad[0, 1, hd // 2] = float("nan")
+    bad[start[-1] - 1, 0] = float("nan")
+    got = mq.kv4_attend(bad, *args)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[0, 1], hit[start[-1] - 1, 0] = True, True
+    assert torch.isnan(got[hit]).all()
+    want, tol = _reference(torch, q, start, lens, table, page, kv, vv, hd ** -0.5)
+    want[hit.any(-1).any(-1)] = float("nan")  # (their other heads: below)
+    _check(torch, torch.where(hit, 0.0, got), want, tol)
+    assert torch.isfinite(got[~hit]).all()
+    # every key of request 0
+    blocks = kp.view(kp.shape[0], nkv, page, hd // 32, 20)
+    blocks[table[0, :-(-lens[0] // page)].long(), :, :, 0, :4] = torch.tensor(
+        [float("nan")], device="cuda").view(torch.uint8)
+    got = mq.kv4_attend(q, *args)
+    assert torch.isnan(got[:start[1]]).all() and torch.isfinite(got[start[1]:]).all()
+
+
 # ---- sampling -------------------------------------------------------------------
 
 def _rows(mq, torch, x, u, s):
