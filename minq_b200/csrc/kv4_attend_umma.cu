@@ -499,6 +499,9 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
         const int k1 = min(k, 14), k2 = min(k - k1, 24);
         const __half2 f1 = __float2half2_rn(__uint_as_float((uint32_t)(127 - k1) << 23)),
                       f2 = __float2half2_rn(__uint_as_float((uint32_t)(127 - k2) << 23));
+        // the parts that are read back were stored asynchronously (by the steps
+        // before and by earlier moves), and a load may pass a store
+        tm_wait_st();
         for (int y = 0; y < x; ++y) {
           float v[16];
           uint32_t part[16];

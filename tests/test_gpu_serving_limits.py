@@ -96,6 +96,38 @@ def test_attend_keeps_what_is_not_a_number(mq, torch, nh, nkv, hd, lens, new):
     assert torch.isnan(got[:start[1]]).all() and torch.isfinite(got[start[1]:]).all()
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (14, 2, 64)])
+@pytest.mark.parametrize("page", [16, 64])
+def test_attend_chunks_whose_maximum_moves_within_a_tile(mq, torch, nh, nkv, hd, page):
+    """Scores that grow in steps of 6 to 40 log2 units at every step of 16 columns
+    of a tile (the columns' positions are 2 x, 2 x + 1 mod 8), in some tiles over
+    several tiles: the weights stored before are read back and scaled each time."""
+    lens, new = [515, 200], [70, 130]
+    kp, vp, table, kv, vv = _fill(mq, torch, 4, lens, nkv, hd, page)
+    n_pages = kp.shape[0]
+    g = torch.Generator(device="cuda").manual_seed(2)
+    u = torch.nn.functional.normalize(torch.randn(nkv, hd, generator=g, device="cuda"), dim=-1)
+    pos = torch.zeros(n_pages * page, device="cuda")  # position of a slot
+    for r, n in enumerate(lens):
+        i = torch.arange(n, device="cuda")
+        pos[table[r].long()[i // page] * page + i % page] = i.float()
+    step, tile = (pos.int() % 8) // 2, pos.int() // 64
+    rise = torch.tensor([6.0, 11.0, 40.0], device="cuda")[tile.long() % 3]
+    level = (step * rise + torch.where(tile % 4 == 3, 130.0, 0.0) + 0.3 * torch.randn(
+        pos.shape, generator=g, device="cuda")) * 0.6931472 + torch.where(tile % 2 == 1, -20.0, 0.0)
+    k = (level[:, None, None] * u).contiguous()
+    mq.kv4_write(k, k, torch.arange(n_pages * page, device="cuda"), kp, mq.kv4_pool(*kp.shape[:3], hd))
+    kv = mq.kv4_read(torch.arange(n_pages * page, device="cuda"), kp, vp)[0].double()
+    start = [0, new[0], sum(new)]
+    q = u.repeat_interleave(nh // nkv, 0)[None] * (1 + 0.1 * torch.rand(
+        start[-1], nh, 1, generator=g, device="cuda"))
+    q = q.contiguous()
+    got = mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp, scale=1.0)
+    want, tol = _reference(torch, q, start, lens, table, page, kv, vv, 1.0)
+    _check(torch, got, want, tol)
+    assert torch.equal(got, mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp, scale=1.0))
+
+
 # ---- sampling -------------------------------------------------------------------
 
 def _rows(mq, torch, x, u, s):
