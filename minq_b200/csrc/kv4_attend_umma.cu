@@ -25,7 +25,12 @@
 //   warps 8-15   values: raw tile -> Kh Kl, Vh Vl in 128-byte swizzled tiles.
 //   warps 17-19  bulk copies, K's scales, V's scales.
 //   warp 16      one thread issues the MMAs: S of the next tile, then P V.
-// S, O and the K and V tiles are double buffered; TMEM: Qh Ql, 2 S, 2 O.
+// K and V tiles are double buffered; TMEM: Qh Ql, 4 S, O (512 columns at head_dim
+// 128). P takes the place of its S, and MMAs of other accumulators and shapes may run
+// in another order than they were issued in: S of tile g + 3 and later only may
+// overwrite P of tile g, since P V of g + 1 waits until O of g has been read. (Two
+// places of S and two of O, where S of g + 2 has to wait for P V of g by itself, took
+// 259 us for the case below.)
 // The order of dimensions inside S's contraction and of positions inside
 // P V's is free, so both are chosen for the code layout and for stores without
 // bank conflicts (q_dim and the packing of P follow them).
@@ -69,6 +74,7 @@ constexpr int kUValThreads = 32 * kUVal;
 constexpr int kUExtra = 256;     // an item's start and end, in positions
 constexpr int kUMinPiece = 512;  // smallest piece of the line per CTA
 constexpr int kURaw = 4;         // raw tiles in flight
+constexpr int kUScores = 4;      // places for S and P
 
 template <int HD>
 struct UmGeom {
@@ -78,7 +84,8 @@ struct UmGeom {
   static constexpr int KT = kUTile * HD * 2;   // Kh, Kl, Vh or Vl
   static constexpr int K = 0, V = 4 * KT, R = 8 * KT, CTL = R + kURaw * RAW;
   // TMEM columns
-  static constexpr int QH = 0, QL = HD / 2, S = HD, O = HD + 2 * kUTile;
+  static constexpr int QH = 0, QL = HD / 2, S = HD, O = HD + kUScores * kUTile;
+  static_assert(O + HD <= 512, "tensor memory");
 };
 
 struct UmCtl {
@@ -93,8 +100,8 @@ struct UmCtl {
   uint32_t bad[8][8];           // not finite value scales: word and bit of (position * NB + block)
   int raw_ok[kURaw];
   uint64_t raw_full[kURaw], raw_free[kURaw], scale_full[kURaw];
-  uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], o_free[2];
-  uint64_t q_full, drain;
+  uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
+  uint64_t o_free, q_full, drain;
   uint32_t tmem;
   int abort, more, req;
   long long req_start, red[kUThreads / 32];
@@ -463,6 +470,7 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
   float m = -INFINITY, l = 0.0f;
   for (int i = 0; i < tl.n; ++i) {
     const uint32_t g = g0 + i, st = g & 1;
+    const uint32_t place = tlane + GM::S + g % kUScores * kUTile;
     if (!um_wait(&c.s_full[st], (g >> 1) & 1, &c.abort)) return;
     fence_after();
     const int pos0 = (tl.first + i) * kUTile, ok = c.ok[g & 7];
@@ -505,12 +513,12 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
         for (int y = 0; y < x; ++y) {
           float v[16];
           uint32_t part[16];
-          tm_ld16(tlane + GM::S + st * kUTile + 16 * y, v);
+          tm_ld16(place + 16 * y, v);
           tm_wait_ld16(v);
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             part[e] = h2_bits(__hmul2(__hmul2(bits_h2(__float_as_uint(v[e])), f1), f2));
-          tm_st16(tlane + GM::S + st * kUTile + 16 * y, part);
+          tm_st16(place + 16 * y, part);
         }
       }
       const float off = m == -INFINITY ? 0.0f : 10.0f - m;
@@ -523,12 +531,12 @@ __device__ __forceinline__ void um_softmax(const Kv4AttnParams& p, UmCtl& c, con
         add_f2(sum, s + e);
         split2(s[e], s[e + 1], part[e / 2], part[e / 2 + 8]);
       }
-      tm_st16(tlane + GM::S + st * kUTile + 16 * x, part);
+      tm_st16(place + 16 * x, part);
     };
 #pragma unroll 1
     for (int x = 0; x < kUTile / 16; ++x) {
       float s[16];
-      tm_ld16(tlane + GM::S + st * kUTile + 16 * x, s);
+      tm_ld16(place + 16 * x, s);
       tm_wait_ld16(s);
       process(x, s);
     }
@@ -561,7 +569,7 @@ __device__ __forceinline__ void um_mma(UmCtl& c, uint32_t tmem, uint32_t base, U
   const int n = __shfl_sync(0xffffffffu, tl.n, 0);
   if (!um_wait(&c.q_full, items & 1, &c.abort)) return;
   auto scores = [&](int i) {
-    const uint32_t g = g0 + i, st = g & 1, d = tmem + GM::S + st * kUTile;
+    const uint32_t g = g0 + i, st = g & 1, d = tmem + GM::S + g % kUScores * kUTile;
     const uint32_t kt = sw128_lo(base + GM::K + st * 2 * GM::KT);
     if (!um_wait(&c.k_full[st], (g >> 1) & 1, &c.abort)) return false;
     fence_after();
@@ -581,10 +589,10 @@ __device__ __forceinline__ void um_mma(UmCtl& c, uint32_t tmem, uint32_t base, U
   for (int i = 0; i < n; ++i) {
     if (i + 1 < n && !scores(i + 1)) return;
     const uint32_t g = g0 + i, st = g & 1, par = (g >> 1) & 1;
-    const uint32_t a = tmem + GM::S + st * kUTile, d = tmem + GM::O + st * HD;
+    const uint32_t a = tmem + GM::S + g % kUScores * kUTile, d = tmem + GM::O;
     const uint32_t vt = sw128_lo(base + GM::V + st * 2 * GM::KT);
     if (!um_wait(&c.v_full[st], par, &c.abort)) return;
-    if (g >= 2 && !um_wait(&c.o_free[st], par ^ 1, &c.abort)) return;
+    if (g >= 1 && !um_wait(&c.o_free, (g - 1) & 1, &c.abort)) return;
     if (!um_wait(&c.p_full[st], par, &c.abort)) return;
     fence_after();
 #pragma unroll
@@ -667,14 +675,14 @@ __device__ __forceinline__ void um_sums(const Kv4AttnParams& p, UmCtl& c, const 
 #pragma unroll
     for (int d0 = 0; d0 < HD; d0 += 16) {
       float o[16];
-      tm_ld16(col + st * HD + d0, o);
+      tm_ld16(col + d0, o);
       tm_wait_ld16(o);
       const float fn = (nan >> (d0 / 32)) & 1 ? NAN : f;
 #pragma unroll
       for (int d = 0; d < 16; d += 2) fma_acc2(acc + d0 + d, o + d, fn);
     }
     fence_before();
-    mbar_arrive(&c.o_free[st]);
+    mbar_arrive(&c.o_free);
   }
   __syncthreads();
   if (on) {
@@ -736,8 +744,8 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
         mbar_init(&c.s_full[i], 1);
         mbar_init(&c.p_full[i], 32 * kUSoft);
         mbar_init(&c.pv_done[i], 1);
-        mbar_init(&c.o_free[i], 32 * kUSum);
       }
+      mbar_init(&c.o_free, 32 * kUSum);
       mbar_init(&c.q_full, 32 * kUSum);
       mbar_init(&c.drain, 1);
       c.abort = 0;

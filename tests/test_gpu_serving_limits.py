@@ -128,6 +128,23 @@ def test_attend_chunks_whose_maximum_moves_within_a_tile(mq, torch, nh, nkv, hd,
     assert torch.equal(got, mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp, scale=1.0))
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 4, 128), (8, 2, 64)])
+def test_attend_chunks_of_every_number_of_tiles(mq, torch, nh, nkv, hd):
+    """Chunks of one to thirteen tiles one behind the other in a CTA: the places of
+    scores, weights, outputs and their barriers' phases go on from item to item."""
+    page = 32
+    lens = [64 * t + d for t in range(1, 14) for d in (-3, 0, 17)]
+    new = [61 if n < 64 else 64 for n in lens]
+    kp, vp, table, kv, vv = _fill(mq, torch, 11, lens, nkv, hd, page)
+    start = [0] + np.cumsum(new).tolist()
+    q = torch.randn(start[-1], nh, hd, device="cuda")
+    args = (q, dev(torch, start), dev(torch, lens), table, kp, vp)
+    got = mq.kv4_attend(*args)
+    want, tol = _reference(torch, q, start, lens, table, page, kv, vv, hd ** -0.5)
+    _check(torch, got, want, tol)
+    assert all(torch.equal(got, mq.kv4_attend(*args)) for _ in range(20))
+
+
 # ---- sampling -------------------------------------------------------------------
 
 def _rows(mq, torch, x, u, s):
