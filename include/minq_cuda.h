@@ -569,6 +569,15 @@ void* minq_model_stream(minq_model* m);
  * MINQ_ERR_ARG when the model does not use the decode megakernel. */
 minq_status minq_debug_inject_timeout(minq_model* m, int what);
 
+/* The same for the serving step: the waits of the next launch of one kernel for
+ * its bulk copies also expect 16 bytes that nothing sends, so they run out after
+ * the wait limit (1 s each). kernel = 0: minq_kv4_attend's for single tokens and
+ * short runs; 1: its kernel for prompt chunks; 2: minq_sample_rows (rows that
+ * shared memory holds). The call itself returns MINQ_OK, as it is asynchronous;
+ * minq_device_status then returns MINQ_ERR_TIMEOUT once, the call's output holds
+ * nothing defined, and later calls run normally. Not for a launch that is captured. */
+minq_status minq_debug_inject_stall(int kernel);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,6 +135,7 @@ SIGNATURES = {
                             P]),
     "minq_sample_rows": (I, [P, S, S, S, P, P, P, P, P, P, P]),
     "minq_debug_inject_timeout": (I, [P, I]),
+    "minq_debug_inject_stall": (I, [I]),
 }
 
 _lib = None

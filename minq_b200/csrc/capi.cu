@@ -124,6 +124,13 @@ minq_status require_device() {
   return MINQ_OK;
 }
 
+static std::atomic<uint32_t> g_stall[kStallKernels];
+
+uint32_t take_stall(StallKernel kernel) {
+  // (the exchange only where something was asked for: this is on every launch's way)
+  return g_stall[kernel].load(std::memory_order_relaxed) ? g_stall[kernel].exchange(0) : 0u;
+}
+
 static bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 // ---- kernel timer ----
@@ -184,6 +191,13 @@ minq_status minq_device_status(void) {
   const minq_status c = take_kv4_status();
   const minq_status d = take_sample_rows_status();
   return a != MINQ_OK ? a : b != MINQ_OK ? b : c != MINQ_OK ? c : d;
+}
+
+minq_status minq_debug_inject_stall(int kernel) {
+  if (kernel < 0 || kernel >= kStallKernels)
+    return fail(MINQ_ERR_ARG, "kernel: 0 (kv4_attend), 1 (its prompt chunks) or 2 (sample_rows)");
+  g_stall[kernel].store(16);
+  return MINQ_OK;
 }
 
 minq_status minq_kernel_timer_start(const char* family) {

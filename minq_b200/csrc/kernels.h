@@ -167,6 +167,10 @@ minq_status launch_advance_pos(int* pos, int by, cudaStream_t s);
 // pages.cu: page sizes of the paged 4-bit cache (a power of two in 16..1024,
 // so that 16 positions lie in one page and a 16-byte aligned run)
 bool kv4_page_size_ok(size_t page_size);
+// Bytes that the next launch of a serving kernel expects beyond its copies (0, or
+// once what minq_debug_inject_stall(kernel) asked for).
+enum StallKernel { kStallAttend, kStallAttendChunks, kStallSampleRows, kStallKernels };
+uint32_t take_stall(StallKernel kernel);
 // sampler.cu: the device a sampler was created on
 int sampler_device(const minq_sampler* s);
 // per-row negative log-likelihood (ppl.rs:30-35) of logits [rows][V] at

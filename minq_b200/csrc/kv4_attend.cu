@@ -618,7 +618,7 @@ __device__ __forceinline__ void kv_run(const Kv4AttnParams& p, const KvItem& it,
     if (lane == 0 && ring.alive) {
       const uint32_t n = (have & 1) + ((have >> 1) & 1);
       if (n)
-        mbar_arrive_expect_tx(bar, n * 2 * GM::HALF);
+        mbar_arrive_expect_tx(bar, n * 2 * GM::HALF + p.stall);
       else
         mbar_arrive(bar);
     }
@@ -1242,6 +1242,7 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
     p.n_lo = 1;
     p.n_hi = plan.umma_lo ? plan.umma_lo - 1 : INT_MAX;
     p.extra = kKvExtra;
+    p.stall = take_stall(kStallAttend);
     p.n_piece = plan.n_cta * kKvWarps;
     p.rec = static_cast<KvRec*>(workspace);
     p.part_o = reinterpret_cast<float*>(p.rec + p.n_piece);

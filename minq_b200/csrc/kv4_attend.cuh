@@ -40,6 +40,7 @@ struct Kv4AttnParams {
   float* part_o;     // [n_piece][2][cols][hd] unnormalised partial outputs
   float* part_ml;    // [n_piece][2][cols][2] their maxima and sums
   KvRec* rec;        // [n_piece]
+  uint32_t stall;    // bytes a tile's wait expects beyond its copies (tests)
 };
 
 __device__ __forceinline__ float ex2(float x) {
