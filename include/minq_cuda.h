@@ -575,7 +575,8 @@ minq_status minq_debug_inject_timeout(minq_model* m, int what);
  * short runs; 1: its kernel for prompt chunks; 2: minq_sample_rows (rows that
  * shared memory holds). The call itself returns MINQ_OK, as it is asynchronous;
  * minq_device_status then returns MINQ_ERR_TIMEOUT once, the call's output holds
- * nothing defined, and later calls run normally. Not for a launch that is captured. */
+ * nothing defined (minq_sample_rows: token 0 for the rows that did not come), and
+ * later calls run normally. Not for a launch that is captured. */
 minq_status minq_debug_inject_stall(int kernel);
 
 #ifdef __cplusplus

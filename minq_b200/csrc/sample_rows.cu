@@ -84,6 +84,7 @@ struct RowsParams {
   const float* min_p;        // null or <= 0: off
   const float* u;
   uint32_t* out;
+  uint32_t stall;            // bytes the row's wait expects beyond its copies (tests)
 };
 
 // Whether a token can be drawn (a number above -infinity).
@@ -908,6 +909,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   }
   __syncthreads();
   pdl_wait();
+  bool got = true;  // the row has come
   if (CACHED) {
     // the 16-byte aligned middle by bulk copies, the ragged ends by loads; the
     // copy keeps the row's misalignment, the ends are padded
@@ -915,7 +917,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     float* dst = s_row + mis;
     const uint32_t head = min(row.count, (4 - mis) & 3), body = (row.count - head) / 4 * 4;
     if (tid == 0 && body) {
-      mbar_arrive_expect_tx(&sh.bar, body * 4);
+      mbar_arrive_expect_tx(&sh.bar, body * 4 + p.stall);
       for (uint32_t o = 0; o < body; o += 4096)
         bulk_g2s(dst + head + o, src + head + o, min(4096u, body - o) * 4, &sh.bar);
     }
@@ -924,8 +926,11 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     if ((uint32_t)tid < head) dst[tid] = src[tid];
     if (tid < 4 && tail + tid < row.count) dst[tail + tid] = src[tail + tid];
     if (tid < 4 && end + tid < (end + 3) / 4 * 4) s_row[end + tid] = __uint_as_float(kRowsPad);
-    if (body) mbar_wait_timed(&sh.bar, 0, &g_rows_status);
-    __syncthreads();
+    if (body) {
+      got = mbar_wait_timed(&sh.bar, 0, &g_rows_status);
+      if (!got) mbar_wait_timed(&sh.bar, 0, &g_rows_status);  // the copies still in flight
+    }
+    got = __syncthreads_and(got) != 0;
     row.x = s_row;
     row.first = row.base - mis;
     row.n4 = (end + 3) / 4;
@@ -959,13 +964,15 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   if (lane == 0) sh.redu[warp] = best;
   __syncthreads();
   best = warp_max_u64(lane < kRowsWarps ? sh.redu[lane] : 0ull);
-  if (tid == 0) sh.best = best;
+  // a row that did not come in one CTA is none in all: the highest key stands for
+  // it (with index 0; a greedy row's NaN of that key and index gives token 0 anyway)
+  if (tid == 0) sh.best = got ? best : ~0ull;
   cl.sync();
   best = warp_max_u64(rows_lane<unsigned long long>(
       ctas, [&](int q) { return *cl.map_shared_rank(&sh.best, q); }));
   row.top = (uint32_t)(best >> 32);
   uint32_t token = 0xffffffffu;  // set in the CTA that writes it
-  if (greedy) {
+  if (greedy || best == ~0ull) {
     if (rank == 0) token = ~(uint32_t)best;
   } else if (row.top <= kKeyNone) {
     if (rank == 0) token = 0;  // nothing to draw from
@@ -1079,6 +1086,7 @@ minq_status minq_sample_rows(const float* logits, size_t row_stride, size_t n_ro
   p.part_bits = 32 - chunk_bits < 15 ? 32 - chunk_bits : 15;
   p.drop = 30 - 2 * p.part_bits;
   p.mass_bits = 62 - n_bits < 47 ? 62 - n_bits : 47;
+  p.stall = take_stall(kStallSampleRows);
   const size_t smem = p.cached ? rows_cached_smem(p.chunk) : 0;
   auto kernel = p.cached ? sample_rows_kernel<true> : sample_rows_kernel<false>;
   const void* fn = reinterpret_cast<const void*>(kernel);

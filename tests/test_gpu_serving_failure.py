@@ -54,3 +54,16 @@ def _attend(mq, torch, nh, nkv, hd, lens, new):
 @pytest.mark.parametrize("lens", [[300, 5000], [20]])
 def test_attend_wait_runs_out(mq, torch, nh, nkv, hd, new, lens):
     _stalled(mq, torch, 0, _attend(mq, torch, nh, nkv, hd, lens, [new] * len(lens)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(1, 5000), (3, 151936), (40, 20000)])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_sample_rows_wait_runs_out(mq, torch, rows, n, temperature):
+    """Every row of the stalled call gets token 0."""
+    x, u = torch.randn(rows, n, device="cuda"), torch.rand(rows, device="cuda")
+    x[:, 0] = -5.0
+    t = torch.full((rows,), temperature, device="cuda")
+    tp = torch.full((rows,), 0.9, device="cuda")
+    got, _ = _stalled(mq, torch, 2, lambda: mq.sample_rows(x, u, temperature=t, top_p=tp))
+    assert not got.any()
