@@ -1237,6 +1237,7 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
     if (plan.umma_lo) {
       u.n_lo = plan.umma_lo;
       u.n_hi = INT_MAX;
+      u.stall = take_stall(kStallAttendChunks);
       MINQ_TRY(launch_kv4_umma(u, static_cast<uint8_t*>(workspace) + plan.ws, s));
     }
     p.n_lo = 1;

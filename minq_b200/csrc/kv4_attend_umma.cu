@@ -278,10 +278,11 @@ __device__ __forceinline__ UmTiles um_tiles(const KvItem& it) {
   return {a, max(b - a, 0)};
 }
 
-// Copies: one warp, whose lanes 0..7 take a run of K or V each.
+// Copies: one warp, whose lanes 0..7 take a run of K or V each. Returns the number
+// of tiles issued.
 template <int HD>
-__device__ __forceinline__ void um_copies(const Kv4AttnParams& p, UmCtl& c, const KvItem& it, uint8_t* sm,
-                                          UmTiles tl, uint32_t g0) {
+__device__ __forceinline__ int um_copies(const Kv4AttnParams& p, UmCtl& c, const KvItem& it, uint8_t* sm,
+                                         UmTiles tl, uint32_t g0) {
   using GM = UmGeom<HD>;
   const int lane = threadIdx.x & 31, run = lane & 3, lim_max = it.lim_max;
   const uint8_t* side =
@@ -293,18 +294,16 @@ __device__ __forceinline__ void um_copies(const Kv4AttnParams& p, UmCtl& c, cons
     return lane < 8 && i < tl.n && pos < lim_max ? tab[pos >> p.page_shift] : -1;
   };
   int id = load_id(0), i = 0;
-  bool alive = true;
   for (; i < tl.n; ++i) {
     const int id_next = load_id(i + 1);
     const uint32_t g = g0 + i, st = g % kURaw;
-    if (g >= kURaw) alive = um_wait(&c.raw_free[st], (g / kURaw - 1) & 1, &c.abort);
-    if (!alive) break;
+    if (g >= kURaw && !um_wait(&c.raw_free[st], (g / kURaw - 1) & 1, &c.abort)) break;
     const bool on = id >= 0 && id < p.n_pages;
     const uint32_t have = __ballot_sync(0xffffffffu, on) & 15u;
     if (lane == 0) {
       c.raw_ok[st] = (int)have;
       if (have)
-        mbar_arrive_expect_tx(&c.raw_full[st], 2 * __popc(have) * GM::RUN);
+        mbar_arrive_expect_tx(&c.raw_full[st], 2 * __popc(have) * GM::RUN + p.stall);
       else
         mbar_arrive(&c.raw_full[st]);
     }
@@ -316,9 +315,7 @@ __device__ __forceinline__ void um_copies(const Kv4AttnParams& p, UmCtl& c, cons
     }
     id = id_next;
   }
-  if (!alive)  // let the copies in flight end
-    for (int k = i > kURaw ? i - kURaw : 0; k < i; ++k)
-      mbar_wait_timed(&c.raw_full[(g0 + k) % kURaw], ((g0 + k) / kURaw) & 1, &g_kv4_umma_status);
+  return i;
 }
 
 // Scales: one warp for K's, one for V's.
@@ -868,20 +865,26 @@ __global__ void __launch_bounds__(kUThreads, 1) kv4_umma_kernel(const __grid_con
     __syncthreads();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kURegMma));
+    uint32_t issued = 0;  // tiles whose copies this warp has issued
     for (uint32_t items = 0; more; ++items) {
       tl = um_tiles(c.item[cur]);
       if (warp == kMmaWarp) um_mma<HD>(c, tmem, base, tl, g0, items);
-      if (warp == kMmaWarp + 1) um_copies<HD>(p, c, c.item[cur], sm, tl, g0);
+      if (warp == kMmaWarp + 1) issued = g0 + um_copies<HD>(p, c, c.item[cur], sm, tl, g0);
       if (warp == kMmaWarp + 2) um_scales<HD, false>(c, c.item[cur], sm, tl, g0);
       if (warp == kMmaWarp + 3) um_scales<HD, true>(c, c.item[cur], sm, tl, g0);
       __syncwarp();
       __syncthreads();
       next();
     }
-    if (tid == 32 * kMmaWarp && c.abort) {  // after a wait that gave up: let the MMAs end
-      mma_commit(&c.drain);
+    // after a wait that gave up, anyone's: let the MMAs and the copies end
+    if (warp == kMmaWarp && c.abort) {
+      if (elect_lane()) mma_commit(&c.drain);  // the lane that issues them
+      __syncwarp();
       mbar_wait_timed(&c.drain, 0, &g_kv4_umma_status);
     }
+    if (warp == kMmaWarp + 1 && c.abort)
+      for (uint32_t g = issued > kURaw ? issued - kURaw : 0; g < issued; ++g)
+        mbar_wait_timed(&c.raw_full[g % kURaw], (g / kURaw) & 1, &g_kv4_umma_status);
     __syncthreads();
   }
 }

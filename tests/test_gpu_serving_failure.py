@@ -57,6 +57,14 @@ def test_attend_wait_runs_out(mq, torch, nh, nkv, hd, new, lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (14, 2, 64)])
+@pytest.mark.parametrize("lens,new", [([64], [64]), ([900, 3000, 40], [200, 64, 1])])
+def test_attend_chunk_wait_runs_out(mq, torch, nh, nkv, hd, lens, new):
+    """Tensor memory and the copies in flight are let go: the next calls run."""
+    _stalled(mq, torch, 1, _attend(mq, torch, nh, nkv, hd, lens, new))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,n", [(1, 5000), (3, 151936), (40, 20000)])
 @pytest.mark.parametrize("temperature", [0.0, 1.0])
 def test_sample_rows_wait_runs_out(mq, torch, rows, n, temperature):
