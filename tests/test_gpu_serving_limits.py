@@ -145,6 +145,26 @@ def test_attend_chunks_of_every_number_of_tiles(mq, torch, nh, nkv, hd):
     assert all(torch.equal(got, mq.kv4_attend(*args)) for _ in range(20))
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 4, 64), (8, 2, 128)])
+@pytest.mark.parametrize("qs,qo,os_,oo", [(1, 1, 1, 3), (0, 0, 2, 0), (3, 0, 0, 2)])
+def test_attend_chunk_rows_off_sixteen_bytes(mq, torch, nh, nkv, hd, qs, qo, os_, oo):
+    """Queries and outputs of a chunk whose rows do not start on 16 bytes, whole
+    items and pieces of one alike; nothing beside the rows is touched."""
+    page, lens, new = 32, [100, 9000, 64], [70, 65, 1]
+    start = [0] + np.cumsum(new).tolist()
+    T, w = start[-1], nh * hd
+    kp, vp, table, kv, vv = _fill(mq, torch, 4, lens, nkv, hd, page)
+    base = torch.randn(T * (w + qs) + 8, device="cuda")
+    q = torch.as_strided(base, (T, nh, hd), (w + qs, hd, 1), qo)
+    room = torch.full((T * (w + 64 + os_) + 8,), 9.0, device="cuda")
+    out = torch.as_strided(room, (T, nh, hd), (w + 64 + os_, hd, 1), oo)
+    mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp, out=out)
+    want, tol = _reference(torch, q, start, lens, table, page, kv, vv, hd ** -0.5)
+    _check(torch, out, want, tol)
+    gaps = torch.as_strided(room, (T, 64 + os_), (w + 64 + os_, 1), oo + w)
+    assert (gaps == 9.0).all() and (room[:oo] == 9.0).all()
+
+
 # ---- sampling -------------------------------------------------------------------
 
 def _rows(mq, torch, x, u, s):
