@@ -548,10 +548,11 @@ minq_status minq_kv4_attend(const float* q, size_t q_stride, const int32_t* q_st
  * order when a filter is on and by index otherwise; logits of -infinity or
  * NaN are never drawn, nor is one more than 745 T below the maximum (its w is 0
  * in f64), and a row of nothing but -infinity and NaN gives token 0. Greedy rows
- * (also top_k = 1) take minq_argmax's token. Weights are fixed-point integers
- * to 2^-28 of themselves and their sums exact, so a result depends on no order;
- * temperatures below 1e-12 of the largest |logit| are treated alike.
- * n <= 4194304, n_rows <= 2^20. */
+ * (also top_k = 1) take minq_argmax's token. Weights and their sums are integers,
+ * so a result depends on no order: 30 bits of a weight (28 to 26 above 2^20
+ * logits), summed in units of 2^-47 (shorter rows) to 2^-40 (4194304 logits) of
+ * the maximum's weight. Temperatures below 1e-12 of the maximum's magnitude are
+ * treated alike. n <= 4194304, n_rows <= 2^20. */
 minq_status minq_sample_rows(const float* logits, size_t row_stride, size_t n_rows, size_t n,
                              const float* temperature, const int32_t* top_k, const float* top_p,
                              const float* min_p, const float* uniforms, uint32_t* tokens,

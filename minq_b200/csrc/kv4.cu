@@ -14,10 +14,12 @@
 // each: two 16-byte loads, a maximum over the four lanes by two shuffles, and
 // one 4-byte word of codes per lane, the scale by the first; a warp covers
 // 256 consecutive values, so every global access of it is one contiguous run.
-// A value costs seven instructions (with roundf and an integer conversion each
-// it is twenty, and the write then waits for the arithmetic): the rounding half
+// A value's code costs seven instructions (with roundf and an integer conversion
+// each it is twenty, and the write then waits for the arithmetic): the rounding half
 // away from zero is two additions rounded towards zero, and four codes are
-// added up in one float before a single conversion. Measured at 8191 tokens of 8
+// added up in one float before a single conversion. The write runs 25 a value in
+// all: the other eighteen are the two divisions by multiplication, the slot's 64-bit
+// arithmetic, loads, shuffles and the loop, for a unit of eight values. Measured at 8191 tokens of 8
 // heads of 128 (77 MB each): write 19.7 us, 3.9 TB/s (24.4 us before), read 16.6 us,
 // 4.7 TB/s; a copy of as many bytes at the measured rate takes 12 us.
 #include <string>

@@ -23,7 +23,10 @@
 //     [2^10, 2^11), so the low part's smallest step is 2^-35 of that value;
 //   * p e is scaled by 2^10 / 2^floor(log2 max e), which follows the largest
 //     value scale seen, like the running maximum of the softmax; a step of its
-//     low part is 2^-34 of the largest p e.
+//     low part is 2^-34 of the largest p e, whichever block of dimensions has that:
+//     a block whose values are far smaller than another's is summed in its steps.
+//     (V's scales may lie anywhere from 2^-64 to 2^100. Below, the steps no longer
+//     shrink with them; above, weights under 2^-36 of the largest are flushed.)
 // Codes become exact signed f16 integers, two per instruction pair. (Left
 // unsigned, as the subnormals that their bits are, they cost half as much,
 // but the offset 8 sum q then costs the scores a digit.)
@@ -51,9 +54,9 @@
 // order, so results repeat bit for bit.
 //
 // What bounds it: 64 requests of 1 to 8192 positions (8 kv heads of 128, 306 MB,
-// 47 us at the measured copy rate) take 89 us, 3.4 TB/s: the two f16 parts and the
-// scales cost about 400 warp instructions per 16 positions of a kv head, and a
-// scheduler issues one in 0.67 of its cycles. 2 x 131071 positions of 2 kv heads
+// 47 us at the measured copy rate) take 89 us, 3.4 TB/s: the parts of q and p e, the
+// scales and the moves between lanes cost 460 warp instructions per 16 positions of a
+// kv head, and a scheduler issues one in 0.67 of its cycles. 2 x 131071 positions of 2 kv heads
 // of 64 take 31 us (41 MB), a third of it the join; 1 x 1000 positions 18 us, the
 // launches and the dependent loads.
 #include <limits.h>
@@ -949,6 +952,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 4 : 2)
 // behind them, always in a fixed order. An item of few pieces is summed by a warp
 // per column, the (item, column) pairs dealt out to the eight warps; one of many
 // by all eight warps, column by column. Columns are spread over gridDim.y blocks.
+// (At four blocks an SM head_dim 128 spills 80 bytes, 64 four.)
 constexpr int kKvJoinWarps = 8;
 constexpr int kKvJoinAlone = 32;  // pieces
 constexpr int kKvJoinRecs = 16;   // most pieces that a block looks through
@@ -1100,7 +1104,10 @@ KvPlan kv_plan(size_t n_req, size_t n_tokens, size_t n_heads, size_t n_kv, size_
   // G = 4, one token each: both parts of q in one tile of 8 columns 171, a tile a
   // part 256, two tiles a part 329. Two tiles a part or one: 12 to 16 heads to a
   // kv head, 32 x 4096, 52 / 60; 2, 3, 4, 8 tokens each of G = 4, 32 x 2048,
-  // 91 / 83, 97 / 105, 99 / 124, 144 / 200.
+  // 91 / 83, 97 / 105, 99 / 124, 144 / 200 (two tokens lose a little this way: the
+  // host has the step's totals only). Of the variants, <128, 1, false> spills 168 bytes
+  // at its 128 registers, <128, 1, true> 40; the ones of two tiles have 229 to 254 and
+  // spill nothing.
   // With kKvUmmaMin rows a request and more, the chunks are the tcgen05 kernel's and what
   // is left for the other one are mostly single tokens.
   const size_t gsz = G < (size_t)kKvUmmaRows ? G : kKvUmmaRows;

@@ -16,10 +16,18 @@
 //
 // Next to a border a draw is decided by digits that an f32 sum over a
 // vocabulary does not hold (with 100,000 even tokens, borders moved by 1e-7 of
-// the mass would change one draw in a hundred). So a weight is a fixed-point
-// integer, to 2^-28 of itself, and all sums are exact integers: the roundings
-// of 100,000 even tokens move a border by about 1e-6 of one token, and no
-// result depends on an order of summation. The exponent 256 log2 w comes from
+// the mass would change one draw in a hundred). So weights are integers and sums
+// of integers: no result depends on an order of summation, and the roundings of
+// 100,000 even tokens move a border by about 1e-6 of one token. What is rounded:
+//   * a weight has 30 bits in its bucket's unit (within 2^-28 of itself; from
+//     2^20 logits on 28 to 26 bits, cut, so that a CTA's sums fit 32);
+//   * sums over buckets are in units of 2^-b of the maximum's weight, b = 62 -
+//     ceil(log2 n), at most 47 (44 at 151936 logits, 40 at 4194304). A weight below
+//     2^(28 - b) has fewer than 28 bits there, one below 2^-b none;
+//   * the histogram cuts a bucket's sum once to that unit and a list each token, so
+//     the two may differ by a unit a token: at most n units, 2^-26 of the maximum's
+//     weight at 151936 logits and 2^-18 at 4194304.
+// The exponent 256 log2 w comes from
 // one f64 FMA whose addend leaves 24 fractional bits; 2^(a/256) is the
 // table-driven exponential (Tang 1989), a table of 256 steps and a polynomial
 // of degree 3 for the rest, in f32 and integers.
