@@ -521,7 +521,8 @@ minq_status minq_kv4_read(const void* k_pages, const void* v_pages, size_t n_pag
  * nothing is zero; positions in a page whose id is outside the pool, or past
  * the table row, are not seen; rows behind q_start[n_req] are left as they
  * were, and so are those of a request whose run of tokens is not inside
- * [0, n_tokens]. Any n_req <= 8192, n_tokens <= 2^24, n_tokens * n_heads < 2^31,
+ * [0, n_tokens]. Accuracy is f32's while V's block scales lie in 2^-64..2^100 (or
+ * are 0). Any n_req <= 8192, n_tokens <= 2^24, n_tokens * n_heads < 2^31,
  * n_heads a multiple of n_kv, head_dim a multiple of 32 up to 256. `workspace`
  * (16-byte aligned) holds minq_kv4_attend_workspace_bytes(...) bytes, needs no
  * initial value, and

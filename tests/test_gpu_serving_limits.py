@@ -96,6 +96,24 @@ def test_attend_keeps_what_is_not_a_number(mq, torch, nh, nkv, hd, lens, new):
     assert torch.isnan(got[:start[1]]).all() and torch.isfinite(got[start[1]:]).all()
 
 
+@pytest.mark.parametrize("nh,nkv,hd,new", [(8, 2, 64, 1), (8, 2, 128, 3), (16, 1, 128, 1), (8, 2, 128, 70),
+                                           (4, 2, 96, 2)])
+@pytest.mark.parametrize("kg,qg,vg", [(1.0, 1.0, 1e-17), (1.0, 1.0, 1e28), (1e-20, 1e20, 1.0),
+                                      (1e18, 1e-18, 1e-10), (1e-30, 1.0, 1.0)])
+def test_attend_over_the_range_of_sizes(mq, torch, nh, nkv, hd, new, kg, qg, vg):
+    """Keys, queries and values far from 1: the bound is relative to them."""
+    lens, page = [90, 700], 16
+    kp, vp, table, kv, vv = _fill(mq, torch, 5, lens, nkv, hd, page)
+    every = torch.arange(kv.shape[0], device="cuda")
+    mq.kv4_write((kv * kg).float(), (vv * vg).float(), every, kp, vp)
+    k, v = mq.kv4_read(every, kp, vp)
+    start = [0, new, 2 * new]
+    q = torch.randn(2 * new, nh, hd, device="cuda") * qg
+    got = mq.kv4_attend(q, dev(torch, start), dev(torch, lens), table, kp, vp)
+    want, tol = _reference(torch, q, start, lens, table, page, k.double(), v.double(), hd ** -0.5)
+    _check(torch, got / vg, want / vg, tol / vg)
+
+
 @pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (14, 2, 64)])
 @pytest.mark.parametrize("page", [16, 64])
 def test_attend_chunks_whose_maximum_moves_within_a_tile(mq, torch, nh, nkv, hd, page):
